@@ -1,0 +1,119 @@
+"""ctypes binding of drloco_amd/csrc/libdrloco_learner.so (the C-ABI in include/drloco_learner.h): the learner's operators,
+wrapped by drloco_amd.memory and drloco_amd.muon.
+
+A library of its own next to libdrloco_hip.so: its kernels need neither the step kernels' compiler flags nor their two code
+objects.  There is no CPU fallback: the functions refuse tensors that are not on a HIP device."""
+import ctypes as C
+import os
+import subprocess
+
+import torch
+
+from . import lib
+
+CSRC = os.path.join(lib.CSRC, 'learner')
+LIB_PATH = os.path.join(lib.CSRC, 'libdrloco_learner.so')
+ABI_VERSION = 1
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # DL_F32, DL_BF16, DL_F16
+MARK = 16                                                                 # DL_MEMORY_MARK
+# hipcc turns pairs of float operations into packed ones by itself; some forms of those are not trusted on this hardware
+EXTRA_FLAGS = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
+
+_I64, _I32, _P = C.c_int64, C.c_int32, C.c_void_p
+
+
+class MemoryShape(C.Structure):
+    """dl_memory_shape"""
+    _fields_ = [(n, _I64) for n in ('T', 'N', 'D', 'x_t', 'x_n', 'gate_t', 'gate_n', 'starts_t', 'starts_n', 'grad_t', 'grad_n')] + [('dtype', _I32), ('reserved', _I32)]
+
+
+_SIGNATURES = {
+    # name: (restype, argtypes)       -- every symbol include/drloco_learner.h declares
+    'dl_learner_last_error': (C.c_char_p, []),
+    'dl_learner_abi_version': (C.c_int, []),
+    'dl_memory_workspace_bytes': (_I64, [C.POINTER(MemoryShape)]),
+    'dl_memory_forward': (C.c_int, [C.POINTER(MemoryShape), _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    'dl_memory_backward': (C.c_int, [C.POINTER(MemoryShape), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
+    'dl_memory_step': (C.c_int, [C.POINTER(MemoryShape), _P, _P, _P, _P, _P, _P, _P]),
+}
+
+_lib = None
+
+
+def _sources():
+    return [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith(('.hip', '.hpp'))] + [os.path.join(lib.INCLUDE, 'drloco_learner.h')]
+
+
+def build(force=False, verbose=False):
+    """hipcc --offload-arch=gfx950 of the learner's kernels into an in-tree shared library."""
+    if not force and os.path.exists(LIB_PATH) and all(os.path.getmtime(s) <= os.path.getmtime(LIB_PATH) for s in _sources()):
+        return LIB_PATH
+    hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
+    cmd = [hipcc, '--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-shared', '-Wno-unused-command-line-argument',
+           '-ffile-prefix-map=' + os.path.dirname(lib.INCLUDE) + '=.', '-I' + lib.INCLUDE, '-I' + CSRC] + EXTRA_FLAGS + [os.path.join(CSRC, 'dl_learner.hip'), '-o', LIB_PATH]
+    if verbose:
+        print(' '.join(cmd))
+    subprocess.check_call(cmd)
+    return LIB_PATH
+
+
+def load():
+    """Load the library; raises DrlocoError if it has not been built."""
+    global _lib
+    if _lib is None:
+        if not os.path.exists(LIB_PATH):
+            raise lib.DrlocoError(f'{LIB_PATH} is missing: run `python -c "import __graft_entry__ as g; g.build()"` '
+                                  '(hipcc --offload-arch=gfx950); there is no CPU fallback')
+        so = C.CDLL(LIB_PATH)
+        for name, (res, args) in _SIGNATURES.items():
+            fn = getattr(so, name)
+            fn.restype, fn.argtypes = res, args
+        if so.dl_learner_abi_version() != ABI_VERSION:
+            raise lib.DrlocoError(f'ABI version mismatch between drloco_amd/learner_lib.py and {os.path.basename(LIB_PATH)}')
+        _lib = so
+    return _lib
+
+
+def check(rc):
+    """rc of a call, or the DrlocoError of a negative one."""
+    if rc < 0:
+        raise lib.DrlocoError(f'drloco_learner error {rc}: {load().dl_learner_last_error().decode()}')
+    return rc
+
+
+class _Here:
+    """Nothing to change: the tensors' device is the current one."""
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *_):
+        return False
+
+
+_HERE = _Here()
+
+
+def on(device):
+    """Context in which `device` is the current one (work goes to ITS current stream)."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def require_device(name, *tensors):
+    """All of `tensors` (None: skipped) on one HIP device, or ValueError / DrlocoError."""
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not torch.is_tensor(t):
+            raise TypeError(f'{name}: expected tensors, got {type(t).__name__}')
+        if t.device.type != 'cuda':
+            raise lib.DrlocoError(f'{name}: needs tensors on a HIP device, got one on {t.device} (there is no CPU fallback)')
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise ValueError(f'{name}: tensors on {device} and on {t.device}')
+    return device
