@@ -6,6 +6,7 @@
 
 #include "drloco_learner.h"
 #include "dl_memory.hpp"
+#include "dl_orth.hpp"
 
 namespace {
 
@@ -88,6 +89,75 @@ template <typename F> void with_type(int dtype, F&& f) {
     if (dtype == DL_F32) f(float{}); else if (dtype == DL_BF16) f(__bf16{}); else f(_Float16{});
 }
 
+// ---- orthogonalised updates ----
+const char* orth_shape_error(const dl_orth_shape* s) {
+    if (!s) return "shape must not be NULL";
+    for (int t : {s->grad_type, s->weight_type, s->out_type})
+        if (t != DL_F32 && t != DL_BF16 && t != DL_F16) return "unknown type";
+    if (s->reserved != 0) return "reserved must be 0";
+    if (s->batch < 0 || s->rows < 0 || s->cols < 0) return "batch, rows and cols must not be negative";
+    if (s->batch > 65535 || s->rows > (1 << 20) || s->cols > (1 << 20)) return "more than 65535 matrices, or a side above 2^20";
+    if (s->rows * s->cols > ((int64_t)1 << 32)) return "a matrix of more than 2^32 elements";
+    if (s->steps < 1 || s->steps > 100) return "steps must be 1 .. 100";
+    for (int64_t st : {s->grad_b, s->grad_r, s->momentum_b, s->momentum_r, s->momentum_out_b, s->momentum_out_r, s->weight_b, s->weight_r, s->out_b, s->out_r})
+        if (st < 0) return "negative strides";
+    return nullptr;
+}
+
+struct orth_form {
+    dlo::plan p;
+    int tile;
+    bool turned;
+    int64_t x_bytes, a_bytes, bytes;          // of the whole batch; the workspace: partials, XR, XC, XC', A, Q
+};
+
+orth_form orth_plan(const dl_orth_shape* s) {
+    orth_form f;
+    f.turned = s->rows > s->cols;
+    f.p.m = (int32_t)std::min(s->rows, s->cols);
+    f.p.n = (int32_t)std::max(s->rows, s->cols);
+    const int64_t big = s->batch * ceil_div(f.p.m, 128) * ceil_div(f.p.n, 128);
+    f.tile = big >= 128 ? 128 : 64;
+    f.p.mp = (int32_t)(ceil_div(f.p.m, f.tile) * f.tile);
+    f.p.np = (int32_t)(ceil_div(f.p.n, f.tile) * f.tile);
+    f.p.x_size = (int64_t)f.p.mp * f.p.np * 2;
+    f.p.a_size = (int64_t)f.p.mp * f.p.mp * 2;
+    f.p.partials = (int32_t)std::min<int64_t>(256, ceil_div(s->rows * s->cols, 4096));
+    f.x_bytes = s->batch * f.p.x_size * 2;
+    f.a_bytes = s->batch * f.p.a_size * 2;
+    f.bytes = ceil_div(s->batch * f.p.partials * 8, 256) * 256 + 3 * f.x_bytes + 2 * f.a_bytes;
+    return f;
+}
+
+template <int TILE, int MODE> void launch_product(const dlo::product& p, int64_t tiles, int64_t batch, hipStream_t st) {
+    constexpr int W = TILE / 2;
+    dlo::k_orth_product<TILE, TILE, W, W, MODE><<<dim3((unsigned)tiles, 1, (unsigned)batch), 256, 0, st>>>(p);
+}
+
+template <int TILE> void launch_steps(const dl_orth_shape* s, const orth_form& f, dlo::product last, char* work, hipStream_t st) {
+    _Float16* xr = (_Float16*)work;
+    _Float16* xc[2] = {(_Float16*)(work + f.x_bytes), (_Float16*)(work + 2 * f.x_bytes)};
+    _Float16* A = (_Float16*)(work + 3 * f.x_bytes);
+    _Float16* Q = (_Float16*)(work + 3 * f.x_bytes + f.a_bytes);
+    const int64_t ti = f.p.mp / TILE, tj = f.p.np / TILE, tri = ti * (ti + 1) / 2;
+    const int32_t km = f.p.mp / 32, kn = f.p.np / 32;
+    for (int k = 0; k < s->steps; ++k) {
+        dlo::product p = last;
+        p.P = p.Q = xr; p.P_b = p.Q_b = f.p.x_size; p.kb = kn;
+        p.out0 = A; p.out0_b = f.p.a_size; p.out0_kb = km;
+        launch_product<TILE, dlo::GRAM>(p, tri, s->batch, st);
+        p.P = p.Q = A; p.P_b = p.Q_b = f.p.a_size; p.kb = km;
+        p.A = A; p.out0 = Q;
+        launch_product<TILE, dlo::POLY>(p, tri, s->batch, st);
+        p.P = Q; p.Q = xc[k & 1]; p.Q_b = f.p.x_size;
+        p.tiles_i = (int32_t)ti; p.tiles_j = (int32_t)tj;
+        p.out0 = xr; p.out0_b = f.p.x_size; p.out0_kb = kn;
+        p.out1 = xc[(k + 1) & 1]; p.out1_b = f.p.x_size; p.out1_kb = km;
+        if (k + 1 < s->steps) launch_product<TILE, dlo::STEP>(p, ti * tj, s->batch, st);
+        else launch_product<TILE, dlo::LAST>(p, ti * tj, s->batch, st);
+    }
+}
+
 }  // namespace
 
 extern "C" {
@@ -160,6 +230,36 @@ int dl_memory_step(const dl_memory_shape* s, const void* x, const void* gate, co
         dlm::k_memory_step<E, V_><<<(unsigned)blocks, 256, 0, (hipStream_t)stream>>>(s->N, s->D, s->x_n, s->gate_n, s->starts_n, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out);
     }); });
     return launched("dl_memory_step");
+}
+
+int64_t dl_orth_workspace_bytes(const dl_orth_shape* s) {
+    if (const char* e = orth_shape_error(s)) return fail(DL_E_INVAL, e);
+    if (s->batch == 0 || s->rows == 0 || s->cols == 0) return 0;
+    return orth_plan(s).bytes;
+}
+
+int dl_orth_update(const dl_orth_shape* s, const void* grad, const float* momentum, float* momentum_out, const void* weight, void* out, void* workspace, void* stream) {
+    if (const char* e = orth_shape_error(s)) return fail(DL_E_INVAL, e);
+    if (s->batch == 0 || s->rows == 0 || s->cols == 0) return DL_OK;
+    if (!grad || !out || !workspace) return fail(DL_E_INVAL, "dl_orth_update: grad, out and workspace must not be NULL");
+    if (!momentum != !momentum_out) return fail(DL_E_INVAL, "dl_orth_update: momentum and momentum_out must be given together");
+    if (!aligned(workspace, 16)) return fail(DL_E_INVAL, "dl_orth_update: workspace must be aligned to 16 bytes");
+    const orth_form f = orth_plan(s);
+    hipStream_t st = (hipStream_t)stream;
+    double* partials = (double*)workspace;
+    char* work = (char*)workspace + ceil_div(s->batch * f.p.partials * 8, 256) * 256;
+    const dlo::source src{grad, s->grad_type, momentum, momentum_out, (float)s->beta, s->nesterov, s->grad_b, s->grad_r, s->momentum_b, s->momentum_r, s->momentum_out_b, s->momentum_out_r};
+    dlo::k_orth_norm<<<dim3((unsigned)f.p.partials, (unsigned)s->batch), 256, 0, st>>>(src, s->rows, s->cols, partials);
+    dlo::k_orth_load<<<dim3((unsigned)(f.p.np / 32), (unsigned)(f.p.mp / 32), (unsigned)s->batch), 256, 0, st>>>(src, f.p, f.turned, partials, (_Float16*)work, (_Float16*)(work + f.x_bytes));
+    dlo::product p{};
+    p.a = (float)s->a; p.b = (float)s->b; p.c = (float)s->c;
+    p.out = out; p.w = weight; p.out_type = s->out_type; p.w_type = s->weight_type;
+    p.out_at = f.turned ? dlo::matrix{s->out_b, 1, s->out_r} : dlo::matrix{s->out_b, s->out_r, 1};
+    p.w_at = f.turned ? dlo::matrix{s->weight_b, 1, s->weight_r} : dlo::matrix{s->weight_b, s->weight_r, 1};
+    p.keep = (float)s->weight_keep; p.gain = (float)s->gain;
+    p.m = f.p.m; p.n = f.p.n;
+    if (f.tile == 128) launch_steps<128>(s, f, p, work, st); else launch_steps<64>(s, f, p, work, st);
+    return launched("dl_orth_update");
 }
 
 }  // extern "C"

@@ -1,0 +1,271 @@
+// dl_orth.hpp -- orthogonalisation of an update by Newton-Schulz products, and the weight update built on it.
+//
+//     X = G / |G|_F (from the short side: X is [m, n], m <= n);  repeat:  A = X X',  Q = a I + b A + c A A,  X = Q X
+//
+// Bound by the matrix cores.  A product of 32-bit matrices on them would run at a sixteenth of the 16-bit rate, and one rounding of X
+// to 16 bits is amplified by up to a^steps (485 for five steps) in the directions of small singular values.  So every matrix is
+// held as the sum of two float16 planes, hi + lo = 22 bits, and a product is three 16-bit ones accumulated in 32 bits,
+// hi hi + hi lo + lo hi (what is left out is below 2^-22): the splitting of Ootomo and Yokota (2022).  All entries are at most
+// about one, so they are held times 2^10, which keeps lo clear of float16's smallest numbers.
+// A and Q are symmetric: only their tiles on and below the diagonal are computed, and written to both places.
+//
+// Layout.  A matrix that is an operand lies in memory as the matrix cores read it: for 16 rows and 32 columns k a "fragment" of
+// [plane][lane][8] float16, lane = row + 16 * (k / 8), 2 KB; fragments of a row block follow each other along k.  Copies to LDS and
+// reads from it are then straight runs of 16 bytes per lane without bank conflicts, and every product has the form
+// C[i][j] = sum_k P[i][k] Q[j][k].  X is kept in both orientations (XR: rows i, XC: rows j) because A needs one and Q X the other.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace dlo {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float float4_ __attribute__((ext_vector_type(4)));
+
+constexpr float SCALE = 1024.0f;
+constexpr int FRAG = 1024;            // float16 of a fragment: two planes of 64 lanes x 8
+
+// Where a matrix [batch][rows][cols] of the caller lies, seen from the short side: element (i, j), i < m, j < n, at i * si + j * sj.
+struct matrix {
+    int64_t b, si, sj;
+};
+
+struct plan {
+    int32_t m, n, mp, np;             // short and long side, and what they are padded to
+    int64_t x_size, a_size;           // float16 of one X, one A
+    int32_t partials;
+};
+
+__device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
+    hi = (_Float16)v;
+    lo = (_Float16)(v - (float)hi);
+}
+
+template <typename E> __device__ __forceinline__ float load_as(const void* p, int64_t i) { return (float)((const E*)p)[i]; }
+__device__ __forceinline__ float load_elem(const void* p, int dtype, int64_t i) {
+    return dtype == 0 ? load_as<float>(p, i) : dtype == 1 ? load_as<__bf16>(p, i) : load_as<_Float16>(p, i);
+}
+__device__ __forceinline__ void store_elem(void* p, int dtype, int64_t i, float v) {
+    if (dtype == 0) ((float*)p)[i] = v;
+    else if (dtype == 1) ((__bf16*)p)[i] = (__bf16)v;
+    else ((_Float16*)p)[i] = (_Float16)v;
+}
+
+// ---- the sum of squares, in 64 bits (a float32 gradient of 1e30 or of 1e-30 is as good as another) --------------------------------
+// With a momentum: m' = beta m + g first, and the matrix is g + beta m' (nesterov) or m'.  rows x cols as the caller sees them.
+struct source {
+    const void* g; int dtype;
+    const float* m; float* m_out;     // NULL: no momentum
+    float beta; int nesterov;
+    int64_t g_b, g_r, m_b, m_r, o_b, o_r;          // strides of g, m, m_out: matrix, row
+};
+
+__global__ __launch_bounds__(256) void k_orth_norm(source s, int64_t rows, int64_t cols, double* __restrict__ partials) {
+    const int64_t b = blockIdx.y;
+    const int64_t all = rows * cols, per = (all + gridDim.x - 1) / gridDim.x;
+    const int64_t lo = (int64_t)blockIdx.x * per, hi = min(lo + per, all);
+    double sum = 0.0;
+    for (int64_t e = lo + threadIdx.x; e < hi; e += 256) {
+        const int64_t r = e / cols, c = e - r * cols;
+        float u = load_elem(s.g, s.dtype, b * s.g_b + r * s.g_r + c);
+        if (s.m) {
+            const float v = fmaf(s.beta, s.m[b * s.m_b + r * s.m_r + c], u);
+            s.m_out[b * s.o_b + r * s.o_r + c] = v;
+            u = s.nesterov ? fmaf(s.beta, v, u) : v;
+        }
+        sum += (double)u * u;
+    }
+    __shared__ double part[4];
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) partials[b * gridDim.x + blockIdx.x] = part[0] + part[1] + part[2] + part[3];
+}
+
+// ---- X = G / |G| into both orientations: one workgroup per 32 x 32 ---------------------------------------------------------------
+__global__ __launch_bounds__(256) void k_orth_load(source s, plan p, int turned, const double* __restrict__ partials, _Float16* __restrict__ xr, _Float16* __restrict__ xc) {
+    const int b = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    double sum = 0.0;
+    for (int k = lane; k < p.partials; k += 64) sum += partials[(int64_t)b * p.partials + k];
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    const double inv = sum != 0.0 ? (double)SCALE / sqrt(sum) : 0.0;          // (NaN != 0)
+    __shared__ float tile[32][33];
+    const int i0 = blockIdx.y * 32, j0 = blockIdx.x * 32;
+    for (int e = threadIdx.x; e < 1024; e += 256) {
+        const int fast = e & 31, slow = e >> 5;
+        const int i = turned ? fast : slow, j = turned ? slow : fast;
+        float u = 0.0f;
+        if (i0 + i < p.m && j0 + j < p.n) {
+            const int64_t r = turned ? j0 + j : i0 + i, c = turned ? i0 + i : j0 + j;
+            u = load_elem(s.g, s.dtype, b * s.g_b + r * s.g_r + c);
+            if (s.m) {
+                const float v = s.m_out[b * s.o_b + r * s.o_r + c];
+                u = s.nesterov ? fmaf(s.beta, v, u) : v;
+            }
+            u = (float)(u * inv);
+        }
+        tile[i][j] = u;
+    }
+    __syncthreads();
+    const int row = (wave & 1) * 16 + (lane & 15), k = (lane >> 4) * 8;
+    half8 hi, lo;
+    const bool c_side = wave >= 2;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) { _Float16 h, l; split(c_side ? tile[k + q][row] : tile[row][k + q], h, l); hi[q] = h; lo[q] = l; }
+    const int64_t block = (c_side ? j0 : i0) / 16 + (wave & 1), kb = (c_side ? i0 : j0) / 32, kbs = (c_side ? p.mp : p.np) / 32;
+    _Float16* to = (c_side ? xc : xr) + b * p.x_size + (block * kbs + kb) * FRAG + lane * 8;
+    *(half8*)to = hi;
+    *(half8*)(to + 512) = lo;
+}
+
+// ---- the products ----------------------------------------------------------------------------------------------------------------
+enum { GRAM, POLY, STEP, LAST };      // A = XR XR';  Q = aI + bA + cAA;  X = Q X as the next operand;  X = Q X as the result
+
+struct product {
+    const _Float16* P; const _Float16* Q;          // operands, [rows / 16][kb][FRAG]
+    int64_t P_b, Q_b;
+    int32_t kb;                                    // steps of 32 along k
+    int32_t tiles_i, tiles_j;
+    _Float16* out0; int64_t out0_b, out0_kb;       // GRAM, POLY: the symmetric result;  STEP: XR
+    _Float16* out1; int64_t out1_b, out1_kb;       // STEP: XC
+    const _Float16* A;                             // POLY: as out0
+    float a, b, c;
+    // LAST: out = keep * w + gain * X
+    void* out; const void* w; int out_type, w_type;
+    matrix out_at, w_at;
+    float keep, gain;
+    int32_t m, n;
+};
+
+template <int BM, int BN, int WM, int WN, int MODE>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void k_orth_product(product p) {
+    constexpr int WAVES = (BM / WM) * (BN / WN), TM = WM / 16, TN = WN / 16;
+    constexpr int ROWS = BM / 16 + BN / 16;                    // fragments of a step
+    constexpr int PITCH = BN + 4;
+    constexpr int STAGE = ROWS * FRAG * 2;                     // bytes
+    constexpr int BYTES = 2 * STAGE > BM * PITCH * 4 ? 2 * STAGE : BM * PITCH * 4;
+    __shared__ __attribute__((aligned(16))) char lds[BYTES];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int64_t b = blockIdx.z;
+    int ti, tj;
+    if (MODE == GRAM || MODE == POLY) {                        // the tiles on and below the diagonal, row by row
+        const int t = blockIdx.x;
+        ti = (int)((sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
+        while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
+        while (ti * (ti + 1) / 2 > t) --ti;
+        tj = t - ti * (ti + 1) / 2;
+    } else {
+        ti = blockIdx.x % p.tiles_i; tj = blockIdx.x / p.tiles_i;
+    }
+    const _Float16* P = p.P + b * p.P_b + (int64_t)ti * (BM / 16) * p.kb * FRAG;
+    const _Float16* Q = p.Q + b * p.Q_b + (int64_t)tj * (BN / 16) * p.kb * FRAG;
+
+    // a step's fragments: one instruction of a wave moves 1 KB, a plane of a fragment
+    auto fetch = [&](int k, int stage) {
+#pragma unroll
+        for (int f = 0; f < ROWS * 2 / WAVES; ++f) {
+            const int piece = f * WAVES + wave, r = piece >> 1, plane = piece & 1;
+            const _Float16* from = (r < BM / 16 ? P + ((int64_t)r * p.kb + k) * FRAG : Q + ((int64_t)(r - BM / 16) * p.kb + k) * FRAG) + plane * 512 + lane * 8;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)(lds + stage * STAGE + piece * 1024), 16, 0, 0);
+        }
+    };
+    static_assert(ROWS * 2 % WAVES == 0, "every wave moves the same number of pieces");
+
+    float4_ acc[TM][TN] = {};
+    const int wi = wave / (BN / WN), wj = wave % (BN / WN);
+    fetch(0, 0);
+    for (int k = 0; k < p.kb; ++k) {
+        // this wave's copies have arrived, and with the barrier everyone's; everyone is also done reading the other stage
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (k + 1 < p.kb) fetch(k + 1, (k + 1) & 1);
+        const char* stage = lds + (k & 1) * STAGE;
+        half8 ph[TM], pl[TM], qh[TN], ql[TN];
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const char* f = stage + (wi * TM + i) * 2048 + lane * 16;
+            ph[i] = *(const half8*)f; pl[i] = *(const half8*)(f + 1024);
+        }
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const char* f = stage + (BM / 16 + wj * TN + j) * 2048 + lane * 16;
+            qh[j] = *(const half8*)f; ql[j] = *(const half8*)(f + 1024);
+        }
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[i], ql[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[i], qh[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[i], qh[j], acc[i][j], 0, 0, 0);
+    }
+    __syncthreads();
+    // the tile through LDS, so that both orientations leave in whole fragments.  A lane holds rows 4 (lane / 16) + r of column lane % 16.
+    float* tile = (float*)lds;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) tile[(wi * WM + i * 16 + (lane >> 4) * 4 + r) * PITCH + wj * WN + j * 16 + (lane & 15)] = acc[i][j][r];
+    __syncthreads();
+    const int i0 = ti * BM, j0 = tj * BN, row = lane & 15, k8 = (lane >> 4) * 8;
+    if (MODE == LAST) {
+        constexpr int THREADS = WAVES * 64;
+        const bool down = p.out_at.si == 1 && p.out_at.sj != 1;          // the short side runs along the caller's rows
+        for (int e = threadIdx.x; e < BM * BN; e += THREADS) {
+            const int i = down ? e % BM : e / BN, j = down ? e / BM : e % BN;
+            if (i0 + i < p.m && j0 + j < p.n) {
+                float v = tile[i * PITCH + j] * (p.gain / (SCALE * SCALE));
+                if (p.w) v = fmaf(p.keep, load_elem(p.w, p.w_type, b * p.w_at.b + (i0 + i) * p.w_at.si + (j0 + j) * p.w_at.sj), v);
+                store_elem(p.out, p.out_type, b * p.out_at.b + (i0 + i) * p.out_at.si + (j0 + j) * p.out_at.sj, v);
+            }
+        }
+        return;
+    }
+    // rows i, k along j
+    for (int f = wave; f < (BM / 16) * (BN / 32); f += WAVES) {
+        const int ri = f / (BN / 32), kj = f % (BN / 32);
+        const int64_t at = (((int64_t)(i0 / 16 + ri)) * p.out0_kb + j0 / 32 + kj) * FRAG + lane * 8;
+        float* src = tile + (ri * 16 + row) * PITCH + kj * 32 + k8;
+        half8 hi, lo, ah, al;
+        if (MODE == POLY) { const _Float16* A = p.A + b * p.out0_b + at; ah = *(const half8*)A; al = *(const half8*)(A + 512); }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            float v = src[q] * (1.0f / SCALE);
+            if (MODE == POLY) {
+                v = fmaf(p.c, v, p.b * ((float)ah[q] + (float)al[q]));
+                if (i0 + ri * 16 + row == j0 + kj * 32 + k8 + q) v += p.a * SCALE;
+                src[q] = v * SCALE;           // for the other orientation
+            }
+            _Float16 h, l; split(v, h, l); hi[q] = h; lo[q] = l;
+        }
+        _Float16* to = p.out0 + b * p.out0_b + at;
+        *(half8*)to = hi; *(half8*)(to + 512) = lo;
+    }
+    if (MODE == STEP || ti != tj) {
+        if (MODE == POLY) __syncthreads();
+        // rows j, k along i: the mirror image of a symmetric result, or X's other orientation
+        _Float16* out = MODE == STEP ? p.out1 + b * p.out1_b : p.out0 + b * p.out0_b;
+        const int64_t kbs = MODE == STEP ? p.out1_kb : p.out0_kb;
+        for (int f = wave; f < (BN / 16) * (BM / 32); f += WAVES) {
+            const int rj = f / (BM / 32), ki = f % (BM / 32);
+            half8 hi, lo;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                _Float16 h, l;
+                split(tile[(ki * 32 + k8 + q) * PITCH + rj * 16 + row] * (1.0f / SCALE), h, l);
+                hi[q] = h; lo[q] = l;
+            }
+            _Float16* to = out + ((int64_t)(j0 / 16 + rj) * kbs + i0 / 32 + ki) * FRAG + lane * 8;
+            *(half8*)to = hi; *(half8*)(to + 512) = lo;
+        }
+    }
+}
+
+}  // namespace dlo

@@ -27,6 +27,12 @@ class MemoryShape(C.Structure):
     _fields_ = [(n, _I64) for n in ('T', 'N', 'D', 'x_t', 'x_n', 'gate_t', 'gate_n', 'starts_t', 'starts_n', 'grad_t', 'grad_n')] + [('dtype', _I32), ('reserved', _I32)]
 
 
+class OrthShape(C.Structure):
+    """dl_orth_shape"""
+    _fields_ = [(n, _I64) for n in ('batch', 'rows', 'cols', 'grad_b', 'grad_r', 'momentum_b', 'momentum_r', 'momentum_out_b', 'momentum_out_r', 'weight_b', 'weight_r', 'out_b', 'out_r')] + \
+               [(n, C.c_double) for n in ('a', 'b', 'c', 'beta', 'weight_keep', 'gain')] + [(n, _I32) for n in ('steps', 'nesterov', 'grad_type', 'weight_type', 'out_type', 'reserved')]
+
+
 _SIGNATURES = {
     # name: (restype, argtypes)       -- every symbol include/drloco_learner.h declares
     'dl_learner_last_error': (C.c_char_p, []),
@@ -35,6 +41,8 @@ _SIGNATURES = {
     'dl_memory_forward': (C.c_int, [C.POINTER(MemoryShape), _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     'dl_memory_backward': (C.c_int, [C.POINTER(MemoryShape), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     'dl_memory_step': (C.c_int, [C.POINTER(MemoryShape), _P, _P, _P, _P, _P, _P, _P]),
+    'dl_orth_workspace_bytes': (_I64, [C.POINTER(OrthShape)]),
+    'dl_orth_update': (C.c_int, [C.POINTER(OrthShape), _P, _P, _P, _P, _P, _P, _P]),
 }
 
 _lib = None

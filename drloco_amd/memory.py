@@ -174,4 +174,5 @@ def gated_memory_step(x, gate, state, starts=None, out=None, state_out=None):
     s.dtype = ll.DTYPES[x.dtype]
     with ll.on(x.device):
         ll.check(ll.load().dl_memory_step(_shape_ref(s), x.data_ptr(), gate.data_ptr(), _ptr(starts), state.data_ptr(), out.data_ptr(), state_out.data_ptr(), ll.stream(x.device)))
+    torch.autograd.graph.increment_version((out, state_out))          # the library wrote behind torch's back
     return out, state_out

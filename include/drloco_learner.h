@@ -79,6 +79,39 @@ int dl_memory_backward(const dl_memory_shape* shape, const void* x, const void* 
 int dl_memory_step(const dl_memory_shape* shape, const void* x, const void* gate, const uint8_t* starts,
                    const float* state, void* h, float* state_out, void* stream);
 
+/* ---- orthogonalised updates --------------------------------------------------------------------------------------
+ * The orthogonal factor of a gradient, approached by `steps` Newton-Schulz products (the update of the Muon optimiser, Jordan
+ * et al. 2024), and the weight update built on it, for `batch` matrices [rows, cols]:
+ *
+ *     U = grad                                            without momentum (momentum == NULL)
+ *     M' = beta M + grad,  U = grad + beta M' | M'        with momentum: nesterov | not;  M' goes to momentum_out
+ *     X = U / |U|_F   (zeros stay zeros);   steps times:  A = X X',  X = (a I + b A + c A A) X      from the short side
+ *     out = weight_keep * weight + gain * X               weight == NULL: out = gain * X
+ *
+ * Products are exact to about 2^-22 of their operands and summed in 32 bits, norms in 64; out is rounded once.  A NaN or an
+ * infinity anywhere in U makes the whole of its matrix NaN.  The coefficients have to keep every iterate's entries below
+ * 60 in size (those of the Muon optimiser, 3.4445 -4.7750 2.0315, and of the classic cubic, 1.5 -0.5 0, keep them
+ * below 1.3).  Strides are in elements: of a matrix in its batch and of a row; rows are contiguous. */
+typedef struct dl_orth_shape {
+    int64_t batch, rows, cols;
+    int64_t grad_b, grad_r;
+    int64_t momentum_b, momentum_r;          /* momentum, float */
+    int64_t momentum_out_b, momentum_out_r;
+    int64_t weight_b, weight_r;
+    int64_t out_b, out_r;
+    double a, b, c;                          /* coefficients of a step */
+    double beta, weight_keep, gain;
+    int32_t steps, nesterov;
+    int32_t grad_type, weight_type, out_type, reserved;
+} dl_orth_shape;
+
+/* Bytes of device workspace dl_orth_update needs for this shape, or a DL_E_ code. */
+int64_t dl_orth_workspace_bytes(const dl_orth_shape* shape);
+
+/* momentum_out may be momentum, out may be weight (in place, with the same strides) or grad; no other overlap. */
+int dl_orth_update(const dl_orth_shape* shape, const void* grad, const float* momentum, float* momentum_out,
+                   const void* weight, void* out, void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

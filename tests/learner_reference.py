@@ -37,3 +37,32 @@ def memory_backward(x, gate, starts, state, grad_h, grad_last):
         dg[t] = lam * (before - x[t]) * a[t] * s[t]
         lam = np.where(keep > 0, a[t] * lam, 0.0)
     return dx, dg, lam, most
+
+
+def orthogonal(g, steps=5, coefficients=(3.4445, -4.7750, 2.0315), trace=None):
+    """float64 [..., rows, cols]: `steps` Newton-Schulz steps from g / |g|.  trace: a list that takes |X|_F of every iterate."""
+    g = np.asarray(g, np.float64)
+    a, b, c = coefficients
+    out = np.empty_like(g)
+    for at in np.ndindex(g.shape[:-2]):
+        x = g[at]
+        turned = x.shape[0] > x.shape[1]
+        x = x.T if turned else x
+        norm = np.sqrt((x * x).sum())
+        x = x / norm if norm != 0 else x
+        for _ in range(steps):
+            if trace is not None:
+                trace.append(np.sqrt((x * x).sum()))
+            p = x @ x.T
+            x = a * x + (b * p + c * (p @ p)) @ x
+        out[at] = x.T if turned else x
+    return out
+
+
+def muon(w, g, m, lr, beta=0.95, nesterov=True, weight_decay=0.0, scale=None, **kw):
+    """(new weight, new momentum), float64"""
+    w, g, m = (np.asarray(t, np.float64) for t in (w, g, m))
+    m = beta * m + g
+    o = orthogonal(g + beta * m if nesterov else m, **kw)
+    scale = np.sqrt(max(1.0, w.shape[-2] / w.shape[-1])) if scale is None else scale
+    return (1 - lr * weight_decay) * w - lr * scale * o, m

@@ -1,0 +1,120 @@
+"""CPU side of the orthogonalised updates (drloco_amd.muon, dl_orth_update): refusals of the C and of the Python entry points, workspace
+sizes, the optimiser's bookkeeping.  Nothing here touches a device."""
+import ctypes as C
+import math
+import os
+
+import pytest
+import torch
+
+from drloco_amd import learner_lib as ll
+from drloco_amd import lib, muon
+
+
+@pytest.fixture(scope='module')
+def L():
+    if not os.path.exists(ll.LIB_PATH):
+        ll.build()
+    return ll.load()
+
+
+def shape(batch=1, rows=8, cols=16, **kw):
+    s = ll.OrthShape(batch=batch, rows=rows, cols=cols, a=3.0, b=-4.0, c=2.0, beta=0.9, weight_keep=1.0, gain=1.0, steps=5)
+    for n in ('grad', 'momentum', 'momentum_out', 'weight', 'out'):
+        setattr(s, n + '_b', rows * cols), setattr(s, n + '_r', cols)
+    for k, v in kw.items():
+        setattr(s, k, v)
+    return s
+
+
+BAD = [dict(grad_type=3), dict(weight_type=-1), dict(out_type=7), dict(reserved=1), dict(batch=-1), dict(rows=-1), dict(cols=-1), dict(batch=65536), dict(rows=(1 << 20) + 1), dict(cols=1 << 30),
+       dict(rows=1 << 20, cols=1 << 13), dict(steps=0), dict(steps=101), dict(steps=-5)] + [{f'{n}_{a}': -1} for n in ('grad', 'momentum', 'momentum_out', 'weight', 'out') for a in 'br']
+
+
+@pytest.mark.parametrize('bad', BAD, ids=str)
+def test_bad_shapes_are_refused(L, bad):
+    s, p = C.byref(shape(**bad)), 4096
+    assert L.dl_orth_workspace_bytes(s) == -1
+    assert L.dl_orth_update(s, p, None, None, None, p, p, None) == -1
+    assert len(L.dl_learner_last_error()) > 5
+
+
+def test_bad_pointers_are_refused(L):
+    s, p = C.byref(shape()), 4096
+    assert L.dl_orth_workspace_bytes(None) == -1
+    assert L.dl_orth_update(None, p, None, None, None, p, p, None) == -1
+    for k in (0, 4, 5):
+        a = [p, None, None, None, p, p, None]
+        a[k] = None
+        assert L.dl_orth_update(s, *a) == -1
+    assert L.dl_orth_update(s, p, p, None, None, p, p, None) == -1
+    assert L.dl_orth_update(s, p, None, p, None, p, p, None) == -1
+    assert L.dl_orth_update(s, p, None, None, None, p, p + 4, None) == -1
+
+
+def test_empty_shapes_are_done_at_once(L):
+    for kw in (dict(batch=0), dict(rows=0), dict(cols=0)):
+        s = C.byref(shape(**kw))
+        assert L.dl_orth_workspace_bytes(s) == 0 and L.dl_orth_update(s, None, None, None, None, None, None, None) == 0
+
+
+@pytest.mark.parametrize('batch,rows,cols', [(1, 1, 1), (1, 8, 512), (3, 512, 512), (1, 4096, 8192), (7, 1031, 4099)])
+def test_the_workspace_is_a_small_multiple_of_the_matrix(L, batch, rows, cols):
+    size = L.dl_orth_workspace_bytes(C.byref(shape(batch, rows, cols)))
+    up = lambda n: -(-n // 128) * 128
+    m, n = sorted((up(rows), up(cols)))
+    assert 0 < size <= batch * (3 * m * n * 4 + 2 * m * m * 4 + 2048) + 256
+
+
+z = lambda *s, dtype=torch.float32: torch.zeros(*s, dtype=dtype)
+
+
+@pytest.mark.parametrize('args,kw,error', [
+    ((z(8),), {}, ValueError), ((z(2, 2, dtype=torch.float64),), {}, TypeError), (([1.0],), {}, TypeError), ((z(2, 2), 0), {}, ValueError), ((z(2, 2), 101), {}, ValueError),
+    ((z(2, 2), 2.5), {}, ValueError), ((z(2, 2), 5, (1.0, 2.0)), {}, ValueError), ((z(2, 2), 5, (1.0, 2.0, math.inf)), {}, ValueError), ((z(2, 2),), {}, lib.DrlocoError),
+])
+def test_refusals_of_orthogonalise(args, kw, error):
+    with pytest.raises(error):
+        muon.orthogonalise(*args, **kw)
+
+
+@pytest.mark.parametrize('args,kw,error', [
+    ((z(4, 2), z(2, 4), z(4, 2)), {}, ValueError), ((z(4, 2), z(4, 2), z(4, 3)), {}, ValueError), ((z(4, 2), z(4, 2), z(4, 2, dtype=torch.bfloat16)), {}, TypeError),
+    ((z(4), z(4), z(4)), {}, ValueError), ((z(4, 2), z(4, 2), z(4, 2)), dict(steps=0), ValueError), ((z(4, 2), z(4, 2), z(4, 2)), {}, lib.DrlocoError),
+])
+def test_refusals_of_the_update(args, kw, error):
+    with pytest.raises(error):
+        muon.muon_update(*args, lr=0.1, **kw)
+
+
+def test_destinations_are_looked_at():
+    w, other = z(6, 4), z(7, 4)
+    ok = lambda t, aliases: muon._result('f', 'out', t, w, torch.float32, aliases)
+    assert ok(w, [(True, w)]) is w and ok(z(6, 4), [(False, w)]) is not None
+    for t, aliases in ((w, [(False, w)]), (other[1:], [(True, other[:6])]), (z(4, 6).t(), []), (z(6, 5), []), (z(6, 4, dtype=torch.float16), [])):
+        with pytest.raises(ValueError):
+            ok(t, aliases)
+
+
+def test_the_optimiser_refuses_what_is_not_a_matrix():
+    p = lambda *s, **kw: torch.nn.Parameter(z(*s, **kw))
+    for bad in (p(8), p(4, 4, dtype=torch.float64), torch.nn.Parameter(z(4, 6).t())):
+        with pytest.raises(ValueError):
+            muon.HipMuon([p(4, 4), bad])
+    for kw in (dict(lr=-1.0), dict(beta=1.0), dict(weight_decay=-0.1), dict(steps=0), dict(lr=math.nan)):
+        with pytest.raises(ValueError):
+            muon.HipMuon([p(4, 4)], **kw)
+    opt = muon.HipMuon([p(4, 4)])
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=[p(3)]))
+    assert len(opt.param_groups) == 1 and opt.step() is None          # (no gradients: nothing to do)
+
+
+def test_the_optimiser_state_round_trips_in_32_bits():
+    q = torch.nn.Parameter(z(4, 4, dtype=torch.bfloat16))
+    a, b = muon.HipMuon([q]), muon.HipMuon([q], lr=0.5)
+    a.state[q]['momentum'] = torch.full((4, 4), 1.0 + 2.0 ** -20)
+    b.load_state_dict(a.state_dict())
+    m = b.state[q]['momentum']
+    assert m.dtype == torch.float32 and torch.equal(m, a.state[q]['momentum']) and m.data_ptr() != a.state[q]['momentum'].data_ptr()
+    assert b.param_groups[0]['lr'] == 0.02
