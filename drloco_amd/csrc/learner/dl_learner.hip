@@ -33,57 +33,61 @@ const char* memory_shape_error(const dl_memory_shape* s) {
     if (s->dtype != DL_F32 && s->dtype != DL_BF16 && s->dtype != DL_F16) return "unknown dtype";
     if (s->reserved != 0) return "reserved must be 0";
     if (s->T < 0 || s->N < 0 || s->D < 0 || s->T > MAX_DIM || s->N > MAX_DIM || s->D > MAX_DIM) return "T, N and D must not be negative (nor above 2^40)";
+    if (s->T > (1 << 30)) return "more than 2^30 steps";
     if ((__int128)s->T * s->N * s->D > ((__int128)1 << 46)) return "more than 2^46 elements";
     for (int64_t st : {s->x_t, s->x_n, s->gate_t, s->gate_n, s->starts_t, s->starts_n, s->grad_t, s->grad_n})
         if (st < 0) return "negative strides";
+    // 64 walkers' rows are addressed with 32 bits
+    const int64_t walkers = std::min<int64_t>(s->N, s->D ? 256 / s->D + 2 : 1), far = (int64_t)1 << 29;
+    if (s->D > far) return "more than 2^29 channels";
+    if (walkers > 1 && (s->x_n >= far / walkers || s->gate_n >= far / walkers || s->grad_n >= far / walkers || s->D >= far / walkers)) return "walkers too far apart (2^29 elements over the 64 lanes of a wave): pass a time-major copy";
     return nullptr;
 }
 
 // The form of a launch: V columns per lane, W waves per workgroup along time, `chunks` workgroups along time.
 struct form { int V, W; int64_t chunk, chunks, blocks; };
 
-// Wide loads need every row of every array at a multiple of their size.
-int memory_width(const dl_memory_shape* s, int most, bool back, std::initializer_list<const void*> elems, std::initializer_list<const void*> floats) {
-    for (int V = most; V > 1; V /= 2) {
-        bool ok = s->D % V == 0 && s->x_t % V == 0 && s->x_n % V == 0 && s->gate_t % V == 0 && s->gate_n % V == 0 && (!back || (s->grad_t % V == 0 && s->grad_n % V == 0));
-        for (const void* p : elems) ok = ok && aligned(p, (int64_t)V * elem_bytes(s->dtype));
-        for (const void* p : floats) ok = ok && aligned(p, 4);
-        if (ok) return V;
-    }
-    return 1;
+// Columns per lane: eight bytes forward, four backward, where three arrays and the states of a run are held.
+int memory_width(const dl_memory_shape* s, int most) {
+    int V = most;
+    while (V > s->D) V /= 2;
+    return V;
 }
+int widest_forward(int dtype) { return dtype == DL_F32 ? 2 : 4; }
+int widest_back(int dtype) { return dtype == DL_F32 ? 1 : 2; }
 
-// The chip wants about 2048 waves.  Columns come first (no exchange between waves), then up to eight waves of a workgroup along
-// time, then chunks over workgroups, which cost a second reading of the inputs and never get shorter than 8 runs a wave.
+// Columns come first: with a wave for every SIMD unit of the chip (1024) nothing is exchanged between waves.  Below that up to eight
+// waves of a workgroup share the time axis, and with less than 4096 waves then, chunks over workgroups, which cost a second reading
+// of the inputs and never get shorter than one run a wave.
 form memory_form(const dl_memory_shape* s, int V) {
     form f;
     f.V = V;
-    f.blocks = ceil_div(s->N * (s->D / V), 64);
+    f.blocks = ceil_div(s->N * ceil_div(s->D, V), 64);
     const int64_t runs = ceil_div(s->T, dlm::MARK);
     f.W = 1;
-    while (f.W < 8 && f.W < runs && f.blocks * f.W < 2048) f.W *= 2;
+    if (f.blocks < 1024) while (f.W < 8 && f.W < runs) f.W *= 2;
     const int64_t span = (int64_t)f.W * dlm::MARK;
     const int64_t spans = ceil_div(s->T, span);
     f.chunks = 1;
-    if (f.blocks * f.W < 1024 && spans > 4) f.chunks = std::min<int64_t>(std::min<int64_t>(ceil_div(spans, 2), 256), std::max<int64_t>(1, 2048 / (f.blocks * f.W)));
+    if (f.blocks < 512 && spans > 2) f.chunks = std::min<int64_t>(std::min<int64_t>(spans, 256), std::max<int64_t>(1, ceil_div(4096, f.blocks * f.W)));
     f.chunk = ceil_div(spans, f.chunks) * span;
     f.chunks = ceil_div(s->T, f.chunk);
     return f;
 }
 
 dlm::shape device_shape(const dl_memory_shape* s, const form& f) {
-    return dlm::shape{s->T, s->N, s->D, s->x_t, s->x_n, s->gate_t, s->gate_n, s->starts_t, s->starts_n, s->grad_t, s->grad_n, f.chunk, (int32_t)f.chunks};
+    return dlm::shape{s->N, s->D, s->x_t, s->x_n, s->gate_t, s->gate_n, s->starts_t, s->starts_n, s->grad_t, s->grad_n, (int32_t)s->T, (int32_t)f.chunk, (int32_t)f.chunks};
 }
 
 template <int N> struct Int { static constexpr int value = N; };
-template <typename F> void with_waves(int W, F&& f) {
-    if (W == 8) f(Int<8>()); else if (W == 4) f(Int<4>()); else if (W == 2) f(Int<2>()); else f(Int<1>());
+template <typename F> void with_waves(int W, F&& f) {          // more than one
+    if (W == 8) f(Int<8>()); else if (W == 4) f(Int<4>()); else f(Int<2>());
 }
 template <int MOST, typename F> void with_width(int V, F&& f) {
     if constexpr (MOST >= 4) if (V == 4) return f(Int<4>());
-    if (V == 2) f(Int<2>()); else f(Int<1>());
+    if constexpr (MOST >= 2) if (V == 2) return f(Int<2>());
+    f(Int<1>());
 }
-constexpr int WIDEST_BACK = 2;
 template <typename E> constexpr int widest() { return sizeof(E) == 4 ? 2 : 4; }
 template <typename F> void with_type(int dtype, F&& f) {
     if (dtype == DL_F32) f(float{}); else if (dtype == DL_BF16) f(__bf16{}); else f(_Float16{});
@@ -169,7 +173,7 @@ int64_t dl_memory_workspace_bytes(const dl_memory_shape* s) {
     if (const char* e = memory_shape_error(s)) return fail(DL_E_INVAL, e);
     if (s->T == 0 || s->N == 0 || s->D == 0) return 0;
     int64_t chunks = 1;
-    for (int V : {1, 2, 4}) if (s->D % V == 0) chunks = std::max(chunks, memory_form(s, V).chunks);
+    for (int most : {widest_forward(s->dtype), widest_back(s->dtype)}) chunks = std::max(chunks, memory_form(s, memory_width(s, most)).chunks);
     return chunks > 1 ? chunks * 2 * s->N * s->D * 4 : 0;
 }
 
@@ -179,18 +183,22 @@ int dl_memory_forward(const dl_memory_shape* s, const void* x, const void* gate,
     if (s->T == 0) return fail(DL_E_INVAL, "dl_memory_forward: T = 0 (there is no step: the state stays as it is)");
     if (!x || !gate || !h) return fail(DL_E_INVAL, "dl_memory_forward: x, gate and h must not be NULL");
     if (state && state == state_out) return fail(DL_E_INVAL, "dl_memory_forward: state_out may not be state");
-    const form f = memory_form(s, memory_width(s, s->dtype == DL_F32 ? 2 : 4, false, {x, gate, h}, {}));
+    const form f = memory_form(s, memory_width(s, widest_forward(s->dtype)));
     if (f.chunks > 1 && !workspace) return fail(DL_E_INVAL, "dl_memory_forward: workspace must not be NULL (dl_memory_workspace_bytes)");
     if (f.blocks > 0x7fffffff) return fail(DL_E_INVAL, "dl_memory_forward: N * D too large");
     const dlm::shape d = device_shape(s, f);
     const dim3 grid((unsigned)f.blocks, (unsigned)f.chunks);
     hipStream_t st = (hipStream_t)stream;
-    with_type(s->dtype, [&](auto e) { with_width<widest<decltype(e)>()>(f.V, [&](auto v) { with_waves(f.W, [&](auto w) {
+    with_type(s->dtype, [&](auto e) { with_width<widest<decltype(e)>()>(f.V, [&](auto v) {
         using E = decltype(e);
-        constexpr int V = decltype(v)::value, W = decltype(w)::value;
-        if (f.chunks > 1) dlm::k_memory_forward<E, V, W, true><<<dim3(grid.x, grid.y - 1), 64 * W, 0, st>>>(d, (const E*)x, (const E*)gate, starts, nullptr, nullptr, nullptr, nullptr, (float*)workspace);
-        dlm::k_memory_forward<E, V, W, false><<<grid, 64 * W, 0, st>>>(d, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks, (float*)workspace);
-    }); }); });
+        constexpr int V = decltype(v)::value;
+        if (f.W == 1) return dlm::k_memory_run<E, V><<<grid, 64, 0, st>>>(d, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks);
+        with_waves(f.W, [&](auto w) {
+            constexpr int W = decltype(w)::value;
+            if (f.chunks > 1) dlm::k_memory_forward<E, V, W, true><<<dim3(grid.x, grid.y - 1), 64 * W, 0, st>>>(d, (const E*)x, (const E*)gate, starts, nullptr, nullptr, nullptr, nullptr, (float*)workspace);
+            dlm::k_memory_forward<E, V, W, false><<<grid, 64 * W, 0, st>>>(d, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks, (float*)workspace);
+        });
+    }); });
     return launched("dl_memory_forward");
 }
 
@@ -201,18 +209,22 @@ int dl_memory_backward(const dl_memory_shape* s, const void* x, const void* gate
     if (s->T == 0) return fail(DL_E_INVAL, "dl_memory_backward: T = 0 (there is no step: the gradient of the state is grad_state)");
     if (!x || !gate || !marks || !dx || !dgate) return fail(DL_E_INVAL, "dl_memory_backward: x, gate, marks, dx and dgate must not be NULL");
     if (grad_state && grad_state == dstate) return fail(DL_E_INVAL, "dl_memory_backward: dstate may not be grad_state");
-    const form f = memory_form(s, memory_width(s, WIDEST_BACK, grad_h != nullptr, {x, gate, grad_h, dx, dgate}, {}));
+    const form f = memory_form(s, memory_width(s, widest_back(s->dtype)));
     if (f.chunks > 1 && !workspace) return fail(DL_E_INVAL, "dl_memory_backward: workspace must not be NULL (dl_memory_workspace_bytes)");
     if (f.blocks > 0x7fffffff) return fail(DL_E_INVAL, "dl_memory_backward: N * D too large");
     const dlm::shape d = device_shape(s, f);
     const dim3 grid((unsigned)f.blocks, (unsigned)f.chunks);
     hipStream_t st = (hipStream_t)stream;
-    with_type(s->dtype, [&](auto e) { with_width<WIDEST_BACK>(f.V, [&](auto v) { with_waves(f.W, [&](auto w) {
+    with_type(s->dtype, [&](auto e) { with_width<widest<decltype(e)>() / 2>(f.V, [&](auto v) {
         using E = decltype(e);
-        constexpr int V = decltype(v)::value, W = decltype(w)::value;
-        if (f.chunks > 1) dlm::k_memory_backward<E, V, W, true><<<grid, 64 * W, 0, st>>>(d, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, nullptr, nullptr, nullptr, nullptr, (float*)workspace);
-        dlm::k_memory_backward<E, V, W, false><<<grid, 64 * W, 0, st>>>(d, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, grad_state, (E*)dx, (E*)dgate, dstate, (float*)workspace);
-    }); }); });
+        constexpr int V = decltype(v)::value;
+        if (f.W == 1) return dlm::k_memory_backward<E, V, 1, false><<<grid, 64, 0, st>>>(d, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, grad_state, (E*)dx, (E*)dgate, dstate, nullptr);
+        with_waves(f.W, [&](auto w) {
+            constexpr int W = decltype(w)::value;
+            if (f.chunks > 1) dlm::k_memory_backward<E, V, W, true><<<grid, 64 * W, 0, st>>>(d, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, nullptr, nullptr, nullptr, nullptr, (float*)workspace);
+            dlm::k_memory_backward<E, V, W, false><<<grid, 64 * W, 0, st>>>(d, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, grad_state, (E*)dx, (E*)dgate, dstate, (float*)workspace);
+        });
+    }); });
     return launched("dl_memory_backward");
 }
 
@@ -221,7 +233,8 @@ int dl_memory_step(const dl_memory_shape* s, const void* x, const void* gate, co
     if (s->T != 1) return fail(DL_E_INVAL, "dl_memory_step: T must be 1");
     if (s->N == 0 || s->D == 0) return DL_OK;
     if (!x || !gate || !h || !state_out) return fail(DL_E_INVAL, "dl_memory_step: x, gate, h and state_out must not be NULL");
-    const int V = memory_width(s, s->dtype == DL_F32 ? 2 : 4, false, {x, gate, h}, {});
+    int V = widest_forward(s->dtype);
+    while (s->D % V) V /= 2;
     const int64_t blocks = ceil_div(s->N * (s->D / V), 256);
     if (blocks > 0x7fffffff) return fail(DL_E_INVAL, "dl_memory_step: N * D too large");
     with_type(s->dtype, [&](auto e) { with_width<widest<decltype(e)>()>(V, [&](auto v) {

@@ -3,23 +3,29 @@
 //     a = sigmoid(g), s = 1 - a:      h[t] = a h' + s x[t],   h' = start ? 0 : h[t-1]
 //     l[t] = dh[t] + c[t+1],  c[t] = start ? 0 : a l[t]:      dx = s l,   dg = (h' - x) a s l,   dstate = c[0]
 //
-// Bound by memory: three elements moved per step forward, five backward.  Every element is loaded once: a wave keeps MARK steps
-// of 64 columns in registers, reduces them to the affine map (A, B) of its run, the waves of a workgroup exchange their maps
-// through LDS, and each wave then finishes its own steps from the registers.  With too few columns for the chip the time axis is
-// also cut into chunks over workgroups: a first kernel reduces every chunk to its map, the second starts from the maps before it.
+// Bound by memory (three elements moved per step forward, five backward) with the arithmetic, 20 to 40 operations per element, close
+// behind.  Every element is loaded once: a wave keeps MARK steps of 64 x V columns in registers.  With enough columns for the chip a
+// wave runs through time by itself and loads the next run while it computes this one.  With fewer, the waves of a workgroup take
+// consecutive runs, reduce each to its affine map, exchange the maps through LDS, and finish their steps from the registers.
+// With fewer still the time axis is also cut into chunks over workgroups: a first kernel reduces every chunk to its map, the second
+// starts from the maps before it.
 //
 // Rounding.  The smaller of a and s is computed as e / (1 + e), e = exp(-|g|), and both products go through it:
 //     g >= 0:  h = h' + s (x - h'),  c = l - s l        g < 0:  h = x + a (h' - x),  c = a l
 // so that a long memory (s small) loses nothing to the rounding of a = 1 - s, and a closed gate gives x exactly.
+//
+// Columns.  A lane takes V neighbouring channels with one load (4 or 8 bytes, any alignment); where V does not divide D the last
+// lane of a row moves back, and two lanes compute, and write, the same values.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 
 namespace dlm {
 
 constexpr int MARK = 16;          // steps of a wave's run, and between two saved states
 
-template <typename E, int V> struct vec { typedef E type __attribute__((ext_vector_type(V))); };
+template <typename E, int V> struct vec { typedef E type __attribute__((ext_vector_type(V), aligned(sizeof(E)))); };
 template <typename E> struct vec<E, 1> { typedef E type; };
 template <typename E, int V> using vec_t = typename vec<E, V>::type;
 
@@ -27,45 +33,33 @@ template <typename E, int V> __device__ __forceinline__ float get(const vec_t<E,
     if constexpr (V == 1) return (float)v; else return (float)v[i];
 }
 template <typename E, int V> __device__ __forceinline__ void put(vec_t<E, V>& v, int i, float f) {
+    // float16: rounded from the 32-bit value everywhere, not in one kernel by a product-sum that rounds to 16 bits at once
+    if constexpr (std::is_same<E, _Float16>::value) asm("" : "+v"(f));
     if constexpr (V == 1) v = (E)f; else v[i] = (E)f;
 }
 
 struct shape {
-    int64_t T, N, D;
+    int64_t N, D;
     int64_t x_t, x_n, gate_t, gate_n, starts_t, starts_n, grad_t, grad_n;
-    int64_t chunk;                // steps of a workgroup (a multiple of waves * MARK)
-    int32_t chunks;
+    int32_t T;
+    int32_t chunk, chunks;        // steps of a workgroup (a multiple of waves * MARK), workgroups along time
 };
 
-// min(a, s), with the sign of the gate: >= +0 where a is the larger one (g >= 0), <= -0 where s is.
-// exp(-|g|) with the rounding of |g| log2(e) carried along: one unit of the result, far tails included.
+// min(a, s) with the sign of the gate.
 __device__ __forceinline__ float gate_of(float g) {
-    const float u = -fabsf(g);
-    const float p = u * 1.44269504f;
-    const float r = fmaf(u, 1.44269504f, -p) + u * 1.92596299e-8f;
-    float e = __builtin_amdgcn_exp2f(p);
-    e = fmaf(e, r * 0.693147181f, e);
-    if (p < -150.0f) e = 0.0f;                         // (infinite gates: r is NaN)
-    const float m = e * __builtin_amdgcn_rcpf(1.0f + e);
-    return g >= 0.0f ? m : (g < 0.0f ? -m : g);        // a NaN stays one
+    const float e = __builtin_amdgcn_exp2f(-fabsf(g) * 1.44269504f);
+    return copysignf(e * __builtin_amdgcn_rcpf(1.0f + e), g);
 }
-__device__ __forceinline__ bool keeps(float m) { return !(__float_as_uint(m) >> 31); }
-// Between the passes over a run: the comparisons of the first are made again instead of being kept, a pair of scalar registers each.
-template <int V> __device__ __forceinline__ void forget(float (&m)[MARK][V], uint32_t& begin) {
-#pragma unroll
-    for (int t = 0; t < MARK; ++t) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) asm volatile("" : "+v"(m[t][v]));
-    }
-    asm volatile("" : "+v"(begin));
-}
+__device__ __forceinline__ bool keeps(float m) { return !(__float_as_uint(m) >> 31); }          // s is the smaller one
 // one step of the state
 __device__ __forceinline__ float step_of(float m, float x, float h) {
-    const float d = x - h;
-    return keeps(m) ? fmaf(m, d, h) : fmaf(m, d, x);   // (m < 0: x + |m| (h - x) = x + m (x - h))
+    return fmaf(m, x - h, keeps(m) ? h : x);           // (m < 0: x + |m| (h - x) = x + m (x - h))
 }
-// one step of a product of a
-__device__ __forceinline__ float decay_of(float m, float l) { return keeps(m) ? fmaf(-m, l, l) : -m * l; }
+// one step of a product of a: l -> a l
+__device__ __forceinline__ float decay_of(float m, float l) {
+    const float w = m * l;
+    return keeps(m) ? l - w : -w;
+}
 
 // The map h -> a h + b of a run, a = the product of its steps'.  Like a step it is held by the smaller of a and p = 1 - a: m = p
 // where p <= 1/2, else -a; so a product over thousands of open gates is as exact as its steps.  BEGUN: an episode began inside
@@ -74,8 +68,9 @@ constexpr float BEGUN = 2.0f;
 struct factor {
     float a = 1.0f, p = 0.0f;
     __device__ __forceinline__ void step(float m) {
-        p = fmaf(keeps(m) ? m : 1.0f + m, a, p);
-        a = decay_of(m, a);
+        const float w = fabsf(m) * a, o = a - w;
+        p += keeps(m) ? w : o;
+        a = keeps(m) ? o : w;
     }
     __device__ __forceinline__ float held(bool begun) const { return begun ? BEGUN : p <= 0.5f ? p : -a; }          // (a NaN stays one)
 };
@@ -87,18 +82,39 @@ __device__ __forceinline__ float after(float m, float n) {          // m, then n
     return f.held(false);
 }
 
+__device__ __forceinline__ int64_t uniform(int64_t v) {          // the same in all lanes: into scalar registers
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+
+// Where a lane's columns lie.  Rows are addressed as a pointer of the workgroup (scalar registers) at channel 0 of its first walker,
+// n0, plus 32 bits of a lane; the host refuses strides for which 64 walkers are further apart than that.
 template <int V> struct columns {
-    int64_t n, d, col;            // walker, channel, place in an [N, D] array
-    bool valid;
+    int64_t n0;
+    uint32_t dn, d;               // walkers after n0, channel
+    bool valid, few;              // few: the wave spans at most four walkers
     __device__ columns(int64_t N, int64_t D) {
-        const int64_t per = D / V;
-        const int64_t q = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+        const int64_t per = (D + V - 1) / V;
+        const int64_t q0 = (int64_t)blockIdx.x * 64, q = q0 + (threadIdx.x & 63);
+        n0 = uniform(q0 / per);
         valid = q < N * per;
-        n = valid ? q / per : 0;
-        d = valid ? (q - n * per) * V : 0;
-        col = n * D + d;
+        dn = valid ? (uint32_t)(q / per - n0) : 0;
+        d = valid ? (uint32_t)min((q - (n0 + dn) * per) * V, D - V) : 0;
+        few = per >= 32;
     }
+    template <typename E> __device__ __forceinline__ uint32_t bytes(int64_t stride_n) const { return (dn * (uint32_t)stride_n + d) * (uint32_t)sizeof(E); }
 };
+// base in scalar registers, kept there: no 64-bit addition per lane and access
+#define DLM_GLOBAL __attribute__((address_space(1)))
+template <typename T> __device__ __forceinline__ T load_at(const void* base, uint32_t bytes) {
+    const DLM_GLOBAL char* p = (const DLM_GLOBAL char*)base;
+    asm("" : "+s"(p));
+    return *(const DLM_GLOBAL T*)(p + bytes);
+}
+template <typename T> __device__ __forceinline__ void store_at(void* base, uint32_t bytes, const T& v) {
+    DLM_GLOBAL char* p = (DLM_GLOBAL char*)base;
+    asm("" : "+s"(p));
+    *(DLM_GLOBAL T*)(p + bytes) = v;
+}
 
 // The state (or gradient) that enters the run of each wave from the maps of the waves before it, and the one behind the last.
 // `from` = how many maps come first in the order of the recurrence for this wave.
@@ -119,7 +135,7 @@ __device__ __forceinline__ void join(const float (*la)[64 * V], const float (*lb
 // Maps of whole chunks -> the value that enters chunk k, by the whole workgroup: every wave joins a part of the chunks before.
 // maps: float [chunks][2][N * D].
 template <int V, bool BACK>
-__device__ __forceinline__ void enter(const float* maps, int64_t plane, int k, int chunks, const columns<V>& c, int waves, int wave, int lane, float (*la)[64 * V], float (*lb)[64 * V], float (&carry)[V]) {
+__device__ __forceinline__ void enter(const float* maps, int64_t plane, int k, int chunks, uint32_t floats, int waves, int wave, int lane, float (*la)[64 * V], float (*lb)[64 * V], float (&carry)[V]) {
     const int before = BACK ? chunks - 1 - k : k;
     if (before == 0) return;
     float A[V], B[V];
@@ -129,10 +145,11 @@ __device__ __forceinline__ void enter(const float* maps, int64_t plane, int k, i
 #pragma unroll 4
     for (int i = lo; i < hi; ++i) {
         const int j = BACK ? chunks - 1 - i : i;
-        const float* p = maps + (int64_t)j * 2 * plane + c.col;
+        const float* p = maps + (int64_t)j * 2 * plane;          // (maps: at channel 0 of the first walker)
+        const vec_t<float, V> ma = load_at<vec_t<float, V>>(p, floats), mb = load_at<vec_t<float, V>>(p + plane, floats);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const float a = p[v], b = p[plane + v];
+            const float a = get<float, V>(ma, v), b = get<float, V>(mb, v);
             B[v] = apply(a, b, B[v]);
             A[v] = after(A[v], a);
         }
@@ -147,169 +164,269 @@ __device__ __forceinline__ void enter(const float* maps, int64_t plane, int k, i
     __syncthreads();
 }
 
-// MAPS: only reduce the chunk to its map.
+// Between the passes over a run: the comparisons of the first are made again instead of being kept, a pair of scalar registers each.
+template <int V> __device__ __forceinline__ void forget(float (&m)[MARK][V], uint32_t& begin) {
+#pragma unroll
+    for (int t = 0; t < MARK; ++t) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) asm volatile("" : "+v"(m[t][v]));
+    }
+    asm volatile("" : "+v"(begin));
+}
+
+template <typename T> __device__ __forceinline__ void opaque(T& v) {
+    if constexpr (sizeof(T) == 8) { uint64_t u = __builtin_bit_cast(uint64_t, v); asm volatile("" : "+v"(u)); v = __builtin_bit_cast(T, u); }
+    else if constexpr (sizeof(T) == 4) { uint32_t u = __builtin_bit_cast(uint32_t, v); asm volatile("" : "+v"(u)); v = __builtin_bit_cast(T, u); }
+    else { uint16_t u = __builtin_bit_cast(uint16_t, v); asm volatile("" : "+v"(u)); v = __builtin_bit_cast(T, u); }
+}
+// The scheduler would start all the steps of a run at once and keep their halves in registers: every few elements it may not look further.
+template <int V> __device__ __forceinline__ void pause(int t) {
+    if ((t + 1) * V % 8 == 0) __builtin_amdgcn_sched_barrier(0);
+}
+
+// Rows t0 .. t0 + R - 1 as they lie in memory.  Rows behind the end read the last one again.
+template <typename E, int V, int R, bool X, bool G> struct rows {
+    typedef vec_t<E, V> vec;
+    vec x[R], g[R], d[R];
+    uint32_t begin;               // bit t: an episode begins at row t
+    uint8_t flag;                 // few walkers: lane 16 w + t looks at row t of walker n0 + w, for all
+
+    __device__ __forceinline__ static void each(vec (&to)[R], const E* base, int64_t stride, uint32_t off, int len) {
+        const E* p = base;
+        if (len >= R) {
+#pragma unroll
+            for (int t = 0; t < R; ++t) { to[t] = load_at<vec>(p, off); p += stride; }
+        } else {
+#pragma unroll
+            for (int t = 0; t < R; ++t) { to[t] = load_at<vec>(p, off); if (t + 1 < len) p += stride; }
+        }
+    }
+    __device__ __forceinline__ void load(const shape& s, const columns<V>& c, int t0, int last, const E* x_, const E* g_, const E* d_, const uint8_t* b_) {
+        const int len = max(0, min(R, last - t0));
+        const int64_t from = min(t0, last - 1);
+        if (X) each(x, x_ + from * s.x_t + c.n0 * s.x_n, s.x_t, c.template bytes<E>(s.x_n), len);
+        each(g, g_ + from * s.gate_t + c.n0 * s.gate_n, s.gate_t, c.template bytes<E>(s.gate_n), len);
+        if (G) {
+            if (d_) each(d, d_ + from * s.grad_t + c.n0 * s.grad_n, s.grad_t, c.template bytes<E>(s.grad_n), len);
+            else {
+#pragma unroll
+                for (int t = 0; t < R; ++t)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) put<E, V>(d[t], v, 0.0f);
+            }
+        }
+        begin = 0;
+        flag = 0;
+        if (b_) {
+            const uint8_t* p = b_ + from * s.starts_t + c.n0 * s.starts_n;
+            if (c.few) {
+                const int t = threadIdx.x & 15, w = (threadIdx.x >> 4) & 3;
+                if (t < len && c.n0 + w < s.N) flag = p[(int64_t)t * s.starts_t + (int64_t)w * s.starts_n];
+            } else {
+#pragma unroll
+                for (int t = 0; t < R; ++t)
+                    if (t < len) begin |= (uint32_t)(p[(int64_t)t * s.starts_t + (int64_t)c.dn * s.starts_n] != 0) << t;
+            }
+        }
+    }
+    // when the rows are needed
+    __device__ __forceinline__ uint32_t begins(const columns<V>& c) const {
+        return c.few ? (uint32_t)(__ballot(flag != 0) >> (16 * c.dn)) & 0xffffu : begin;
+    }
+    // As forget(): what was converted from the elements is converted again.
+    __device__ __forceinline__ void forget() {
+#pragma unroll
+        for (int t = 0; t < R; ++t) { if (X) opaque(x[t]); if (G) opaque(d[t]); }
+    }
+};
+
+template <int V> __device__ __forceinline__ void load_floats(float (&to)[V], const float* base, uint32_t bytes) {
+    const vec_t<float, V> f = load_at<vec_t<float, V>>(base, bytes);
+#pragma unroll
+    for (int v = 0; v < V; ++v) to[v] = get<float, V>(f, v);
+}
+template <int V> __device__ __forceinline__ void store_floats(float* base, uint32_t bytes, const float (&from)[V]) {
+    vec_t<float, V> f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) put<float, V>(f, v, from[v]);
+    store_at<vec_t<float, V>>(base, bytes, f);
+}
+
+struct yes { static constexpr bool value = true; };
+struct no { static constexpr bool value = false; };
+
+// ---- enough columns: a wave runs through all of time by itself, half a run ahead with its loads -----------------------------------
+template <typename E, int V>
+__global__ __launch_bounds__(64) void k_memory_run(shape s, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ state,
+                                                   E* __restrict__ h, float* __restrict__ state_out, float* __restrict__ marks) {
+    typedef vec_t<E, V> vec;
+    constexpr int R = MARK / 2;
+    const columns<V> c(s.N, s.D);
+    const int64_t plane = s.N * s.D, corner = c.n0 * s.D;
+    const uint32_t elems = c.template bytes<E>(s.D), floats = c.template bytes<float>(s.D);
+    float now[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) now[v] = 0.0f;
+    if (state) load_floats<V>(now, state + corner, floats);
+    typedef rows<E, V, R, true, false> half;
+    auto steps = [&](const half& r, int t0, int len, auto all, uint32_t begin) {
+        E* ph = h + (int64_t)t0 * plane + corner;
+#pragma unroll
+        for (int t = 0; t < R; ++t) {
+            if (decltype(all)::value || t < len) {
+                vec o;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    if (!decltype(all)::value) now[v] = (begin >> t) & 1 ? 0.0f : now[v];
+                    now[v] = step_of(gate_of(get<E, V>(r.g[t], v)), get<E, V>(r.x[t], v), now[v]);
+                    put<E, V>(o, v, now[v]);
+                }
+                if (c.valid) store_at<vec>(ph, elems, o);
+                ph += plane;
+            }
+        }
+    };
+    auto run = [&](const half& r, int t0) {          // whole and without a beginning, as nearly always, or not
+        const int len = max(0, min(R, s.T - t0));
+        const uint32_t begin = r.begins(c);
+        if (len == R && __ballot(begin != 0) == 0) steps(r, t0, len, yes(), 0u); else steps(r, t0, len, no(), begin);
+    };
+    half p, q;
+    p.load(s, c, 0, s.T, x, gate, nullptr, starts);
+    for (int t0 = 0; t0 < s.T; t0 += MARK) {
+        q.load(s, c, t0 + R, s.T, x, gate, nullptr, starts);
+        if (marks && c.valid) store_floats<V>(marks + (int64_t)(t0 / MARK) * plane + corner, floats, now);
+        run(p, t0);
+        p.load(s, c, t0 + MARK, s.T, x, gate, nullptr, starts);
+        run(q, t0 + R);
+    }
+    if (state_out && c.valid) store_floats<V>(state_out + corner, floats, now);
+}
+
+// ---- W waves of a workgroup take consecutive runs.  MAPS: only reduce the chunk to its map -----------------------------------------
 template <typename E, int V, int W, bool MAPS>
 __global__ __launch_bounds__(64 * W) void k_memory_forward(shape s, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ state,
                                                            E* __restrict__ h, float* __restrict__ state_out, float* __restrict__ marks, float* __restrict__ maps) {
     typedef vec_t<E, V> vec;
     __shared__ float la[W][64 * V], lb[W][64 * V];
-    const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const columns<V> c(s.N, s.D);
-    const int64_t plane = s.N * s.D;
+    const int64_t plane = s.N * s.D, corner = c.n0 * s.D;
+    const uint32_t elems = c.template bytes<E>(s.D), floats = c.template bytes<float>(s.D);
     const int k = blockIdx.y;
-    const int64_t first = (int64_t)k * s.chunk, last = min(first + s.chunk, s.T);
+    const int first = k * s.chunk, last = min(first + s.chunk, s.T);
     float carry[V], chunk[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) { carry[v] = 0.0f; chunk[v] = 0.0f; }
     if (!MAPS) {
-        if (state) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) carry[v] = state[c.col + v];
-        }
-        if (s.chunks > 1) enter<V, false>(maps, plane, k, s.chunks, c, W, wave, lane, la, lb, carry);
+        if (state) load_floats<V>(carry, state + corner, floats);
+        if (s.chunks > 1) enter<V, false>(maps + corner, plane, k, s.chunks, floats, W, wave, lane, la, lb, carry);
     }
-    for (int64_t base = first; base < last; base += W * MARK) {
-        const int64_t t0 = base + wave * MARK;
-        const int len = (int)max((int64_t)0, min((int64_t)MARK, last - t0));
-        // Rows behind the end read the last one again and count as steps with an open gate (h stays as it is).
-        vec xs[MARK], gs[MARK]; float m[MARK][V]; uint8_t bs[MARK]; uint32_t begin = 0;
+    for (int base = first; base < last; base += W * MARK) {
+        const int t0 = base + wave * MARK;
+        const int len = max(0, min(MARK, last - t0));
+        rows<E, V, MARK, true, false> r;
+        r.load(s, c, t0, last, x, gate, nullptr, starts);
+        float m[MARK][V];
+        uint32_t begin = r.begins(c);
+        factor A[V]; float B[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) B[v] = 0.0f;
 #pragma unroll
         for (int t = 0; t < MARK; ++t) {
-            const int64_t row = min(t0 + t, last - 1);
-            xs[t] = *(const vec*)(x + row * s.x_t + c.n * s.x_n + c.d);
-            gs[t] = *(const vec*)(gate + row * s.gate_t + c.n * s.gate_n + c.d);
-            bs[t] = starts ? starts[row * s.starts_t + c.n * s.starts_n] : 0;
-        }
 #pragma unroll
-        for (int t = 0; t < MARK; ++t) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) m[t][v] = t < len ? gate_of(get<E, V>(gs[t], v)) : 0.0f;
-            if (t < len && bs[t]) begin |= 1u << t;
-        }
-        float in[V];
-        if (W > 1 || MAPS) {
-            factor A[V]; float B[V];
-#pragma unroll
-            for (int v = 0; v < V; ++v) B[v] = 0.0f;
-#pragma unroll
-            for (int t = 0; t < MARK; ++t) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    B[v] = step_of(m[t][v], get<E, V>(xs[t], v), (begin >> t) & 1 ? 0.0f : B[v]);
-                    A[v].step(m[t][v]);
-                }
+            for (int v = 0; v < V; ++v) {
+                m[t][v] = t < len ? gate_of(get<E, V>(r.g[t], v)) : 0.0f;          // (behind the end: an open gate, h stays as it is)
+                B[v] = step_of(m[t][v], get<E, V>(r.x[t], v), (begin >> t) & 1 ? 0.0f : B[v]);
+                A[v].step(m[t][v]);
             }
-#pragma unroll
-            for (int v = 0; v < V; ++v) { la[wave][v * 64 + lane] = A[v].held(begin != 0); lb[wave][v * 64 + lane] = B[v]; }
-            forget<V>(m, begin);
-            __syncthreads();
-            float next[V];
-            join<V>(la, lb, lane, W, wave, carry, in, next, false);
-            if (MAPS) {
-                for (int w = 0; w < W; ++w) {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) chunk[v] = after(chunk[v], la[w][v * 64 + lane]);
-                }
-            }
-#pragma unroll
-            for (int v = 0; v < V; ++v) carry[v] = next[v];
-            __syncthreads();
-        } else {
-#pragma unroll
-            for (int v = 0; v < V; ++v) in[v] = carry[v];
+            pause<V>(t);
         }
+#pragma unroll
+        for (int v = 0; v < V; ++v) { la[wave][v * 64 + lane] = A[v].held(begin != 0); lb[wave][v * 64 + lane] = B[v]; }
+        forget<V>(m, begin); r.forget();
+        __syncthreads();
+        float in[V], next[V];
+        join<V>(la, lb, lane, W, wave, carry, in, next, false);
+        if (MAPS) {
+            for (int w = 0; w < W; ++w) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) chunk[v] = after(chunk[v], la[w][v * 64 + lane]);
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) carry[v] = next[v];
+        __syncthreads();
         if (!MAPS) {
-            if (marks && c.valid && len > 0) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) marks[(t0 / MARK) * plane + c.col + v] = in[v];
-            }
-            E* ph = h + t0 * plane + c.col;
+            if (marks && c.valid && len > 0) store_floats<V>(marks + (int64_t)(t0 / MARK) * plane + corner, floats, in);
+            E* ph = h + (int64_t)t0 * plane + corner;
 #pragma unroll
             for (int t = 0; t < MARK; ++t) {
                 if (t < len) {
                     vec o;
 #pragma unroll
                     for (int v = 0; v < V; ++v) {
-                        in[v] = step_of(m[t][v], get<E, V>(xs[t], v), (begin >> t) & 1 ? 0.0f : in[v]);
+                        in[v] = step_of(m[t][v], get<E, V>(r.x[t], v), (begin >> t) & 1 ? 0.0f : in[v]);
                         put<E, V>(o, v, in[v]);
                     }
-                    if (c.valid) *(vec*)(ph + t * plane) = o;
+                    if (c.valid) store_at<vec>(ph, elems, o);
+                    ph += plane;
                 }
-            }
-            if (W == 1) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) carry[v] = in[v];
             }
         }
     }
     if (MAPS) {
         if (wave == 0 && c.valid) {
-            float* p = maps + (int64_t)k * 2 * plane + c.col;
-#pragma unroll
-            for (int v = 0; v < V; ++v) { p[v] = chunk[v]; p[plane + v] = carry[v]; }
+            float* p = maps + (int64_t)k * 2 * plane + corner;
+            store_floats<V>(p, floats, chunk);
+            store_floats<V>(p + plane, floats, carry);
         }
     } else if (state_out && wave == 0 && c.valid && last == s.T) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) state_out[c.col + v] = carry[v];
+        store_floats<V>(state_out + corner, floats, carry);
     }
 }
 
+// ---- gradients.  W = 1: a wave runs through all of time by itself, a run ahead with its loads ---------------------------------------
 template <typename E, int V, int W, bool MAPS>
 __global__ __launch_bounds__(64 * W) void k_memory_backward(shape s, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ marks,
                                                             const E* __restrict__ grad_h, const float* __restrict__ grad_state, E* __restrict__ dx, E* __restrict__ dgate,
                                                             float* __restrict__ dstate, float* __restrict__ maps) {
     typedef vec_t<E, V> vec;
+    typedef rows<E, V, MARK, !MAPS, true> run;
     __shared__ float la[W][64 * V], lb[W][64 * V];
     const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const columns<V> c(s.N, s.D);
-    const int64_t plane = s.N * s.D;
+    const int64_t plane = s.N * s.D, corner = c.n0 * s.D;
+    const uint32_t elems = c.template bytes<E>(s.D), floats = c.template bytes<float>(s.D);
     const int k = blockIdx.y;
-    const int64_t first = (int64_t)k * s.chunk, last = min(first + s.chunk, s.T);
+    const int first = k * s.chunk, last = min(first + s.chunk, s.T);
     float carry[V], chunk[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) { carry[v] = 0.0f; chunk[v] = 0.0f; }
     if (!MAPS) {
-        if (grad_state) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) carry[v] = grad_state[c.col + v];
-        }
-        if (s.chunks > 1) enter<V, true>(maps, plane, k, s.chunks, c, W, wave, lane, la, lb, carry);
+        if (grad_state) load_floats<V>(carry, grad_state + corner, floats);
+        if (s.chunks > 1) enter<V, true>(maps + corner, plane, k, s.chunks, floats, W, wave, lane, la, lb, carry);
     }
-    const int64_t span = W * MARK;
-    for (int64_t base = first + (last - first - 1) / span * span; base >= first; base -= span) {
-        const int64_t t0 = base + wave * MARK;
-        const int len = (int)max((int64_t)0, min((int64_t)MARK, last - t0));
-        vec xs[MARK], gs[MARK], ds[MARK]; float m[MARK][V], hs[MARK][V], h0[V]; uint8_t bs[MARK]; uint32_t begin = 0;
-        if (!MAPS) {
-            const int64_t mark = min(t0, last - 1) / MARK;
+    auto one = [&](run& r, int base, const float (&h0)[V]) {
+        const int t0 = base + wave * MARK;
+        const int len = max(0, min(MARK, last - t0));
+        uint32_t begin = r.begins(c);
+        float m[MARK][V], hs[MARK][V], h[V];
 #pragma unroll
-            for (int v = 0; v < V; ++v) h0[v] = marks[mark * plane + c.col + v];
-        }
+        for (int v = 0; v < V; ++v) h[v] = h0[v];
 #pragma unroll
         for (int t = 0; t < MARK; ++t) {
-            const int64_t row = min(t0 + t, last - 1);
-            if (!MAPS) xs[t] = *(const vec*)(x + row * s.x_t + c.n * s.x_n + c.d);
-            gs[t] = *(const vec*)(gate + row * s.gate_t + c.n * s.gate_n + c.d);
-            if (grad_h && t < len) ds[t] = *(const vec*)(grad_h + row * s.grad_t + c.n * s.grad_n + c.d);
-            else {
-#pragma unroll
-                for (int v = 0; v < V; ++v) put<E, V>(ds[t], v, 0.0f);
-            }
-            bs[t] = starts ? starts[row * s.starts_t + c.n * s.starts_n] : 0;
-        }
-#pragma unroll
-        for (int t = 0; t < MARK; ++t) {
-            if (t < len && bs[t]) begin |= 1u << t;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                m[t][v] = t < len ? gate_of(get<E, V>(gs[t], v)) : 0.0f;
+                m[t][v] = t < len ? gate_of(get<E, V>(r.g[t], v)) : 0.0f;
                 if (!MAPS) {
-                    hs[t][v] = (begin >> t) & 1 ? 0.0f : h0[v];
-                    h0[v] = step_of(m[t][v], get<E, V>(xs[t], v), hs[t][v]);
+                    hs[t][v] = (begin >> t) & 1 ? 0.0f : h[v];
+                    h[v] = step_of(m[t][v], get<E, V>(r.x[t], v), hs[t][v]);
                 }
             }
+            pause<V>(t);
         }
-        forget<V>(m, begin);
+        if (!MAPS) { forget<V>(m, begin); r.forget(); }
         float in[V];
         if (W > 1 || MAPS) {
             factor A[V]; float B[V];
@@ -319,13 +436,14 @@ __global__ __launch_bounds__(64 * W) void k_memory_backward(shape s, const E* __
             for (int t = MARK - 1; t >= 0; --t) {
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    B[v] = (begin >> t) & 1 ? 0.0f : decay_of(m[t][v], get<E, V>(ds[t], v) + B[v]);
+                    B[v] = (begin >> t) & 1 ? 0.0f : decay_of(m[t][v], (t < len ? get<E, V>(r.d[t], v) : 0.0f) + B[v]);
                     A[v].step(m[t][v]);
                 }
+                pause<V>(MARK - 1 - t);
             }
 #pragma unroll
             for (int v = 0; v < V; ++v) { la[wave][v * 64 + lane] = A[v].held(begin != 0); lb[wave][v * 64 + lane] = B[v]; }
-            forget<V>(m, begin);
+            if (!MAPS) { forget<V>(m, begin); r.forget(); }
             __syncthreads();
             float next[V];
             join<V>(la, lb, lane, W, W - 1 - wave, carry, in, next, true);
@@ -343,42 +461,78 @@ __global__ __launch_bounds__(64 * W) void k_memory_backward(shape s, const E* __
             for (int v = 0; v < V; ++v) in[v] = carry[v];
         }
         if (!MAPS) {
-            E* pdx = dx + t0 * plane + c.col;
-            E* pdg = dgate + t0 * plane + c.col;
+            E* pdx = dx + (int64_t)(t0 + len - 1) * plane + corner;
+            E* pdg = dgate + (int64_t)(t0 + len - 1) * plane + corner;
 #pragma unroll
             for (int t = MARK - 1; t >= 0; --t) {
                 if (t < len) {
                     vec ox, og;
 #pragma unroll
                     for (int v = 0; v < V; ++v) {
-                        const float q = fabsf(m[t][v]), l = get<E, V>(ds[t], v) + in[v];
-                        const float s_ = keeps(m[t][v]) ? q : 1.0f - q;
-                        put<E, V>(ox, v, s_ * l);
-                        put<E, V>(og, v, (hs[t][v] - get<E, V>(xs[t], v)) * ((q - q * q) * l));
-                        in[v] = (begin >> t) & 1 ? 0.0f : decay_of(m[t][v], l);
+                        const float l = get<E, V>(r.d[t], v) + in[v];
+                        const float q = fabsf(m[t][v]), w = q * l, o = l - w;          // the smaller and the larger share
+                        put<E, V>(ox, v, keeps(m[t][v]) ? w : o);
+                        put<E, V>(og, v, (hs[t][v] - get<E, V>(r.x[t], v)) * fmaf(-q, w, w));
+                        in[v] = (begin >> t) & 1 ? 0.0f : keeps(m[t][v]) ? o : w;
                     }
-                    if (c.valid) { *(vec*)(pdx + t * plane) = ox; *(vec*)(pdg + t * plane) = og; }
+                    if (c.valid) { store_at<vec>(pdx, elems, ox); store_at<vec>(pdg, elems, og); }
+                    pdx -= plane; pdg -= plane;
                 }
+                pause<V>(MARK - 1 - t);
             }
             if (W == 1) {
 #pragma unroll
                 for (int v = 0; v < V; ++v) carry[v] = in[v];
             }
         }
+    };
+    auto get_marks = [&](float (&h0)[V], int base) {
+        if (!MAPS) load_floats<V>(h0, marks + (int64_t)(min(base + wave * MARK, last - 1) / MARK) * plane + corner, floats);
+        else {
+#pragma unroll
+            for (int v = 0; v < V; ++v) h0[v] = 0.0f;
+        }
+    };
+    const int span = W * MARK;
+    int base = first + (last - first - 1) / span * span;
+    auto fetch = [&](run& r, float (&h0)[V], int at_) {          // (the one behind the first run: that again)
+        const int t = max(at_, first) + wave * MARK;
+        r.load(s, c, t, last, x, gate, grad_h, starts);
+        get_marks(h0, max(at_, first));
+    };
+    run p;
+    float hp[V];
+    fetch(p, hp, base);
+    if constexpr (W == 1) {
+        run q;
+        float hq[V];
+        for (;;) {
+            fetch(q, hq, base - span);
+            one(p, base, hp);
+            if ((base -= span) < first) break;
+            fetch(p, hp, base - span);
+            one(q, base, hq);
+            if ((base -= span) < first) break;
+        }
+    } else {
+        for (;;) {
+            one(p, base, hp);
+            if ((base -= span) < first) break;
+            fetch(p, hp, base);
+        }
     }
     if (MAPS) {
         if (wave == 0 && c.valid) {
-            float* p = maps + (int64_t)k * 2 * plane + c.col;
-#pragma unroll
-            for (int v = 0; v < V; ++v) { p[v] = chunk[v]; p[plane + v] = carry[v]; }
+            float* to = maps + (int64_t)k * 2 * plane + corner;
+            store_floats<V>(to, floats, chunk);
+            store_floats<V>(to + plane, floats, carry);
         }
     } else if (dstate && wave == 0 && c.valid && first == 0) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) dstate[c.col + v] = carry[v];
+        store_floats<V>(dstate + corner, floats, carry);
     }
 }
 
-// One control step.  state_out may be state: a thread reads its own columns before it writes them.
+// One control step.  state_out may be state: a thread reads its own columns, which are no other's, before it writes them.
 template <typename E, int V>
 __global__ __launch_bounds__(256) void k_memory_step(int64_t N, int64_t D, int64_t x_n, int64_t gate_n, int64_t starts_n, const E* __restrict__ x, const E* __restrict__ gate,
                                                      const uint8_t* __restrict__ starts, const float* state, E* __restrict__ h, float* state_out) {
@@ -389,17 +543,23 @@ __global__ __launch_bounds__(256) void k_memory_step(int64_t N, int64_t D, int64
     const vec xs = *(const vec*)(x + n * x_n + d), gs = *(const vec*)(gate + n * gate_n + d);
     const bool begin = starts && starts[n * starts_n];
     vec o;
+    vec_t<float, V> last;
     float r[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) r[v] = state && !begin ? state[col + v] : 0.0f;
+    for (int v = 0; v < V; ++v) r[v] = 0.0f;
+    if (state) {
+        const vec_t<float, V> f = *(const vec_t<float, V>*)(state + col);
+#pragma unroll
+        for (int v = 0; v < V; ++v) r[v] = get<float, V>(f, v);
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        r[v] = step_of(gate_of(get<E, V>(gs, v)), get<E, V>(xs, v), r[v]);
+        r[v] = step_of(gate_of(get<E, V>(gs, v)), get<E, V>(xs, v), begin ? 0.0f : r[v]);
         put<E, V>(o, v, r[v]);
+        put<float, V>(last, v, r[v]);
     }
     *(vec*)(h + col) = o;
-#pragma unroll
-    for (int v = 0; v < V; ++v) state_out[col + v] = r[v];
+    *(vec_t<float, V>*)(state_out + col) = last;
 }
 
 }  // namespace dlm

@@ -18,8 +18,13 @@ _shape_ref = C.byref
 
 
 def _rows(t):
-    """t with a last axis that lies contiguously (any strides elsewhere)."""
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+    """t with a last axis that lies contiguously and walkers near enough for the kernels' 32-bit row offsets (any strides elsewhere)."""
+    D = t.shape[-1]
+    if t.stride(-1) != 1 and D > 1:
+        return t.contiguous()
+    if t.stride(-2) > 2000000 and t.shape[-2] > 1 and t.stride(-2) >= (1 << 29) // min(t.shape[-2], 256 // D + 2):
+        return t.contiguous()
+    return t
 
 
 def _check(name, x, gate, starts, state, axes):

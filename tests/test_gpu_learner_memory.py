@@ -228,6 +228,17 @@ def test_offsets_beyond_32_bits():
     assert np.all(np.abs(np64(dg[:, cols].cpu()) - rg) <= eh * L / 4 + el * M / 2 + 16 * U * M * L + rounding(torch.bfloat16, rg))
 
 
+def test_walkers_far_apart():
+    """walker-major with more than 2^29 elements under the lanes of a wave: the wrapper makes a time-major copy"""
+    from drloco_amd.memory import _rows
+    far = 1 << 23
+    store = torch.zeros(69 * far + 64, dtype=torch.float16, device='cuda')
+    place = lambda t: store.as_strided(t.shape, (t.shape[2], far, 1)).copy_(t).detach()
+    x, gate, b, st, gh, gl = make(5, 70, 4, torch.float16, seed=3)
+    assert _rows(place(x)).is_contiguous() and not _rows(store.as_strided((5, 2, 4), (4, far, 1))).is_contiguous()
+    check_all(x, gate, b, st, gh, gl, place=lambda t: place(t).clone(memory_format=torch.preserve_format) if t is gh else place(t) if t is x else t.cuda())
+
+
 @pytest.mark.parametrize('dtype', TYPES, ids=str)
 @pytest.mark.parametrize('N,D', [(1, 1), (8, 512), (3, 7), (65, 30), (4096, 64)])
 def test_steps_are_the_rollout_bit_for_bit(N, D, dtype):

@@ -53,7 +53,8 @@ def shape(T=4, N=3, D=8, **kw):
 
 
 BAD_SHAPES = [dict(dtype=3), dict(dtype=-1), dict(reserved=1), dict(T=-1), dict(N=-1), dict(D=-1), dict(T=1 << 41), dict(T=1 << 30, N=1 << 30), dict(x_t=-1), dict(x_n=-8), dict(gate_t=-1),
-              dict(gate_n=-1), dict(starts_t=-1), dict(starts_n=-1), dict(grad_t=-1), dict(grad_n=-1)]
+              dict(gate_n=-1), dict(starts_t=-1), dict(starts_n=-1), dict(grad_t=-1), dict(grad_n=-1),
+              dict(T=(1 << 30) + 1, N=1, D=1), dict(x_n=1 << 28), dict(gate_n=1 << 28), dict(grad_n=1 << 28), dict(T=1, N=1, D=(1 << 29) + 1)]
 
 
 @pytest.mark.parametrize('bad', BAD_SHAPES, ids=str)
