@@ -2,6 +2,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <algorithm>
+#include <cmath>
 #include <string>
 
 #include "drloco_learner.h"
@@ -44,39 +45,43 @@ const char* memory_shape_error(const dl_memory_shape* s) {
     return nullptr;
 }
 
-// The form of a launch: V columns per lane, W waves per workgroup along time, `chunks` workgroups along time.
-struct form { int V, W; int64_t chunk, chunks, blocks; };
+// The form of a launch (dl_memory.hpp): V columns per lane, `blocks` waves across the columns, W waves of a workgroup along time.
+struct form { int V, W; bool parts; int64_t part, chunks, blocks; };
 
-// Columns per lane: eight bytes forward, four backward, where three arrays and the states of a run are held.
+// Columns per lane: eight bytes forward, four backward, where three arrays and the states of a run are held; fewer where the lanes
+// behind the last column of a row and of the last wave would be more than a seventh of all.
 int memory_width(const dl_memory_shape* s, int most) {
+    auto lanes = [&](int V) { return ceil_div(s->N * ceil_div(s->D, V), 64) * 64 * V; };
     int V = most;
-    while (V > s->D) V /= 2;
+    while (V > 1 && (V > s->D || lanes(V) * 7 > lanes(1) * 8)) V /= 2;
     return V;
 }
 int widest_forward(int dtype) { return dtype == DL_F32 ? 2 : 4; }
 int widest_back(int dtype) { return dtype == DL_F32 ? 1 : 2; }
 
-// Columns come first: with a wave for every SIMD unit of the chip (1024) nothing is exchanged between waves.  Below that up to eight
-// waves of a workgroup share the time axis, and with less than 4096 waves then, chunks over workgroups, which cost a second reading
-// of the inputs and never get shorter than one run a wave.
+// With a wave for every SIMD unit of the chip (1024) a wave runs through all of time.  Parts: 4096 waves; at least two runs each, and not
+// so many that the maps before a part (parts / 16 bytes for each of its columns, on average) weigh more than an eighth of its elements.
 form memory_form(const dl_memory_shape* s, int V) {
-    form f;
-    f.V = V;
-    f.blocks = ceil_div(s->N * ceil_div(s->D, V), 64);
+    form f{V, 1, false, s->T, 1, ceil_div(s->N * ceil_div(s->D, V), 64)};
     const int64_t runs = ceil_div(s->T, dlm::MARK);
-    f.W = 1;
-    if (f.blocks < 1024) while (f.W < 8 && f.W < runs) f.W *= 2;
-    const int64_t span = (int64_t)f.W * dlm::MARK;
-    const int64_t spans = ceil_div(s->T, span);
-    f.chunks = 1;
-    if (f.blocks < 512 && spans > 2) f.chunks = std::min<int64_t>(std::min<int64_t>(spans, 256), std::max<int64_t>(1, ceil_div(4096, f.blocks * f.W)));
-    f.chunk = ceil_div(spans, f.chunks) * span;
-    f.chunks = ceil_div(s->T, f.chunk);
+    if (f.blocks >= 1024 || runs <= 1) return f;
+    if (runs <= 8) {
+        while (f.W < runs) f.W *= 2;
+        return f;
+    }
+    f.W = dlm::PARTS;
+    f.parts = true;
+    int64_t parts = ceil_div(4096, f.blocks);
+    parts = std::min(parts, std::max<int64_t>(8, (int64_t)std::sqrt(4.0 * (double)s->T * elem_bytes(s->dtype))));
+    parts = std::max<int64_t>(1, std::min(parts, runs / 2));
+    f.part = ceil_div(runs, parts) * dlm::MARK;
+    f.chunks = ceil_div(ceil_div(s->T, f.part), dlm::PARTS);
     return f;
 }
+int64_t maps_bytes(const dl_memory_shape* s, const form& f) { return f.parts ? f.chunks * (1 + dlm::PARTS) * 2 * s->N * s->D * 4 : 0; }
 
 dlm::shape device_shape(const dl_memory_shape* s, const form& f) {
-    return dlm::shape{s->N, s->D, s->x_t, s->x_n, s->gate_t, s->gate_n, s->starts_t, s->starts_n, s->grad_t, s->grad_n, (int32_t)s->T, (int32_t)f.chunk, (int32_t)f.chunks};
+    return dlm::shape{s->N, s->D, s->x_t, s->x_n, s->gate_t, s->gate_n, s->starts_t, s->starts_n, s->grad_t, s->grad_n, (int32_t)s->T, (int32_t)f.part, (int32_t)f.chunks};
 }
 
 template <int N> struct Int { static constexpr int value = N; };
@@ -172,9 +177,9 @@ int dl_learner_abi_version(void) { return DL_LEARNER_ABI_VERSION; }
 int64_t dl_memory_workspace_bytes(const dl_memory_shape* s) {
     if (const char* e = memory_shape_error(s)) return fail(DL_E_INVAL, e);
     if (s->T == 0 || s->N == 0 || s->D == 0) return 0;
-    int64_t chunks = 1;
-    for (int most : {widest_forward(s->dtype), widest_back(s->dtype)}) chunks = std::max(chunks, memory_form(s, memory_width(s, most)).chunks);
-    return chunks > 1 ? chunks * 2 * s->N * s->D * 4 : 0;
+    int64_t most = 0;
+    for (int V : {widest_forward(s->dtype), widest_back(s->dtype)}) most = std::max(most, maps_bytes(s, memory_form(s, memory_width(s, V))));
+    return most;
 }
 
 int dl_memory_forward(const dl_memory_shape* s, const void* x, const void* gate, const uint8_t* starts, const float* state, void* h, float* state_out, float* marks, void* workspace, void* stream) {
@@ -184,7 +189,7 @@ int dl_memory_forward(const dl_memory_shape* s, const void* x, const void* gate,
     if (!x || !gate || !h) return fail(DL_E_INVAL, "dl_memory_forward: x, gate and h must not be NULL");
     if (state && state == state_out) return fail(DL_E_INVAL, "dl_memory_forward: state_out may not be state");
     const form f = memory_form(s, memory_width(s, widest_forward(s->dtype)));
-    if (f.chunks > 1 && !workspace) return fail(DL_E_INVAL, "dl_memory_forward: workspace must not be NULL (dl_memory_workspace_bytes)");
+    if (f.parts && !workspace) return fail(DL_E_INVAL, "dl_memory_forward: workspace must not be NULL (dl_memory_workspace_bytes)");
     if (f.blocks > 0x7fffffff) return fail(DL_E_INVAL, "dl_memory_forward: N * D too large");
     const dlm::shape d = device_shape(s, f);
     const dim3 grid((unsigned)f.blocks, (unsigned)f.chunks);
@@ -192,11 +197,14 @@ int dl_memory_forward(const dl_memory_shape* s, const void* x, const void* gate,
     with_type(s->dtype, [&](auto e) { with_width<widest<decltype(e)>()>(f.V, [&](auto v) {
         using E = decltype(e);
         constexpr int V = decltype(v)::value;
-        if (f.W == 1) return dlm::k_memory_run<E, V><<<grid, 64, 0, st>>>(d, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks);
-        with_waves(f.W, [&](auto w) {
+        if (f.parts) {
+            dlm::k_memory_maps<E, V, false><<<grid, 64 * dlm::PARTS, 0, st>>>(d, (const E*)x, (const E*)gate, nullptr, starts, (float*)workspace);
+            dlm::k_memory_run<E, V, dlm::PARTS><<<grid, 64 * dlm::PARTS, 0, st>>>(d, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks, (const float*)workspace);
+        } else if (f.W == 1) {
+            dlm::k_memory_run<E, V, 1><<<grid, 64, 0, st>>>(d, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks, nullptr);
+        } else with_waves(f.W, [&](auto w) {
             constexpr int W = decltype(w)::value;
-            if (f.chunks > 1) dlm::k_memory_forward<E, V, W, true><<<dim3(grid.x, grid.y - 1), 64 * W, 0, st>>>(d, (const E*)x, (const E*)gate, starts, nullptr, nullptr, nullptr, nullptr, (float*)workspace);
-            dlm::k_memory_forward<E, V, W, false><<<grid, 64 * W, 0, st>>>(d, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks, (float*)workspace);
+            dlm::k_memory_short<E, V, W><<<grid, 64 * W, 0, st>>>(d, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks);
         });
     }); });
     return launched("dl_memory_forward");
@@ -210,7 +218,7 @@ int dl_memory_backward(const dl_memory_shape* s, const void* x, const void* gate
     if (!x || !gate || !marks || !dx || !dgate) return fail(DL_E_INVAL, "dl_memory_backward: x, gate, marks, dx and dgate must not be NULL");
     if (grad_state && grad_state == dstate) return fail(DL_E_INVAL, "dl_memory_backward: dstate may not be grad_state");
     const form f = memory_form(s, memory_width(s, widest_back(s->dtype)));
-    if (f.chunks > 1 && !workspace) return fail(DL_E_INVAL, "dl_memory_backward: workspace must not be NULL (dl_memory_workspace_bytes)");
+    if (f.parts && !workspace) return fail(DL_E_INVAL, "dl_memory_backward: workspace must not be NULL (dl_memory_workspace_bytes)");
     if (f.blocks > 0x7fffffff) return fail(DL_E_INVAL, "dl_memory_backward: N * D too large");
     const dlm::shape d = device_shape(s, f);
     const dim3 grid((unsigned)f.blocks, (unsigned)f.chunks);
@@ -218,11 +226,14 @@ int dl_memory_backward(const dl_memory_shape* s, const void* x, const void* gate
     with_type(s->dtype, [&](auto e) { with_width<widest<decltype(e)>() / 2>(f.V, [&](auto v) {
         using E = decltype(e);
         constexpr int V = decltype(v)::value;
-        if (f.W == 1) return dlm::k_memory_backward<E, V, 1, false><<<grid, 64, 0, st>>>(d, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, grad_state, (E*)dx, (E*)dgate, dstate, nullptr);
-        with_waves(f.W, [&](auto w) {
+        if (f.parts) {
+            dlm::k_memory_maps<E, V, true><<<grid, 64 * dlm::PARTS, 0, st>>>(d, (const E*)x, (const E*)gate, (const E*)grad_h, starts, (float*)workspace);
+            dlm::k_memory_run_back<E, V, dlm::PARTS><<<grid, 64 * dlm::PARTS, 0, st>>>(d, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, grad_state, (E*)dx, (E*)dgate, dstate, (const float*)workspace);
+        } else if (f.W == 1) {
+            dlm::k_memory_run_back<E, V, 1><<<grid, 64, 0, st>>>(d, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, grad_state, (E*)dx, (E*)dgate, dstate, nullptr);
+        } else with_waves(f.W, [&](auto w) {
             constexpr int W = decltype(w)::value;
-            if (f.chunks > 1) dlm::k_memory_backward<E, V, W, true><<<grid, 64 * W, 0, st>>>(d, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, nullptr, nullptr, nullptr, nullptr, (float*)workspace);
-            dlm::k_memory_backward<E, V, W, false><<<grid, 64 * W, 0, st>>>(d, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, grad_state, (E*)dx, (E*)dgate, dstate, (float*)workspace);
+            dlm::k_memory_short_back<E, V, W><<<grid, 64 * W, 0, st>>>(d, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, grad_state, (E*)dx, (E*)dgate, dstate);
         });
     }); });
     return launched("dl_memory_backward");

@@ -4,11 +4,13 @@
 //     l[t] = dh[t] + c[t+1],  c[t] = start ? 0 : a l[t]:      dx = s l,   dg = (h' - x) a s l,   dstate = c[0]
 //
 // Bound by memory (three elements moved per step forward, five backward) with the arithmetic, 20 to 40 operations per element, close
-// behind.  Every element is loaded once: a wave keeps MARK steps of 64 x V columns in registers.  With enough columns for the chip a
-// wave runs through time by itself and loads the next run while it computes this one.  With fewer, the waves of a workgroup take
-// consecutive runs, reduce each to its affine map, exchange the maps through LDS, and finish their steps from the registers.
-// With fewer still the time axis is also cut into chunks over workgroups: a first kernel reduces every chunk to its map, the second
-// starts from the maps before it.
+// behind.  A wave takes 64 x V columns through time, MARK steps (a run) in registers and the loads of the next ones under way.
+// Three forms, by the number of such waves ("blocks") and of steps:
+//   whole   enough blocks for the chip: a wave runs through all of time, every element is loaded once;
+//   short   few blocks, at most eight runs: the waves of a workgroup take a run each, reduce it to its affine map, exchange the maps
+//           through LDS and finish their steps from the registers: every element is loaded once here too;
+//   parts   few blocks, many steps: the time axis is cut into parts.  A first kernel reduces every part to its map (two of three
+//           elements are read, in the backward direction two of five), the second starts each part from the maps before it.
 //
 // Rounding.  The smaller of a and s is computed as e / (1 + e), e = exp(-|g|), and both products go through it:
 //     g >= 0:  h = h' + s (x - h'),  c = l - s l        g < 0:  h = x + a (h' - x),  c = a l
@@ -24,6 +26,7 @@
 namespace dlm {
 
 constexpr int MARK = 16;          // steps of a wave's run, and between two saved states
+constexpr int PARTS = 8;          // waves of a workgroup that shares the time axis
 
 template <typename E, int V> struct vec { typedef E type __attribute__((ext_vector_type(V), aligned(sizeof(E)))); };
 template <typename E> struct vec<E, 1> { typedef E type; };
@@ -42,7 +45,7 @@ struct shape {
     int64_t N, D;
     int64_t x_t, x_n, gate_t, gate_n, starts_t, starts_n, grad_t, grad_n;
     int32_t T;
-    int32_t chunk, chunks;        // steps of a workgroup (a multiple of waves * MARK), workgroups along time
+    int32_t part, chunks;         // steps of a part (a multiple of MARK), workgroups of PARTS parts along time
 };
 
 // min(a, s) with the sign of the gate.
@@ -116,52 +119,74 @@ template <typename T> __device__ __forceinline__ void store_at(void* base, uint3
     *(DLM_GLOBAL T*)(p + bytes) = v;
 }
 
-// The state (or gradient) that enters the run of each wave from the maps of the waves before it, and the one behind the last.
-// `from` = how many maps come first in the order of the recurrence for this wave.
-template <int V>
-__device__ __forceinline__ void join(const float (*la)[64 * V], const float (*lb)[64 * V], int lane, int waves, int from, const float (&carry)[V], float (&mine)[V], float (&next)[V], bool back) {
+// The value that enters the run of each wave from the maps of the waves before it (`before` of them, in the order of the
+// recurrence), and the one behind the last.
+template <int V, bool BACK>
+__device__ __forceinline__ void join(const float (*la)[64 * V], const float (*lb)[64 * V], int lane, int waves, int before, const float (&carry)[V], float (&mine)[V], float (&next)[V]) {
 #pragma unroll
     for (int v = 0; v < V; ++v) next[v] = mine[v] = carry[v];
     for (int i = 0; i < waves; ++i) {
-        const int w = back ? waves - 1 - i : i;
+        const int w = BACK ? waves - 1 - i : i;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             next[v] = apply(la[w][v * 64 + lane], lb[w][v * 64 + lane], next[v]);
-            if (i + 1 == from) mine[v] = next[v];
+            if (i + 1 == before) mine[v] = next[v];
         }
     }
 }
 
-// Maps of whole chunks -> the value that enters chunk k, by the whole workgroup: every wave joins a part of the chunks before.
-// maps: float [chunks][2][N * D].
+template <int V> __device__ __forceinline__ void load_floats(float (&to)[V], const float* base, uint32_t bytes) {
+    const vec_t<float, V> f = load_at<vec_t<float, V>>(base, bytes);
+#pragma unroll
+    for (int v = 0; v < V; ++v) to[v] = get<float, V>(f, v);
+}
+template <int V> __device__ __forceinline__ void store_floats(float* base, uint32_t bytes, const float (&from)[V]) {
+    vec_t<float, V> f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) put<float, V>(f, v, from[v]);
+    store_at<vec_t<float, V>>(base, bytes, f);
+}
+
+// Maps in memory: float [chunks][2][N * D] of the chunks, behind them [chunks * PARTS][2][N * D] of the parts; `maps` is at channel 0 of
+// the first walker.  The value that enters a wave's part: the workgroup joins the chunks before, a share per wave, and then
+// each wave the parts before its own.
 template <int V, bool BACK>
-__device__ __forceinline__ void enter(const float* maps, int64_t plane, int k, int chunks, uint32_t floats, int waves, int wave, int lane, float (*la)[64 * V], float (*lb)[64 * V], float (&carry)[V]) {
+__device__ __forceinline__ void enter(const float* maps, int64_t plane, int k, int chunks, uint32_t floats, int wave, int lane, float (*la)[64 * V], float (*lb)[64 * V], float (&carry)[V]) {
     const int before = BACK ? chunks - 1 - k : k;
-    if (before == 0) return;
-    float A[V], B[V];
+    if (before > 0) {
+        float A[V], B[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) { A[v] = 0.0f; B[v] = 0.0f; }
-    const int lo = (int)((int64_t)before * wave / waves), hi = (int)((int64_t)before * (wave + 1) / waves);
+        for (int v = 0; v < V; ++v) { A[v] = 0.0f; B[v] = 0.0f; }
+        const int lo = before * wave / PARTS, hi = before * (wave + 1) / PARTS;
 #pragma unroll 4
-    for (int i = lo; i < hi; ++i) {
-        const int j = BACK ? chunks - 1 - i : i;
-        const float* p = maps + (int64_t)j * 2 * plane;          // (maps: at channel 0 of the first walker)
-        const vec_t<float, V> ma = load_at<vec_t<float, V>>(p, floats), mb = load_at<vec_t<float, V>>(p + plane, floats);
+        for (int i = lo; i < hi; ++i) {
+            const float* p = maps + (int64_t)(BACK ? chunks - 1 - i : i) * 2 * plane;
+            float a[V], b[V];
+            load_floats<V>(a, p, floats);
+            load_floats<V>(b, p + plane, floats);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const float a = get<float, V>(ma, v), b = get<float, V>(mb, v);
-            B[v] = apply(a, b, B[v]);
-            A[v] = after(A[v], a);
+            for (int v = 0; v < V; ++v) {
+                B[v] = apply(a[v], b[v], B[v]);
+                A[v] = after(A[v], a[v]);
+            }
         }
+#pragma unroll
+        for (int v = 0; v < V; ++v) { la[wave][v * 64 + lane] = A[v]; lb[wave][v * 64 + lane] = B[v]; }
+        __syncthreads();
+        float mine[V], next[V];
+        join<V, false>(la, lb, lane, PARTS, 0, carry, mine, next);
+#pragma unroll
+        for (int v = 0; v < V; ++v) carry[v] = next[v];
     }
+    const float* parts = maps + ((int64_t)chunks + (int64_t)k * PARTS) * 2 * plane;
+    for (int i = 0; i < (BACK ? PARTS - 1 - wave : wave); ++i) {
+        const float* p = parts + (int64_t)(BACK ? PARTS - 1 - i : i) * 2 * plane;
+        float a[V], b[V];
+        load_floats<V>(a, p, floats);
+        load_floats<V>(b, p + plane, floats);
 #pragma unroll
-    for (int v = 0; v < V; ++v) { la[wave][v * 64 + lane] = A[v]; lb[wave][v * 64 + lane] = B[v]; }
-    __syncthreads();
-    float mine[V], next[V];
-    join<V>(la, lb, lane, waves, 0, carry, mine, next, false);
-#pragma unroll
-    for (int v = 0; v < V; ++v) carry[v] = next[v];
-    __syncthreads();
+        for (int v = 0; v < V; ++v) carry[v] = apply(a[v], b[v], carry[v]);
+    }
 }
 
 // Between the passes over a run: the comparisons of the first are made again instead of being kept, a pair of scalar registers each.
@@ -240,27 +265,94 @@ template <typename E, int V, int R, bool X, bool G> struct rows {
     }
 };
 
-template <int V> __device__ __forceinline__ void load_floats(float (&to)[V], const float* base, uint32_t bytes) {
-    const vec_t<float, V> f = load_at<vec_t<float, V>>(base, bytes);
-#pragma unroll
-    for (int v = 0; v < V; ++v) to[v] = get<float, V>(f, v);
-}
-template <int V> __device__ __forceinline__ void store_floats(float* base, uint32_t bytes, const float (&from)[V]) {
-    vec_t<float, V> f;
-#pragma unroll
-    for (int v = 0; v < V; ++v) put<float, V>(f, v, from[v]);
-    store_at<vec_t<float, V>>(base, bytes, f);
-}
-
 struct yes { static constexpr bool value = true; };
 struct no { static constexpr bool value = false; };
 
-// ---- enough columns: a wave runs through all of time by itself, half a run ahead with its loads -----------------------------------
-template <typename E, int V>
-__global__ __launch_bounds__(64) void k_memory_run(shape s, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ state,
-                                                   E* __restrict__ h, float* __restrict__ state_out, float* __restrict__ marks) {
+// ---- parts: every part and every chunk of PARTS of them to its map ---------------------------------------------------------------
+template <typename E, int V, bool BACK>
+__global__ __launch_bounds__(64 * PARTS, 4) void k_memory_maps(shape s, const E* __restrict__ x, const E* __restrict__ gate, const E* __restrict__ grad_h, const uint8_t* __restrict__ starts, float* __restrict__ maps) {
+    __shared__ float la[PARTS][64 * V], lb[PARTS][64 * V];
+    constexpr int R = MARK / 2;
+    typedef rows<E, V, R, !BACK, BACK> half;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), k = blockIdx.y;
+    const columns<V> c(s.N, s.D);
+    const int64_t plane = s.N * s.D, corner = c.n0 * s.D;
+    const uint32_t floats = c.template bytes<float>(s.D);
+    const int first = (k * PARTS + wave) * s.part, last = min(first + s.part, s.T);
+    factor A[V];
+    float B[V];
+    uint32_t begun = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) B[v] = 0.0f;
+    auto run = [&](half& r, int t0) {
+        const int len = max(0, min(R, last - t0));
+        const uint32_t begin = r.begins(c);
+        begun |= begin;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int t = BACK ? R - 1 - i : i;
+            if (t < len) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const float m = gate_of(get<E, V>(r.g[t], v));
+                    if (BACK) B[v] = (begin >> t) & 1 ? 0.0f : decay_of(m, get<E, V>(r.d[t], v) + B[v]);
+                    else B[v] = step_of(m, get<E, V>(r.x[t], v), (begin >> t) & 1 ? 0.0f : B[v]);
+                    A[v].step(m);
+                }
+            }
+        }
+    };
+    if (first < last) {
+        half p, q;
+        if (BACK) {
+            int t0 = first + (last - first - 1) / R * R;
+            p.load(s, c, t0, last, x, gate, grad_h, starts);
+            for (;;) {
+                q.load(s, c, max(t0 - R, first), last, x, gate, grad_h, starts);
+                run(p, t0);
+                if ((t0 -= R) < first) break;
+                p.load(s, c, max(t0 - R, first), last, x, gate, grad_h, starts);
+                run(q, t0);
+                if ((t0 -= R) < first) break;
+            }
+        } else {
+            p.load(s, c, first, last, x, gate, grad_h, starts);
+            for (int t0 = first; t0 < last; t0 += MARK) {
+                q.load(s, c, t0 + R, last, x, gate, grad_h, starts);
+                run(p, t0);
+                p.load(s, c, t0 + MARK, last, x, gate, grad_h, starts);
+                run(q, t0 + R);
+            }
+        }
+    }
+    float held[V], zero[V], mine[V], next[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) { held[v] = A[v].held(begun != 0); zero[v] = 0.0f; }
+#pragma unroll
+    for (int v = 0; v < V; ++v) { la[wave][v * 64 + lane] = held[v]; lb[wave][v * 64 + lane] = B[v]; }
+    __syncthreads();
+    float* part = maps + ((int64_t)s.chunks + (int64_t)k * PARTS + wave) * 2 * plane + corner;
+    if (c.valid) { store_floats<V>(part, floats, held); store_floats<V>(part + plane, floats, B); }
+    if (wave == 0) {
+        join<V, BACK>(la, lb, lane, PARTS, 0, zero, mine, next);
+#pragma unroll
+        for (int v = 0; v < V; ++v) held[v] = 0.0f;
+        for (int w = 0; w < PARTS; ++w) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) held[v] = after(held[v], la[w][v * 64 + lane]);
+        }
+        float* chunk = maps + (int64_t)k * 2 * plane + corner;
+        if (c.valid) { store_floats<V>(chunk, floats, held); store_floats<V>(chunk + plane, floats, next); }
+    }
+}
+
+// ---- whole (W = 1) and parts (W = PARTS): a wave runs through its steps, half a run ahead with its loads --------------------------------
+template <typename E, int V, int W>
+__global__ __launch_bounds__(64 * W, W == 1 ? 1 : 4) void k_memory_run(shape s, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ state,
+                                                                       E* __restrict__ h, float* __restrict__ state_out, float* __restrict__ marks, const float* __restrict__ maps) {
     typedef vec_t<E, V> vec;
     constexpr int R = MARK / 2;
+    typedef rows<E, V, R, true, false> half;
     const columns<V> c(s.N, s.D);
     const int64_t plane = s.N * s.D, corner = c.n0 * s.D;
     const uint32_t elems = c.template bytes<E>(s.D), floats = c.template bytes<float>(s.D);
@@ -268,7 +360,15 @@ __global__ __launch_bounds__(64) void k_memory_run(shape s, const E* __restrict_
 #pragma unroll
     for (int v = 0; v < V; ++v) now[v] = 0.0f;
     if (state) load_floats<V>(now, state + corner, floats);
-    typedef rows<E, V, R, true, false> half;
+    int first = 0, last = s.T;
+    if constexpr (W > 1) {
+        __shared__ float la[W][64 * V], lb[W][64 * V];
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), k = blockIdx.y;
+        enter<V, false>(maps + corner, plane, k, s.chunks, floats, wave, lane, la, lb, now);
+        first = (k * W + wave) * s.part;
+        last = min(first + s.part, s.T);
+        if (first >= last) return;
+    }
     auto steps = [&](const half& r, int t0, int len, auto all, uint32_t begin) {
         E* ph = h + (int64_t)t0 * plane + corner;
 #pragma unroll
@@ -287,249 +387,205 @@ __global__ __launch_bounds__(64) void k_memory_run(shape s, const E* __restrict_
         }
     };
     auto run = [&](const half& r, int t0) {          // whole and without a beginning, as nearly always, or not
-        const int len = max(0, min(R, s.T - t0));
+        const int len = max(0, min(R, last - t0));
         const uint32_t begin = r.begins(c);
         if (len == R && __ballot(begin != 0) == 0) steps(r, t0, len, yes(), 0u); else steps(r, t0, len, no(), begin);
     };
     half p, q;
-    p.load(s, c, 0, s.T, x, gate, nullptr, starts);
-    for (int t0 = 0; t0 < s.T; t0 += MARK) {
-        q.load(s, c, t0 + R, s.T, x, gate, nullptr, starts);
+    p.load(s, c, first, last, x, gate, nullptr, starts);
+    for (int t0 = first; t0 < last; t0 += MARK) {
+        q.load(s, c, t0 + R, last, x, gate, nullptr, starts);
         if (marks && c.valid) store_floats<V>(marks + (int64_t)(t0 / MARK) * plane + corner, floats, now);
         run(p, t0);
-        p.load(s, c, t0 + MARK, s.T, x, gate, nullptr, starts);
+        p.load(s, c, t0 + MARK, last, x, gate, nullptr, starts);
         run(q, t0 + R);
     }
-    if (state_out && c.valid) store_floats<V>(state_out + corner, floats, now);
+    if (state_out && c.valid && last == s.T) store_floats<V>(state_out + corner, floats, now);
 }
 
-// ---- W waves of a workgroup take consecutive runs.  MAPS: only reduce the chunk to its map -----------------------------------------
-template <typename E, int V, int W, bool MAPS>
-__global__ __launch_bounds__(64 * W) void k_memory_forward(shape s, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ state,
-                                                           E* __restrict__ h, float* __restrict__ state_out, float* __restrict__ marks, float* __restrict__ maps) {
+// ---- short: W waves of a workgroup take one run each ----------------------------------------------------------------------------------
+template <typename E, int V, int W>
+__global__ __launch_bounds__(64 * W) void k_memory_short(shape s, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ state,
+                                                         E* __restrict__ h, float* __restrict__ state_out, float* __restrict__ marks) {
     typedef vec_t<E, V> vec;
     __shared__ float la[W][64 * V], lb[W][64 * V];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const columns<V> c(s.N, s.D);
     const int64_t plane = s.N * s.D, corner = c.n0 * s.D;
     const uint32_t elems = c.template bytes<E>(s.D), floats = c.template bytes<float>(s.D);
-    const int k = blockIdx.y;
-    const int first = k * s.chunk, last = min(first + s.chunk, s.T);
-    float carry[V], chunk[V];
+    float carry[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) { carry[v] = 0.0f; chunk[v] = 0.0f; }
-    if (!MAPS) {
-        if (state) load_floats<V>(carry, state + corner, floats);
-        if (s.chunks > 1) enter<V, false>(maps + corner, plane, k, s.chunks, floats, W, wave, lane, la, lb, carry);
+    for (int v = 0; v < V; ++v) carry[v] = 0.0f;
+    if (state) load_floats<V>(carry, state + corner, floats);
+    const int t0 = wave * MARK, len = max(0, min(MARK, s.T - t0));
+    rows<E, V, MARK, true, false> r;
+    r.load(s, c, t0, s.T, x, gate, nullptr, starts);
+    float m[MARK][V];
+    uint32_t begin = r.begins(c);
+    factor A[V]; float B[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) B[v] = 0.0f;
+#pragma unroll
+    for (int t = 0; t < MARK; ++t) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            m[t][v] = t < len ? gate_of(get<E, V>(r.g[t], v)) : 0.0f;          // (behind the end: an open gate, h stays as it is)
+            B[v] = step_of(m[t][v], get<E, V>(r.x[t], v), (begin >> t) & 1 ? 0.0f : B[v]);
+            A[v].step(m[t][v]);
+        }
+        pause<V>(t);
     }
-    for (int base = first; base < last; base += W * MARK) {
-        const int t0 = base + wave * MARK;
-        const int len = max(0, min(MARK, last - t0));
-        rows<E, V, MARK, true, false> r;
-        r.load(s, c, t0, last, x, gate, nullptr, starts);
-        float m[MARK][V];
-        uint32_t begin = r.begins(c);
-        factor A[V]; float B[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) B[v] = 0.0f;
+    for (int v = 0; v < V; ++v) { la[wave][v * 64 + lane] = A[v].held(begin != 0); lb[wave][v * 64 + lane] = B[v]; }
+    forget<V>(m, begin); r.forget();
+    __syncthreads();
+    float in[V], next[V];
+    join<V, false>(la, lb, lane, W, wave, carry, in, next);
+    if (marks && c.valid && len > 0) store_floats<V>(marks + (int64_t)wave * plane + corner, floats, in);
+    E* ph = h + (int64_t)t0 * plane + corner;
 #pragma unroll
-        for (int t = 0; t < MARK; ++t) {
+    for (int t = 0; t < MARK; ++t) {
+        if (t < len) {
+            vec o;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                m[t][v] = t < len ? gate_of(get<E, V>(r.g[t], v)) : 0.0f;          // (behind the end: an open gate, h stays as it is)
-                B[v] = step_of(m[t][v], get<E, V>(r.x[t], v), (begin >> t) & 1 ? 0.0f : B[v]);
-                A[v].step(m[t][v]);
+                in[v] = step_of(m[t][v], get<E, V>(r.x[t], v), (begin >> t) & 1 ? 0.0f : in[v]);
+                put<E, V>(o, v, in[v]);
             }
-            pause<V>(t);
-        }
-#pragma unroll
-        for (int v = 0; v < V; ++v) { la[wave][v * 64 + lane] = A[v].held(begin != 0); lb[wave][v * 64 + lane] = B[v]; }
-        forget<V>(m, begin); r.forget();
-        __syncthreads();
-        float in[V], next[V];
-        join<V>(la, lb, lane, W, wave, carry, in, next, false);
-        if (MAPS) {
-            for (int w = 0; w < W; ++w) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) chunk[v] = after(chunk[v], la[w][v * 64 + lane]);
-            }
-        }
-#pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = next[v];
-        __syncthreads();
-        if (!MAPS) {
-            if (marks && c.valid && len > 0) store_floats<V>(marks + (int64_t)(t0 / MARK) * plane + corner, floats, in);
-            E* ph = h + (int64_t)t0 * plane + corner;
-#pragma unroll
-            for (int t = 0; t < MARK; ++t) {
-                if (t < len) {
-                    vec o;
-#pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        in[v] = step_of(m[t][v], get<E, V>(r.x[t], v), (begin >> t) & 1 ? 0.0f : in[v]);
-                        put<E, V>(o, v, in[v]);
-                    }
-                    if (c.valid) store_at<vec>(ph, elems, o);
-                    ph += plane;
-                }
-            }
+            if (c.valid) store_at<vec>(ph, elems, o);
+            ph += plane;
         }
     }
-    if (MAPS) {
-        if (wave == 0 && c.valid) {
-            float* p = maps + (int64_t)k * 2 * plane + corner;
-            store_floats<V>(p, floats, chunk);
-            store_floats<V>(p + plane, floats, carry);
-        }
-    } else if (state_out && wave == 0 && c.valid && last == s.T) {
-        store_floats<V>(state_out + corner, floats, carry);
-    }
+    if (state_out && wave == 0 && c.valid) store_floats<V>(state_out + corner, floats, next);
 }
 
-// ---- gradients.  W = 1: a wave runs through all of time by itself, a run ahead with its loads ---------------------------------------
-template <typename E, int V, int W, bool MAPS>
-__global__ __launch_bounds__(64 * W) void k_memory_backward(shape s, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ marks,
-                                                            const E* __restrict__ grad_h, const float* __restrict__ grad_state, E* __restrict__ dx, E* __restrict__ dgate,
-                                                            float* __restrict__ dstate, float* __restrict__ maps) {
+// ---- gradients of a run.  hs: the states before each step, recomputed from the saved one --------------------------------------------------
+template <typename E, int V> struct run_back {
     typedef vec_t<E, V> vec;
-    typedef rows<E, V, MARK, !MAPS, true> run;
-    __shared__ float la[W][64 * V], lb[W][64 * V];
-    const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const columns<V> c(s.N, s.D);
-    const int64_t plane = s.N * s.D, corner = c.n0 * s.D;
-    const uint32_t elems = c.template bytes<E>(s.D), floats = c.template bytes<float>(s.D);
-    const int k = blockIdx.y;
-    const int first = k * s.chunk, last = min(first + s.chunk, s.T);
-    float carry[V], chunk[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) { carry[v] = 0.0f; chunk[v] = 0.0f; }
-    if (!MAPS) {
-        if (grad_state) load_floats<V>(carry, grad_state + corner, floats);
-        if (s.chunks > 1) enter<V, true>(maps + corner, plane, k, s.chunks, floats, W, wave, lane, la, lb, carry);
+    rows<E, V, MARK, true, true> r;
+    float h0[V];
+    __device__ __forceinline__ void load(const shape& s, const columns<V>& c, int t0, int last, const E* x, const E* gate, const E* grad_h, const uint8_t* starts, const float* marks, int64_t plane, int64_t corner, uint32_t floats) {
+        r.load(s, c, t0, last, x, gate, grad_h, starts);
+        load_floats<V>(h0, marks + (int64_t)(min(t0, last - 1) / MARK) * plane + corner, floats);
     }
-    auto one = [&](run& r, int base, const float (&h0)[V]) {
-        const int t0 = base + wave * MARK;
-        const int len = max(0, min(MARK, last - t0));
+    __device__ __forceinline__ uint32_t states(const columns<V>& c, int len, float (&m)[MARK][V], float (&hs)[MARK][V]) {
         uint32_t begin = r.begins(c);
-        float m[MARK][V], hs[MARK][V], h[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = h0[v];
 #pragma unroll
         for (int t = 0; t < MARK; ++t) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 m[t][v] = t < len ? gate_of(get<E, V>(r.g[t], v)) : 0.0f;
-                if (!MAPS) {
-                    hs[t][v] = (begin >> t) & 1 ? 0.0f : h[v];
-                    h[v] = step_of(m[t][v], get<E, V>(r.x[t], v), hs[t][v]);
-                }
+                hs[t][v] = (begin >> t) & 1 ? 0.0f : h0[v];
+                h0[v] = step_of(m[t][v], get<E, V>(r.x[t], v), hs[t][v]);
             }
             pause<V>(t);
         }
-        if (!MAPS) { forget<V>(m, begin); r.forget(); }
-        float in[V];
-        if (W > 1 || MAPS) {
-            factor A[V]; float B[V];
+        forget<V>(m, begin); r.forget();
+        return begin;
+    }
+    // in: the gradient that arrives from behind the run, and then the one that leaves in front of it
+    __device__ __forceinline__ void finish(const columns<V>& c, int t0, int len, uint32_t begin, const float (&m)[MARK][V], const float (&hs)[MARK][V], float (&in)[V], E* dx, E* dgate, int64_t plane, int64_t corner, uint32_t elems) {
+        dx += (int64_t)(t0 + len - 1) * plane + corner;
+        dgate += (int64_t)(t0 + len - 1) * plane + corner;
 #pragma unroll
-            for (int v = 0; v < V; ++v) B[v] = 0.0f;
-#pragma unroll
-            for (int t = MARK - 1; t >= 0; --t) {
+        for (int t = MARK - 1; t >= 0; --t) {
+            if (t < len) {
+                vec ox, og;
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    B[v] = (begin >> t) & 1 ? 0.0f : decay_of(m[t][v], (t < len ? get<E, V>(r.d[t], v) : 0.0f) + B[v]);
-                    A[v].step(m[t][v]);
+                    const float l = get<E, V>(r.d[t], v) + in[v];
+                    const float q = fabsf(m[t][v]), w = q * l, o = l - w;          // the smaller and the larger share
+                    put<E, V>(ox, v, keeps(m[t][v]) ? w : o);
+                    put<E, V>(og, v, (hs[t][v] - get<E, V>(r.x[t], v)) * fmaf(-q, w, w));
+                    in[v] = (begin >> t) & 1 ? 0.0f : keeps(m[t][v]) ? o : w;
                 }
-                pause<V>(MARK - 1 - t);
+                if (c.valid) { store_at<vec>(dx, elems, ox); store_at<vec>(dgate, elems, og); }
+                dx -= plane; dgate -= plane;
             }
-#pragma unroll
-            for (int v = 0; v < V; ++v) { la[wave][v * 64 + lane] = A[v].held(begin != 0); lb[wave][v * 64 + lane] = B[v]; }
-            if (!MAPS) { forget<V>(m, begin); r.forget(); }
-            __syncthreads();
-            float next[V];
-            join<V>(la, lb, lane, W, W - 1 - wave, carry, in, next, true);
-            if (MAPS) {
-                for (int w = 0; w < W; ++w) {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) chunk[v] = after(chunk[v], la[w][v * 64 + lane]);
-                }
-            }
-#pragma unroll
-            for (int v = 0; v < V; ++v) carry[v] = next[v];
-            __syncthreads();
-        } else {
-#pragma unroll
-            for (int v = 0; v < V; ++v) in[v] = carry[v];
-        }
-        if (!MAPS) {
-            E* pdx = dx + (int64_t)(t0 + len - 1) * plane + corner;
-            E* pdg = dgate + (int64_t)(t0 + len - 1) * plane + corner;
-#pragma unroll
-            for (int t = MARK - 1; t >= 0; --t) {
-                if (t < len) {
-                    vec ox, og;
-#pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        const float l = get<E, V>(r.d[t], v) + in[v];
-                        const float q = fabsf(m[t][v]), w = q * l, o = l - w;          // the smaller and the larger share
-                        put<E, V>(ox, v, keeps(m[t][v]) ? w : o);
-                        put<E, V>(og, v, (hs[t][v] - get<E, V>(r.x[t], v)) * fmaf(-q, w, w));
-                        in[v] = (begin >> t) & 1 ? 0.0f : keeps(m[t][v]) ? o : w;
-                    }
-                    if (c.valid) { store_at<vec>(pdx, elems, ox); store_at<vec>(pdg, elems, og); }
-                    pdx -= plane; pdg -= plane;
-                }
-                pause<V>(MARK - 1 - t);
-            }
-            if (W == 1) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) carry[v] = in[v];
-            }
-        }
-    };
-    auto get_marks = [&](float (&h0)[V], int base) {
-        if (!MAPS) load_floats<V>(h0, marks + (int64_t)(min(base + wave * MARK, last - 1) / MARK) * plane + corner, floats);
-        else {
-#pragma unroll
-            for (int v = 0; v < V; ++v) h0[v] = 0.0f;
-        }
-    };
-    const int span = W * MARK;
-    int base = first + (last - first - 1) / span * span;
-    auto fetch = [&](run& r, float (&h0)[V], int at_) {          // (the one behind the first run: that again)
-        const int t = max(at_, first) + wave * MARK;
-        r.load(s, c, t, last, x, gate, grad_h, starts);
-        get_marks(h0, max(at_, first));
-    };
-    run p;
-    float hp[V];
-    fetch(p, hp, base);
-    if constexpr (W == 1) {
-        run q;
-        float hq[V];
-        for (;;) {
-            fetch(q, hq, base - span);
-            one(p, base, hp);
-            if ((base -= span) < first) break;
-            fetch(p, hp, base - span);
-            one(q, base, hq);
-            if ((base -= span) < first) break;
-        }
-    } else {
-        for (;;) {
-            one(p, base, hp);
-            if ((base -= span) < first) break;
-            fetch(p, hp, base);
+            pause<V>(MARK - 1 - t);
         }
     }
-    if (MAPS) {
-        if (wave == 0 && c.valid) {
-            float* to = maps + (int64_t)k * 2 * plane + corner;
-            store_floats<V>(to, floats, chunk);
-            store_floats<V>(to + plane, floats, carry);
-        }
-    } else if (dstate && wave == 0 && c.valid && first == 0) {
-        store_floats<V>(dstate + corner, floats, carry);
+};
+
+// whole (W = 1) and parts (W = PARTS): a wave runs back through its steps, a run ahead with its loads
+template <typename E, int V, int W>
+__global__ __launch_bounds__(64 * W) void k_memory_run_back(shape s, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ marks,
+                                                            const E* __restrict__ grad_h, const float* __restrict__ grad_state, E* __restrict__ dx, E* __restrict__ dgate, float* __restrict__ dstate,
+                                                            const float* __restrict__ maps) {
+    const columns<V> c(s.N, s.D);
+    const int64_t plane = s.N * s.D, corner = c.n0 * s.D;
+    const uint32_t elems = c.template bytes<E>(s.D), floats = c.template bytes<float>(s.D);
+    float in[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) in[v] = 0.0f;
+    if (grad_state) load_floats<V>(in, grad_state + corner, floats);
+    int first = 0, last = s.T;
+    if constexpr (W > 1) {
+        __shared__ float la[W][64 * V], lb[W][64 * V];
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), k = blockIdx.y;
+        enter<V, true>(maps + corner, plane, k, s.chunks, floats, wave, lane, la, lb, in);
+        first = (k * W + wave) * s.part;
+        last = min(first + s.part, s.T);
+        if (first >= last) return;
     }
+    auto load = [&](run_back<E, V>& b, int t0) { b.load(s, c, max(t0, first), last, x, gate, grad_h, starts, marks, plane, corner, floats); };          // (in front of the first run: that again)
+    auto one = [&](run_back<E, V>& b, int t0) {
+        const int len = min(MARK, last - t0);
+        float m[MARK][V], hs[MARK][V];
+        const uint32_t begin = b.states(c, len, m, hs);
+        b.finish(c, t0, len, begin, m, hs, in, dx, dgate, plane, corner, elems);
+    };
+    run_back<E, V> p, q;
+    int t0 = first + (last - first - 1) / MARK * MARK;
+    load(p, t0);
+    for (;;) {
+        load(q, t0 - MARK);
+        one(p, t0);
+        if ((t0 -= MARK) < first) break;
+        load(p, t0 - MARK);
+        one(q, t0);
+        if ((t0 -= MARK) < first) break;
+    }
+    if (dstate && c.valid && first == 0) store_floats<V>(dstate + corner, floats, in);
+}
+
+template <typename E, int V, int W>
+__global__ __launch_bounds__(64 * W) void k_memory_short_back(shape s, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ marks,
+                                                              const E* __restrict__ grad_h, const float* __restrict__ grad_state, E* __restrict__ dx, E* __restrict__ dgate, float* __restrict__ dstate) {
+    __shared__ float la[W][64 * V], lb[W][64 * V];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const columns<V> c(s.N, s.D);
+    const int64_t plane = s.N * s.D, corner = c.n0 * s.D;
+    const uint32_t elems = c.template bytes<E>(s.D), floats = c.template bytes<float>(s.D);
+    float carry[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) carry[v] = 0.0f;
+    if (grad_state) load_floats<V>(carry, grad_state + corner, floats);
+    const int t0 = wave * MARK, len = max(0, min(MARK, s.T - t0));
+    run_back<E, V> b;
+    b.load(s, c, t0, s.T, x, gate, grad_h, starts, marks, plane, corner, floats);
+    float m[MARK][V], hs[MARK][V];
+    uint32_t begin = b.states(c, len, m, hs);
+    factor A[V]; float B[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) B[v] = 0.0f;
+#pragma unroll
+    for (int t = MARK - 1; t >= 0; --t) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            B[v] = (begin >> t) & 1 ? 0.0f : decay_of(m[t][v], (t < len ? get<E, V>(b.r.d[t], v) : 0.0f) + B[v]);
+            A[v].step(m[t][v]);
+        }
+        pause<V>(MARK - 1 - t);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) { la[wave][v * 64 + lane] = A[v].held(begin != 0); lb[wave][v * 64 + lane] = B[v]; }
+    forget<V>(m, begin); b.r.forget();
+    __syncthreads();
+    float in[V], next[V];
+    join<V, true>(la, lb, lane, W, W - 1 - wave, carry, in, next);
+    if (len > 0) b.finish(c, t0, len, begin, m, hs, in, dx, dgate, plane, corner, elems);
+    if (dstate && wave == 0 && c.valid) store_floats<V>(dstate + corner, floats, next);
 }
 
 // One control step.  state_out may be state: a thread reads its own columns, which are no other's, before it writes them.
