@@ -1,11 +1,12 @@
-"""ctypes binding of drloco_amd/csrc/libdrloco_learner.so (the C-ABI in include/drloco_learner.h): the learner's operators,
-wrapped by drloco_amd.memory and drloco_amd.muon.
+"""The learner's operators: drloco_amd/csrc/libdrloco_learner.so (the C-ABI in include/drloco_learner.h) through ctypes, and
+dl_learner_torch.so, which calls it on torch tensors for drloco_amd.memory and drloco_amd.muon.
 
 A library of its own next to libdrloco_hip.so: its kernels need neither the step kernels' compiler flags nor their two code
 objects.  There is no CPU fallback: the functions refuse tensors that are not on a HIP device."""
 import ctypes as C
 import os
 import subprocess
+import sysconfig
 
 import torch
 
@@ -13,6 +14,7 @@ from . import lib
 
 CSRC = os.path.join(lib.CSRC, 'learner')
 LIB_PATH = os.path.join(lib.CSRC, 'libdrloco_learner.so')
+TORCH_PATH = os.path.join(lib.CSRC, 'dl_learner_torch.so')
 ABI_VERSION = 1
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # DL_F32, DL_BF16, DL_F16
 MARK = 16                                                                 # DL_MEMORY_MARK
@@ -46,22 +48,37 @@ _SIGNATURES = {
 }
 
 _lib = None
+_ops = None
 
 
 def _sources():
     return [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith(('.hip', '.hpp'))] + [os.path.join(lib.INCLUDE, 'drloco_learner.h')]
 
 
-def build(force=False, verbose=False):
-    """hipcc --offload-arch=gfx950 of the learner's kernels into an in-tree shared library."""
-    if not force and os.path.exists(LIB_PATH) and all(os.path.getmtime(s) <= os.path.getmtime(LIB_PATH) for s in _sources()):
-        return LIB_PATH
-    hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
-    cmd = [hipcc, '--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-shared', '-Wno-unused-command-line-argument',
-           '-ffile-prefix-map=' + os.path.dirname(lib.INCLUDE) + '=.', '-I' + lib.INCLUDE, '-I' + CSRC] + EXTRA_FLAGS + [os.path.join(CSRC, 'dl_learner.hip'), '-o', LIB_PATH]
+def _fresh(path, sources):
+    return os.path.exists(path) and all(os.path.getmtime(s) <= os.path.getmtime(path) for s in sources)
+
+
+def _run(cmd, verbose):
     if verbose:
         print(' '.join(cmd))
     subprocess.check_call(cmd)
+
+
+def build(force=False, verbose=False):
+    """hipcc --offload-arch=gfx950 of the learner's kernels and g++ of their torch binding, into in-tree shared libraries."""
+    root = os.path.dirname(lib.INCLUDE)
+    if force or not _fresh(LIB_PATH, _sources()):
+        hipcc = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
+        _run([hipcc, '--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-shared', '-Wno-unused-command-line-argument', '-ffile-prefix-map=' + root + '=.', '-I' + lib.INCLUDE, '-I' + CSRC] +
+             EXTRA_FLAGS + [os.path.join(CSRC, 'dl_learner.hip'), '-o', LIB_PATH], verbose)
+    source = os.path.join(CSRC, 'dl_torch.cpp')
+    if force or not _fresh(TORCH_PATH, [source, os.path.join(lib.INCLUDE, 'drloco_learner.h')]):
+        from torch.utils import cpp_extension
+        rocm = os.environ.get('ROCM_PATH', '/opt/rocm')
+        _run(['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-w', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1', f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}',
+              '-ffile-prefix-map=' + root + '=.', '-I' + lib.INCLUDE] + ['-I' + p for p in cpp_extension.include_paths()] + ['-I' + os.path.join(rocm, 'include'), '-I' + sysconfig.get_paths()['include'],
+              source, '-o', TORCH_PATH] + ['-L' + p for p in cpp_extension.library_paths()] + ['-lc10', '-lc10_hip', '-ltorch_cpu', '-ltorch', '-ltorch_python', '-L' + lib.CSRC, '-ldrloco_learner', '-Wl,-rpath,$ORIGIN'], verbose)
     return LIB_PATH
 
 
@@ -89,25 +106,19 @@ def check(rc):
     return rc
 
 
-class _Here:
-    """Nothing to change: the tensors' device is the current one."""
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *_):
-        return False
-
-
-_HERE = _Here()
-
-
-def on(device):
-    """Context in which `device` is the current one (work goes to ITS current stream)."""
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+def ops():
+    """The torch binding (dl_torch.cpp); raises DrlocoError if it has not been built."""
+    global _ops
+    if _ops is None:
+        load()
+        if not os.path.exists(TORCH_PATH):
+            raise lib.DrlocoError(f'{TORCH_PATH} is missing: run `python -c "import __graft_entry__ as g; g.build()"`')
+        import importlib.machinery
+        import importlib.util
+        loader = importlib.machinery.ExtensionFileLoader('dl_learner_torch', TORCH_PATH)
+        _ops = importlib.util.module_from_spec(importlib.util.spec_from_loader('dl_learner_torch', loader))
+        loader.exec_module(_ops)
+    return _ops
 
 
 def require_device(name, *tensors):

@@ -4,7 +4,6 @@ the matrix cores, next to the Adam steps the reference takes (drloco/train.py:11
     orthogonalise(g)       the orthogonal factor of a gradient, by Newton-Schulz products
     muon_update(w, g, m)   momentum, orthogonalisation and the new weight in one call
     HipMuon                a torch optimiser of matrices built on it; vectors (biases, log_std) stay with Adam"""
-import ctypes as C
 import math
 
 import torch
@@ -22,15 +21,6 @@ def _matrix(name, what, t, dtypes):
         raise ValueError(f'{name}: {what} needs at least two axes, got {tuple(t.shape)}')
     if t.dtype not in dtypes:
         raise TypeError(f'{name}: {what} is {t.dtype}, expected {" or ".join(str(d) for d in dtypes)}')
-
-
-def _stacked(t):
-    """t as [batch, rows, cols] with contiguous rows and one stride over the batch (a copy where its strides allow none)."""
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        t = t.contiguous()
-    if t.dim() == 2:
-        return t.unsqueeze(0)
-    return t if t.dim() == 3 else t.reshape(-1, t.shape[-2], t.shape[-1])
 
 
 def _coefficients(name, steps, coefficients):
@@ -55,38 +45,6 @@ def _result(name, what, t, like, dtype, aliases):
     return t
 
 
-def _launch(grad, momentum, momentum_out, weight, out, steps, coefficients, beta, nesterov, keep, gain):
-    g = _stacked(grad)
-    s = ll.OrthShape()
-    s.batch, s.rows, s.cols = g.shape
-    s.grad_b, s.grad_r = g.stride()[:2]
-    s.grad_type = ll.DTYPES[g.dtype]
-    pm = pmo = pw = None
-    if momentum is not None:
-        m, mo = _stacked(momentum), _stacked(momentum_out)
-        s.momentum_b, s.momentum_r = m.stride()[:2]
-        s.momentum_out_b, s.momentum_out_r = mo.stride()[:2]
-        pm, pmo = m.data_ptr(), mo.data_ptr()
-    if weight is not None:
-        w = _stacked(weight)
-        s.weight_b, s.weight_r = w.stride()[:2]
-        s.weight_type = ll.DTYPES[w.dtype]
-        pw = w.data_ptr()
-    o = _stacked(out)
-    s.out_b, s.out_r = o.stride()[:2]
-    s.out_type = ll.DTYPES[o.dtype]
-    s.a, s.b, s.c = coefficients
-    s.beta, s.weight_keep, s.gain = beta, keep, gain
-    s.steps, s.nesterov = int(steps), int(bool(nesterov))
-    so, dev = ll.load(), g.device
-    with ll.on(dev):
-        work = torch.empty(ll.check(so.dl_orth_workspace_bytes(C.byref(s))), dtype=torch.uint8, device=dev)
-        ll.check(so.dl_orth_update(C.byref(s), g.data_ptr(), pm, pmo, pw, o.data_ptr(), work.data_ptr(), ll.stream(dev)))
-    # the library wrote behind torch's back: caches keyed by version counters (HipPolicy's packed weights) and autograd have to see it
-    torch.autograd.graph.increment_version([out] if momentum is None else [out, momentum_out])
-
-
-@torch.no_grad()
 def orthogonalise(g, steps=5, coefficients=COEFFICIENTS, out=None):
     """The orthogonal factor U V' of each matrix G = U S V' of g [..., rows, cols] (float32, bfloat16 or float16), approached by `steps`
     steps X <- a X + b (X X') X + c (X X')^2 X from G / |G|_F: singular values move towards one, zeros and a zero matrix
@@ -103,11 +61,10 @@ def orthogonalise(g, steps=5, coefficients=COEFFICIENTS, out=None):
     else:
         _result('orthogonalise', 'out', out, g, g.dtype, [(True, g)])
     if g.numel():
-        _launch(g, None, None, None, out, steps, coefficients, 0.0, False, 0.0, 1.0)
+        ll.ops().orth_update(g, None, None, None, out, int(steps), *coefficients, 0.0, False, 0.0, 1.0)
     return out
 
 
-@torch.no_grad()
 def muon_update(weight, grad, momentum, lr, beta=0.95, nesterov=True, weight_decay=0.0, scale=None, steps=5, coefficients=COEFFICIENTS, out=None, momentum_out=None):
     """One step of the Muon optimiser for the matrices weight [..., rows, cols] (float32, bfloat16 or float16) with gradient `grad` (one of
     these types too) and momentum (float32):
@@ -137,7 +94,7 @@ def muon_update(weight, grad, momentum, lr, beta=0.95, nesterov=True, weight_dec
     if scale is None:
         scale = math.sqrt(max(1.0, weight.shape[-2] / max(1, weight.shape[-1])))
     if weight.numel():
-        _launch(grad, momentum, momentum_out, weight, out, steps, coefficients, beta, nesterov, 1.0 - lr * weight_decay, -lr * scale)
+        ll.ops().orth_update(grad, momentum, momentum_out, weight, out, int(steps), *coefficients, beta, bool(nesterov), 1.0 - lr * weight_decay, -lr * scale)
     return out, momentum_out
 
 

@@ -216,7 +216,7 @@ def test_offsets_beyond_32_bits():
     M = float(xs.abs().max())
     assert np.all(np.abs(np64(last[cols].detach().cpu()) - last_) <= 12 * U * M * (T + 1))
     assert np.all(np.abs(np64(h[:, cols].detach().cpu()) - h_) <= 12 * U * M * (T + 1) + rounding(torch.bfloat16, h_))
-    assert float(h[:, 1].abs().max()) == 0.0
+    assert float(h[:, 1].detach().abs().max()) == 0.0
     grad = torch.zeros_like(h)
     ghs = torch.randn(T, 3, D, generator=g).to(torch.bfloat16)
     grad[:, cols] = ghs.cuda()
@@ -230,12 +230,10 @@ def test_offsets_beyond_32_bits():
 
 def test_walkers_far_apart():
     """walker-major with more than 2^29 elements under the lanes of a wave: the wrapper makes a time-major copy"""
-    from drloco_amd.memory import _rows
     far = 1 << 23
     store = torch.zeros(69 * far + 64, dtype=torch.float16, device='cuda')
     place = lambda t: store.as_strided(t.shape, (t.shape[2], far, 1)).copy_(t).detach()
     x, gate, b, st, gh, gl = make(5, 70, 4, torch.float16, seed=3)
-    assert _rows(place(x)).is_contiguous() and not _rows(store.as_strided((5, 2, 4), (4, far, 1))).is_contiguous()
     check_all(x, gate, b, st, gh, gl, place=lambda t: place(t).clone(memory_format=torch.preserve_format) if t is gh else place(t) if t is x else t.cuda())
 
 
