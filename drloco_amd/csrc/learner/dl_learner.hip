@@ -116,17 +116,21 @@ const char* orth_shape_error(const dl_orth_shape* s) {
 struct orth_form {
     dlo::plan p;
     int tile;
-    bool turned;
+    bool turned, small;
     int64_t x_bytes, a_bytes, bytes;          // of the whole batch; the workspace: partials, XR, XC, XC', A, Q
 };
+
+constexpr int64_t DIRECT = (int64_t)640 * 640 * 640;
 
 orth_form orth_plan(const dl_orth_shape* s) {
     orth_form f;
     f.turned = s->rows > s->cols;
     f.p.m = (int32_t)std::min(s->rows, s->cols);
     f.p.n = (int32_t)std::max(s->rows, s->cols);
+    f.small = f.p.m <= 32 ? f.p.n <= 1024 : f.p.m <= 64 && f.p.n <= 256;          // what a workgroup's LDS holds
+    const int64_t m32 = ceil_div(f.p.m, 32) * 32, n32 = ceil_div(f.p.n, 32) * 32;
     const int64_t big = s->batch * ceil_div(f.p.m, 128) * ceil_div(f.p.n, 128);
-    f.tile = big >= 128 ? 128 : 64;
+    f.tile = s->batch * m32 * m32 * n32 <= DIRECT ? 32 : big >= 128 ? 128 : 64;
     f.p.mp = (int32_t)(ceil_div(f.p.m, f.tile) * f.tile);
     f.p.np = (int32_t)(ceil_div(f.p.n, f.tile) * f.tile);
     f.p.x_size = (int64_t)f.p.mp * f.p.np * 2;
@@ -139,8 +143,11 @@ orth_form orth_plan(const dl_orth_shape* s) {
 }
 
 template <int TILE, int MODE> void launch_product(const dlo::product& p, int64_t tiles, int64_t batch, hipStream_t st) {
+    if constexpr (TILE == 32) return dlo::k_orth_direct<MODE><<<dim3((unsigned)tiles, 1, (unsigned)batch), 512, 0, st>>>(p);
+    else {
     constexpr int W = TILE / 2;
     dlo::k_orth_product<TILE, TILE, W, W, MODE><<<dim3((unsigned)tiles, 1, (unsigned)batch), 256, 0, st>>>(p);
+    }
 }
 
 template <int TILE> void launch_steps(const dl_orth_shape* s, const orth_form& f, dlo::product last, char* work, hipStream_t st) {
@@ -259,17 +266,31 @@ int dl_memory_step(const dl_memory_shape* s, const void* x, const void* gate, co
 int64_t dl_orth_workspace_bytes(const dl_orth_shape* s) {
     if (const char* e = orth_shape_error(s)) return fail(DL_E_INVAL, e);
     if (s->batch == 0 || s->rows == 0 || s->cols == 0) return 0;
-    return orth_plan(s).bytes;
+    const orth_form f = orth_plan(s);
+    return f.small ? 0 : f.bytes;
 }
 
 int dl_orth_update(const dl_orth_shape* s, const void* grad, const float* momentum, float* momentum_out, const void* weight, void* out, void* workspace, void* stream) {
     if (const char* e = orth_shape_error(s)) return fail(DL_E_INVAL, e);
     if (s->batch == 0 || s->rows == 0 || s->cols == 0) return DL_OK;
-    if (!grad || !out || !workspace) return fail(DL_E_INVAL, "dl_orth_update: grad, out and workspace must not be NULL");
+    if (!grad || !out) return fail(DL_E_INVAL, "dl_orth_update: grad and out must not be NULL");
     if (!momentum != !momentum_out) return fail(DL_E_INVAL, "dl_orth_update: momentum and momentum_out must be given together");
+    if (dl_orth_workspace_bytes(s) > 0 && !workspace) return fail(DL_E_INVAL, "dl_orth_update: workspace must not be NULL (dl_orth_workspace_bytes)");
     if (!aligned(workspace, 16)) return fail(DL_E_INVAL, "dl_orth_update: workspace must be aligned to 16 bytes");
     const orth_form f = orth_plan(s);
     hipStream_t st = (hipStream_t)stream;
+    if (f.small) {
+        dlo::small p{{grad, s->grad_type, momentum, momentum_out, (float)s->beta, s->nesterov, s->grad_b, s->grad_r, s->momentum_b, s->momentum_r, s->momentum_out_b, s->momentum_out_r},
+                     f.p.m, f.p.n, s->steps, f.turned, (float)s->a, (float)s->b, (float)s->c, out, weight, s->out_type, s->weight_type,
+                     f.turned ? dlo::matrix{s->out_b, 1, s->out_r} : dlo::matrix{s->out_b, s->out_r, 1}, f.turned ? dlo::matrix{s->weight_b, 1, s->weight_r} : dlo::matrix{s->weight_b, s->weight_r, 1},
+                     (float)s->weight_keep, (float)s->gain};
+        const unsigned batch = (unsigned)s->batch;
+        if (f.p.m > 32) dlo::k_orth_small<4, 2><<<batch, 512, 0, st>>>(p);
+        else if (f.p.n <= 256) dlo::k_orth_small<2, 2><<<batch, 512, 0, st>>>(p);
+        else if (f.p.n <= 512) dlo::k_orth_small<2, 4><<<batch, 512, 0, st>>>(p);
+        else dlo::k_orth_small<2, 8><<<batch, 512, 0, st>>>(p);
+        return launched("dl_orth_update");
+    }
     double* partials = (double*)workspace;
     char* work = (char*)workspace + ceil_div(s->batch * f.p.partials * 8, 256) * 256;
     const dlo::source src{grad, s->grad_type, momentum, momentum_out, (float)s->beta, s->nesterov, s->grad_b, s->grad_r, s->momentum_b, s->momentum_r, s->momentum_out_b, s->momentum_out_r};
@@ -282,7 +303,9 @@ int dl_orth_update(const dl_orth_shape* s, const void* grad, const float* moment
     p.w_at = f.turned ? dlo::matrix{s->weight_b, 1, s->weight_r} : dlo::matrix{s->weight_b, s->weight_r, 1};
     p.keep = (float)s->weight_keep; p.gain = (float)s->gain;
     p.m = f.p.m; p.n = f.p.n;
-    if (f.tile == 128) launch_steps<128>(s, f, p, work, st); else launch_steps<64>(s, f, p, work, st);
+    if (f.tile == 128) launch_steps<128>(s, f, p, work, st);
+    else if (f.tile == 32) launch_steps<32>(s, f, p, work, st);
+    else launch_steps<64>(s, f, p, work, st);
     return launched("dl_orth_update");
 }
 

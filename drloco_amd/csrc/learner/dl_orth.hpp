@@ -268,4 +268,272 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void k_orth_product(pro
     }
 }
 
+// ---- the same products where there are too few tiles, or too few steps along k, to fill the chip with staged ones ----------------------
+// One 32 x 32 tile per workgroup, eight waves take every eighth step along k straight from memory: all their loads are on the way at
+// once, nothing is staged and nothing waited for but the sum over the waves.  Every element comes from the L2 cache 32 times
+// (m n k / 4 bytes in all), which is what bounds it from some 600^3 on.
+template <int MODE>
+__global__ __launch_bounds__(512) void k_orth_direct(product p) {
+    constexpr int WAVES = 8;
+    __shared__ __attribute__((aligned(16))) float part[WAVES][4][256];
+    __shared__ float tile[32][33];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int64_t b = blockIdx.z;
+    int ti, tj;
+    if (MODE == GRAM || MODE == POLY) {
+        const int t = blockIdx.x;
+        ti = (int)((sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
+        while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
+        while (ti * (ti + 1) / 2 > t) --ti;
+        tj = t - ti * (ti + 1) / 2;
+    } else {
+        ti = blockIdx.x % p.tiles_i; tj = blockIdx.x / p.tiles_i;
+    }
+    const _Float16* P = p.P + b * p.P_b + (int64_t)ti * 2 * p.kb * FRAG + lane * 8;
+    const _Float16* Q = p.Q + b * p.Q_b + (int64_t)tj * 2 * p.kb * FRAG + lane * 8;
+    float4_ acc[2][2] = {};
+#pragma unroll 4
+    for (int k = wave; k < p.kb; k += WAVES) {
+        half8 ph[2], pl[2], qh[2], ql[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const _Float16* f = P + ((int64_t)i * p.kb + k) * FRAG;
+            ph[i] = *(const half8*)f; pl[i] = *(const half8*)(f + 512);
+            f = Q + ((int64_t)i * p.kb + k) * FRAG;
+            qh[i] = *(const half8*)f; ql[i] = *(const half8*)(f + 512);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[i], ql[j], acc[i][j], 0, 0, 0);
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[i], qh[j], acc[i][j], 0, 0, 0);
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[i], qh[j], acc[i][j], 0, 0, 0);
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) *(float4_*)&part[wave][i * 2 + j][lane * 4] = acc[i][j];
+    const int i0 = ti * 32, j0 = tj * 32;
+    __syncthreads();
+    if (wave < 4) {          // a wave sums a quarter
+        float4_ v = {};
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) v += *(const float4_*)&part[w][wave][lane * 4];
+        const int i = (wave >> 1) * 16 + (lane >> 4) * 4, j = (wave & 1) * 16 + (lane & 15);
+        if (MODE == POLY) {
+            // A[i + r][j] lies in the fragment of row j (A is symmetric): four neighbours
+            const _Float16* A = p.A + b * p.out0_b + (((int64_t)(j0 / 16 + (wave & 1))) * p.out0_kb + ti) * FRAG + ((lane & 15) + 16 * (i >> 3)) * 8 + (i & 7);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                v[r] = fmaf(p.c, v[r] * (1.0f / SCALE), p.b * ((float)A[r] + (float)A[512 + r])) * SCALE;
+                if (i0 + i + r == j0 + j) v[r] += p.a * (SCALE * SCALE);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) tile[i + r][j] = v[r];
+    }
+    __syncthreads();
+    if (MODE == LAST) {
+        const bool down = p.out_at.si == 1 && p.out_at.sj != 1;
+        for (int e = threadIdx.x; e < 1024; e += 512) {
+            const int i = down ? e & 31 : e >> 5, j = down ? e >> 5 : e & 31;
+            if (i0 + i < p.m && j0 + j < p.n) {
+                float v = tile[i][j] * (p.gain / (SCALE * SCALE));
+                if (p.w) v = fmaf(p.keep, load_elem(p.w, p.w_type, b * p.w_at.b + (i0 + i) * p.w_at.si + (j0 + j) * p.w_at.sj), v);
+                store_elem(p.out, p.out_type, b * p.out_at.b + (i0 + i) * p.out_at.si + (j0 + j) * p.out_at.sj, v);
+            }
+        }
+        return;
+    }
+    if (wave >= 4 || (MODE != STEP && wave >= 2 && ti == tj)) return;
+    // two fragments with rows i and two with rows j: the mirror image of a symmetric result, or X's other orientation
+    const bool turned = wave >= 2;
+    const int row = (wave & 1) * 16 + (lane & 15), k = (lane >> 4) * 8;
+    half8 hi, lo;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) { _Float16 h, l; split((turned ? tile[k + r][row] : tile[row][k + r]) * (1.0f / SCALE), h, l); hi[r] = h; lo[r] = l; }
+    _Float16* out = turned && MODE == STEP ? p.out1 + b * p.out1_b : p.out0 + b * p.out0_b;
+    const int64_t kbs = turned && MODE == STEP ? p.out1_kb : p.out0_kb;
+    _Float16* to = out + (((int64_t)(turned ? j0 : i0) / 16 + (wave & 1)) * kbs + (turned ? ti : tj)) * FRAG + lane * 8;
+    *(half8*)to = hi;
+    *(half8*)(to + 512) = lo;
+}
+
+// ---- small matrices: all of it in one workgroup ----------------------------------------------------------------------------------------
+// m <= 16 RB rows, n <= 128 JB columns.  Wave w owns 16 JB columns.  A result of the matrix cores leaves lane (q, c) = (lane / 16, lane % 16)
+// with rows 16 I + 4 q + r of column c; as an operand over k = 32 s .. a lane needs eight k's, the same ones in both operands, in
+// any order.  With the order {32 s + 4 q + r, 32 s + 16 + 4 q + r} the results of the blocks I = 2 s and 2 s + 1 are an operand as they
+// stand: X goes from step to step in registers, and Q, being symmetric, is one as it comes out.  Only A = X X', which sums over
+// columns, reads X in its other orientation, from the wave's own part of LDS.  Two barriers per step, where A's parts are summed.
+// 8 x 512 and 29 x 512: bound by the latency of some 150 dependent instructions per step, not by a unit.
+struct small {
+    source s;
+    int32_t m, n, steps, turned;
+    float a, b, c;
+    void* out; const void* w; int out_type, w_type;
+    matrix out_at, w_at;
+    float keep, gain;
+};
+
+template <int RB, int JB>
+__global__ __launch_bounds__(512) void k_orth_small(small p) {
+    constexpr int WAVES = 8, KB = JB / 2, S = RB / 2, TILES = RB * (RB + 1) / 2;
+    __shared__ __attribute__((aligned(16))) _Float16 xr[WAVES][RB][KB][FRAG];
+    __shared__ __attribute__((aligned(16))) float red[WAVES][TILES][256];
+    __shared__ __attribute__((aligned(16))) _Float16 am[RB][S][FRAG];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), q = lane >> 4, c = lane & 15;
+    const int64_t b = blockIdx.x;
+    float x[JB][RB][4];
+    double sum = 0.0;
+#pragma unroll
+    for (int jb = 0; jb < JB; ++jb)
+#pragma unroll
+        for (int I = 0; I < RB; ++I)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = 16 * I + 4 * q + r, j = (wave * JB + jb) * 16 + c;
+                float u = 0.0f;
+                if (i < p.m && j < p.n) {
+                    const int64_t row = p.turned ? j : i, col = p.turned ? i : j;
+                    u = load_elem(p.s.g, p.s.dtype, b * p.s.g_b + row * p.s.g_r + col);
+                    if (p.s.m) {
+                        const float v = fmaf(p.s.beta, p.s.m[b * p.s.m_b + row * p.s.m_r + col], u);
+                        p.s.m_out[b * p.s.o_b + row * p.s.o_r + col] = v;
+                        u = p.s.nesterov ? fmaf(p.s.beta, v, u) : v;
+                    }
+                }
+                x[jb][I][r] = u;
+                sum += (double)u * u;
+            }
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    double* sums = (double*)red;
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+    for (int w = 0; w < WAVES; ++w) sum += sums[w];
+    __syncthreads();
+    const double inv = sum != 0.0 ? (double)SCALE / sqrt(sum) : 0.0;          // (NaN != 0)
+#pragma unroll
+    for (int jb = 0; jb < JB; ++jb)
+#pragma unroll
+        for (int I = 0; I < RB; ++I)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[jb][I][r] = (float)(x[jb][I][r] * inv);
+
+    for (int step = 0; step < p.steps; ++step) {
+        // X as operands: over rows in registers, over columns through LDS (this wave's part only)
+        half8 xh[JB][S], xl[JB][S];
+#pragma unroll
+        for (int jb = 0; jb < JB; ++jb)
+#pragma unroll
+            for (int I = 0; I < RB; ++I)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    _Float16 h, l;
+                    split(x[jb][I][r], h, l);
+                    xh[jb][I / 2][(I & 1) * 4 + r] = h;
+                    xl[jb][I / 2][(I & 1) * 4 + r] = l;
+                    _Float16* to = &xr[wave][I][jb / 2][(4 * q + r + 16 * ((jb & 1) * 2 + (c >> 3))) * 8 + (c & 7)];
+                    to[0] = h;
+                    to[512] = l;
+                }
+        float4_ acc[TILES] = {};
+#pragma unroll
+        for (int k = 0; k < KB; ++k) {
+            half8 ph[RB], pl[RB];
+#pragma unroll
+            for (int I = 0; I < RB; ++I) { ph[I] = *(const half8*)&xr[wave][I][k][lane * 8]; pl[I] = *(const half8*)&xr[wave][I][k][512 + lane * 8]; }
+#pragma unroll
+            for (int I = 0; I < RB; ++I)
+#pragma unroll
+                for (int J = 0; J <= I; ++J) {
+                    float4_& t = acc[I * (I + 1) / 2 + J];
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[I], pl[J], t, 0, 0, 0);
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[I], ph[J], t, 0, 0, 0);
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[I], ph[J], t, 0, 0, 0);
+                }
+        }
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) *(float4_*)&red[wave][t][lane * 4] = acc[t];
+        __syncthreads();
+        for (int t = wave; t < TILES; t += WAVES) {          // a wave sums a tile and writes it, and its mirror image, as operands
+            float4_ v = {};
+            for (int w = 0; w < WAVES; ++w) v += *(const float4_*)&red[w][t][lane * 4];
+            int I = 0;
+            while ((I + 1) * (I + 2) / 2 <= t) ++I;
+            const int J = t - I * (I + 1) / 2;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                _Float16 h, l;
+                split(v[r] * (1.0f / SCALE), h, l);
+                const int i = 16 * I + 4 * q + r, j = 16 * J + c;
+                _Float16* to = &am[J][i >> 5][(c + 16 * ((i & 31) >> 3)) * 8 + (i & 7)];
+                to[0] = h; to[512] = l;
+                if (I != J) {
+                    to = &am[I][j >> 5][(4 * q + r + 16 * ((j & 31) >> 3)) * 8 + (j & 7)];
+                    to[0] = h; to[512] = l;
+                }
+            }
+        }
+        __syncthreads();
+        half8 ah[RB][S], al[RB][S], qh[RB][S], ql[RB][S];
+#pragma unroll
+        for (int I = 0; I < RB; ++I)
+#pragma unroll
+            for (int k = 0; k < S; ++k) { ah[I][k] = *(const half8*)&am[I][k][lane * 8]; al[I][k] = *(const half8*)&am[I][k][512 + lane * 8]; }
+#pragma unroll
+        for (int J = 0; J < RB; ++J)
+#pragma unroll
+            for (int I = 0; I < RB; ++I) {
+                float4_ t = {};
+#pragma unroll
+                for (int k = 0; k < S; ++k) {
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[I][k], al[J][k], t, 0, 0, 0);
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[I][k], ah[J][k], t, 0, 0, 0);
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[I][k], ah[J][k], t, 0, 0, 0);
+                }
+                const int i = 16 * I + 4 * q;          // A[i + r][16 J + c] lies as row 16 J + c, columns i + r
+                const _Float16* from = &am[J][i >> 5][(c + 16 * ((i & 31) >> 3)) * 8 + (i & 7)];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float v = fmaf(p.c, t[r] * (1.0f / SCALE), p.b * ((float)from[r] + (float)from[512 + r]));
+                    if (i + r == 16 * J + c) v += p.a * SCALE;
+                    _Float16 h, l;
+                    split(v, h, l);
+                    qh[J][I / 2][(I & 1) * 4 + r] = h;
+                    ql[J][I / 2][(I & 1) * 4 + r] = l;
+                }
+            }
+#pragma unroll
+        for (int jb = 0; jb < JB; ++jb)
+#pragma unroll
+            for (int I = 0; I < RB; ++I) {
+                float4_ t = {};
+#pragma unroll
+                for (int k = 0; k < S; ++k) {
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[I][k], xl[jb][k], t, 0, 0, 0);
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[I][k], xh[jb][k], t, 0, 0, 0);
+                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[I][k], xh[jb][k], t, 0, 0, 0);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[jb][I][r] = t[r] * (1.0f / SCALE);
+            }
+    }
+#pragma unroll
+    for (int jb = 0; jb < JB; ++jb)
+#pragma unroll
+        for (int I = 0; I < RB; ++I)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = 16 * I + 4 * q + r, j = (wave * JB + jb) * 16 + c;
+                if (i < p.m && j < p.n) {
+                    float v = x[jb][I][r] * (p.gain / SCALE);
+                    if (p.w) v = fmaf(p.keep, load_elem(p.w, p.w_type, b * p.w_at.b + i * p.w_at.si + j * p.w_at.sj), v);
+                    store_elem(p.out, p.out_type, b * p.out_at.b + i * p.out_at.si + j * p.out_at.sj, v);
+                }
+            }
+}
+
 }  // namespace dlo

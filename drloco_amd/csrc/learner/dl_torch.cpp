@@ -185,8 +185,10 @@ void orth_update(const Tensor& grad, const Maybe& momentum, const Maybe& momentu
     }
     s.a = a; s.b = b; s.c = c; s.beta = beta; s.weight_keep = keep; s.gain = gain;
     s.steps = (int32_t)steps; s.nesterov = nesterov;
-    const Tensor work = bytes(g, check(dl_orth_workspace_bytes(&s)));
-    check(dl_orth_update(&s, g.data_ptr(), momentum ? m.data_ptr<float>() : nullptr, momentum ? mo.data_ptr<float>() : nullptr, weight ? w.data_ptr() : nullptr, o.data_ptr(), work.data_ptr(), stream_of(g)));
+    const int64_t size = check(dl_orth_workspace_bytes(&s));
+    Tensor work;
+    if (size) work = bytes(g, size);
+    check(dl_orth_update(&s, g.data_ptr(), momentum ? m.data_ptr<float>() : nullptr, momentum ? mo.data_ptr<float>() : nullptr, weight ? w.data_ptr() : nullptr, o.data_ptr(), size ? work.data_ptr() : nullptr, stream_of(g)));
     written(out);
     if (momentum) written(*momentum_out);
 }
