@@ -129,24 +129,25 @@ orth_form orth_plan(const dl_orth_shape* s) {
     f.p.n = (int32_t)std::max(s->rows, s->cols);
     f.small = f.p.m <= 32 ? f.p.n <= 1024 : f.p.m <= 64 && f.p.n <= 256;          // what a workgroup's LDS holds
     const int64_t m32 = ceil_div(f.p.m, 32) * 32, n32 = ceil_div(f.p.n, 32) * 32;
-    const int64_t big = s->batch * ceil_div(f.p.m, 128) * ceil_div(f.p.n, 128);
-    f.tile = s->batch * m32 * m32 * n32 <= DIRECT ? 32 : big >= 128 ? 128 : 64;
+    f.tile = s->batch * m32 * m32 * n32 <= DIRECT ? 32 : 128;
     f.p.mp = (int32_t)(ceil_div(f.p.m, f.tile) * f.tile);
     f.p.np = (int32_t)(ceil_div(f.p.n, f.tile) * f.tile);
     f.p.x_size = (int64_t)f.p.mp * f.p.np * 2;
     f.p.a_size = (int64_t)f.p.mp * f.p.mp * 2;
-    f.p.partials = (int32_t)std::min<int64_t>(256, ceil_div(s->rows * s->cols, 4096));
+    f.p.partials = (int32_t)std::min<int64_t>(1024, ceil_div(s->rows * s->cols, 4096));
     f.x_bytes = s->batch * f.p.x_size * 2;
     f.a_bytes = s->batch * f.p.a_size * 2;
     f.bytes = ceil_div(s->batch * f.p.partials * 8, 256) * 256 + 3 * f.x_bytes + 2 * f.a_bytes;
     return f;
 }
 
-template <int TILE, int MODE> void launch_product(const dlo::product& p, int64_t tiles, int64_t batch, hipStream_t st) {
-    if constexpr (TILE == 32) return dlo::k_orth_direct<MODE><<<dim3((unsigned)tiles, 1, (unsigned)batch), 512, 0, st>>>(p);
+// 512 tiles of 128 fill the chip (two per CU); see k_orth_product
+template <int TILE, int MODE> void launch_product(dlo::product p, int64_t tiles, int64_t batch, hipStream_t st) {
+    if constexpr (TILE == 32) dlo::k_orth_direct<MODE><<<dim3((unsigned)tiles, 1, (unsigned)batch), 512, 0, st>>>(p);
     else {
-    constexpr int W = TILE / 2;
-    dlo::k_orth_product<TILE, TILE, W, W, MODE><<<dim3((unsigned)tiles, 1, (unsigned)batch), 256, 0, st>>>(p);
+        const int64_t all = tiles * batch, rest = all % 512 >= 340 ? 0 : all % 512;
+        p.whole = (int32_t)(tiles - std::min(tiles, ceil_div(rest, batch)));
+        dlo::k_orth_product<MODE><<<dim3((unsigned)(p.whole + (tiles - p.whole) * 4), 1, (unsigned)batch), 256, 0, st>>>(p);
     }
 }
 
@@ -282,7 +283,7 @@ int dl_orth_update(const dl_orth_shape* s, const void* grad, const float* moment
     if (f.small) {
         dlo::small p{{grad, s->grad_type, momentum, momentum_out, (float)s->beta, s->nesterov, s->grad_b, s->grad_r, s->momentum_b, s->momentum_r, s->momentum_out_b, s->momentum_out_r},
                      f.p.m, f.p.n, s->steps, f.turned, (float)s->a, (float)s->b, (float)s->c, out, weight, s->out_type, s->weight_type,
-                     f.turned ? dlo::matrix{s->out_b, 1, s->out_r} : dlo::matrix{s->out_b, s->out_r, 1}, f.turned ? dlo::matrix{s->weight_b, 1, s->weight_r} : dlo::matrix{s->weight_b, s->weight_r, 1},
+                     s->out_b, s->out_r, s->weight_b, s->weight_r,
                      (float)s->weight_keep, (float)s->gain};
         const unsigned batch = (unsigned)s->batch;
         if (f.p.m > 32) dlo::k_orth_small<4, 2><<<batch, 512, 0, st>>>(p);
@@ -294,8 +295,9 @@ int dl_orth_update(const dl_orth_shape* s, const void* grad, const float* moment
     double* partials = (double*)workspace;
     char* work = (char*)workspace + ceil_div(s->batch * f.p.partials * 8, 256) * 256;
     const dlo::source src{grad, s->grad_type, momentum, momentum_out, (float)s->beta, s->nesterov, s->grad_b, s->grad_r, s->momentum_b, s->momentum_r, s->momentum_out_b, s->momentum_out_r};
-    dlo::k_orth_norm<<<dim3((unsigned)f.p.partials, (unsigned)s->batch), 256, 0, st>>>(src, s->rows, s->cols, partials);
-    dlo::k_orth_load<<<dim3((unsigned)(f.p.np / 32), (unsigned)(f.p.mp / 32), (unsigned)s->batch), 256, 0, st>>>(src, f.p, f.turned, partials, (_Float16*)work, (_Float16*)(work + f.x_bytes));
+    const bool flat = s->grad_r == s->cols && (!momentum || (s->momentum_r == s->cols && s->momentum_out_r == s->cols));
+    dlo::k_orth_norm<<<dim3((unsigned)f.p.partials, (unsigned)s->batch), 256, 0, st>>>(src, flat ? 1 : s->rows, flat ? s->rows * s->cols : s->cols, partials);
+    dlo::k_orth_load<<<dim3((unsigned)ceil_div(f.p.np, 64), (unsigned)ceil_div(f.p.mp, 64), (unsigned)s->batch), 256, 0, st>>>(src, f.p, f.turned, partials, (_Float16*)work, (_Float16*)(work + f.x_bytes));
     dlo::product p{};
     p.a = (float)s->a; p.b = (float)s->b; p.c = (float)s->c;
     p.out = out; p.w = weight; p.out_type = s->out_type; p.w_type = s->weight_type;
@@ -303,9 +305,7 @@ int dl_orth_update(const dl_orth_shape* s, const void* grad, const float* moment
     p.w_at = f.turned ? dlo::matrix{s->weight_b, 1, s->weight_r} : dlo::matrix{s->weight_b, s->weight_r, 1};
     p.keep = (float)s->weight_keep; p.gain = (float)s->gain;
     p.m = f.p.m; p.n = f.p.n;
-    if (f.tile == 128) launch_steps<128>(s, f, p, work, st);
-    else if (f.tile == 32) launch_steps<32>(s, f, p, work, st);
-    else launch_steps<64>(s, f, p, work, st);
+    if (f.tile == 32) launch_steps<32>(s, f, p, work, st); else launch_steps<128>(s, f, p, work, st);
     return launched("dl_orth_update");
 }
 

@@ -51,6 +51,25 @@ __device__ __forceinline__ void store_elem(void* p, int dtype, int64_t i, float 
     else ((_Float16*)p)[i] = (_Float16)v;
 }
 
+// four neighbours, at any alignment
+template <typename E> __device__ __forceinline__ float4_ load4_as(const void* p, int64_t i) {
+    typedef E vec __attribute__((ext_vector_type(4), aligned(sizeof(E))));
+    const vec v = *(const vec*)((const E*)p + i);
+    return float4_{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+}
+__device__ __forceinline__ float4_ load4(const void* p, int dtype, int64_t i) {
+    return dtype == 0 ? load4_as<float>(p, i) : dtype == 1 ? load4_as<__bf16>(p, i) : load4_as<_Float16>(p, i);
+}
+template <typename E> __device__ __forceinline__ void store4_as(void* p, int64_t i, float4_ v) {
+    typedef E vec __attribute__((ext_vector_type(4), aligned(sizeof(E))));
+    *(vec*)((E*)p + i) = vec{(E)v[0], (E)v[1], (E)v[2], (E)v[3]};
+}
+__device__ __forceinline__ void store4(void* p, int dtype, int64_t i, float4_ v) {
+    if (dtype == 0) store4_as<float>(p, i, v);
+    else if (dtype == 1) store4_as<__bf16>(p, i, v);
+    else store4_as<_Float16>(p, i, v);
+}
+
 // ---- the sum of squares, in 64 bits (a float32 gradient of 1e30 or of 1e-30 is as good as another) --------------------------------
 // With a momentum: m' = beta m + g first, and the matrix is g + beta m' (nesterov) or m'.  rows x cols as the caller sees them.
 struct source {
@@ -60,20 +79,48 @@ struct source {
     int64_t g_b, g_r, m_b, m_r, o_b, o_r;          // strides of g, m, m_out: matrix, row
 };
 
-__global__ __launch_bounds__(256) void k_orth_norm(source s, int64_t rows, int64_t cols, double* __restrict__ partials) {
-    const int64_t b = blockIdx.y;
-    const int64_t all = rows * cols, per = (all + gridDim.x - 1) / gridDim.x;
-    const int64_t lo = (int64_t)blockIdx.x * per, hi = min(lo + per, all);
-    double sum = 0.0;
-    for (int64_t e = lo + threadIdx.x; e < hi; e += 256) {
-        const int64_t r = e / cols, c = e - r * cols;
-        float u = load_elem(s.g, s.dtype, b * s.g_b + r * s.g_r + c);
-        if (s.m) {
-            const float v = fmaf(s.beta, s.m[b * s.m_b + r * s.m_r + c], u);
-            s.m_out[b * s.o_b + r * s.o_r + c] = v;
-            u = s.nesterov ? fmaf(s.beta, v, u) : v;
+// u of four neighbours (of `n` of them, where fewer are left), and the momentum on the way
+__device__ __forceinline__ float4_ moved(const source& s, int64_t b, int64_t r, int64_t c, int n, bool first) {
+    const int64_t g = b * s.g_b + r * s.g_r + c;
+    float4_ u = {};
+    if (n >= 4) u = load4(s.g, s.dtype, g);
+    else for (int e = 0; e < n; ++e) u[e] = load_elem(s.g, s.dtype, g + e);
+    if (s.m) {
+        const int64_t o = b * s.o_b + r * s.o_r + c;
+        float4_ v = {};
+        if (first) {
+            const int64_t m = b * s.m_b + r * s.m_r + c;
+            if (n >= 4) v = load4_as<float>(s.m, m);
+            else for (int e = 0; e < n; ++e) v[e] = s.m[m + e];
+            for (int e = 0; e < 4; ++e) v[e] = fmaf(s.beta, v[e], u[e]);
+            if (n >= 4) store4_as<float>(s.m_out, o, v);
+            else for (int e = 0; e < n; ++e) s.m_out[o + e] = v[e];
+        } else {
+            if (n >= 4) v = load4_as<float>(s.m_out, o);
+            else for (int e = 0; e < n; ++e) v[e] = s.m_out[o + e];
         }
-        sum += (double)u * u;
+        for (int e = 0; e < 4; ++e) u[e] = s.nesterov ? fmaf(s.beta, v[e], u[e]) : v[e];
+    }
+    return u;
+}
+
+// rows x cols as they are read: one long row where the rows of all arrays follow each other
+__global__ __launch_bounds__(256) void k_orth_norm(source s, int64_t rows, int64_t cols, double* __restrict__ partials) {
+    const int64_t b = blockIdx.y, per = (cols + 3) / 4, all = rows * per;          // in fours
+    const int64_t step = (int64_t)gridDim.x * 256;
+    double sum = 0.0;
+    if (rows == 1) {
+#pragma unroll 4
+        for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < all; e += step) {
+            const float4_ u = moved(s, b, 0, e * 4, (int)min((int64_t)4, cols - e * 4), true);
+            for (int k = 0; k < 4; ++k) sum += (double)u[k] * u[k];
+        }
+    } else {
+        for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < all; e += step) {
+            const int64_t r = e / per, c = (e - r * per) * 4;
+            const float4_ u = moved(s, b, r, c, (int)min((int64_t)4, cols - c), true);
+            for (int k = 0; k < 4; ++k) sum += (double)u[k] * u[k];
+        }
     }
     __shared__ double part[4];
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
@@ -82,40 +129,46 @@ __global__ __launch_bounds__(256) void k_orth_norm(source s, int64_t rows, int64
     if (threadIdx.x == 0) partials[b * gridDim.x + blockIdx.x] = part[0] + part[1] + part[2] + part[3];
 }
 
-// ---- X = G / |G| into both orientations: one workgroup per 32 x 32 ---------------------------------------------------------------
+// ---- X = G / |G| into both orientations: one workgroup per 64 x 64 ---------------------------------------------------------------
 __global__ __launch_bounds__(256) void k_orth_load(source s, plan p, int turned, const double* __restrict__ partials, _Float16* __restrict__ xr, _Float16* __restrict__ xc) {
     const int b = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ float tile[64][65];          // [short side][long side]
+    const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
+    const int r0 = turned ? j0 : i0, c0 = turned ? i0 : j0, rows = turned ? p.n : p.m, cols = turned ? p.m : p.n;
+    float4_ u[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int r = r0 + e * 16 + (threadIdx.x >> 4), c = c0 + (threadIdx.x & 15) * 4;
+        u[e] = float4_{};
+        if (r < rows && c < cols) u[e] = moved(s, b, r, c, min(4, cols - c), false);
+    }
     double sum = 0.0;
     for (int k = lane; k < p.partials; k += 64) sum += partials[(int64_t)b * p.partials + k];
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     const double inv = sum != 0.0 ? (double)SCALE / sqrt(sum) : 0.0;          // (NaN != 0)
-    __shared__ float tile[32][33];
-    const int i0 = blockIdx.y * 32, j0 = blockIdx.x * 32;
-    for (int e = threadIdx.x; e < 1024; e += 256) {
-        const int fast = e & 31, slow = e >> 5;
-        const int i = turned ? fast : slow, j = turned ? slow : fast;
-        float u = 0.0f;
-        if (i0 + i < p.m && j0 + j < p.n) {
-            const int64_t r = turned ? j0 + j : i0 + i, c = turned ? i0 + i : j0 + j;
-            u = load_elem(s.g, s.dtype, b * s.g_b + r * s.g_r + c);
-            if (s.m) {
-                const float v = s.m_out[b * s.o_b + r * s.o_r + c];
-                u = s.nesterov ? fmaf(s.beta, v, u) : v;
-            }
-            u = (float)(u * inv);
-        }
-        tile[i][j] = u;
-    }
-    __syncthreads();
-    const int row = (wave & 1) * 16 + (lane & 15), k = (lane >> 4) * 8;
-    half8 hi, lo;
-    const bool c_side = wave >= 2;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) { _Float16 h, l; split(c_side ? tile[k + q][row] : tile[row][k + q], h, l); hi[q] = h; lo[q] = l; }
-    const int64_t block = (c_side ? j0 : i0) / 16 + (wave & 1), kb = (c_side ? i0 : j0) / 32, kbs = (c_side ? p.mp : p.np) / 32;
-    _Float16* to = (c_side ? xc : xr) + b * p.x_size + (block * kbs + kb) * FRAG + lane * 8;
-    *(half8*)to = hi;
-    *(half8*)(to + 512) = lo;
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int r = e * 16 + (threadIdx.x >> 4), c = (threadIdx.x & 15) * 4 + k;
+            (turned ? tile[c][r] : tile[r][c]) = (float)(u[e][k] * inv);
+        }
+    __syncthreads();
+    // 4 x 2 fragments with rows i and 4 x 2 with rows j
+#pragma unroll
+    for (int f = wave; f < 16; f += 4) {
+        const bool c_side = f >= 8;
+        const int row = (f & 3) * 16 + (lane & 15), k = (f >> 2 & 1) * 32 + (lane >> 4) * 8;
+        const int first = c_side ? j0 : i0, second = c_side ? i0 : j0, rows_ = c_side ? p.np : p.mp, ks = c_side ? p.mp : p.np;
+        if (first + (f & 3) * 16 >= rows_ || second + (f >> 2 & 1) * 32 >= ks) continue;
+        half8 hi, lo;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) { _Float16 h, l; split(c_side ? tile[k + q][row] : tile[row][k + q], h, l); hi[q] = h; lo[q] = l; }
+        const int64_t block = first / 16 + (f & 3), kb = second / 32 + (f >> 2 & 1);
+        _Float16* to = (c_side ? xc : xr) + b * p.x_size + (block * (ks / 32) + kb) * FRAG + lane * 8;
+        *(half8*)to = hi;
+        *(half8*)(to + 512) = lo;
+    }
 }
 
 // ---- the products ----------------------------------------------------------------------------------------------------------------
@@ -125,7 +178,7 @@ struct product {
     const _Float16* P; const _Float16* Q;          // operands, [rows / 16][kb][FRAG]
     int64_t P_b, Q_b;
     int32_t kb;                                    // steps of 32 along k
-    int32_t tiles_i, tiles_j;
+    int32_t tiles_i, tiles_j, whole;               // k_orth_product: tiles that are not cut into four
     _Float16* out0; int64_t out0_b, out0_kb;       // GRAM, POLY: the symmetric result;  STEP: XR
     _Float16* out1; int64_t out1_b, out1_kb;       // STEP: XC
     const _Float16* A;                             // POLY: as out0
@@ -137,26 +190,50 @@ struct product {
     int32_t m, n;
 };
 
+__device__ __forceinline__ void below(int t, int& ti, int& tj) {          // the tiles on and below the diagonal, row by row
+    ti = (int)((sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
+    while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
+    while (ti * (ti + 1) / 2 > t) --ti;
+    tj = t - ti * (ti + 1) / 2;
+}
+
+// out = keep w + gain X for the I x J values of `tile` (at [i * pitch + j]) from (i0, j0) on, in fours along the caller's rows
+template <int I, int J, int THREADS>
+__device__ __forceinline__ void emit(const product& p, int64_t b, const float* tile, int pitch, int i0, int j0) {
+    const float gain = p.gain / (SCALE * SCALE);
+    const bool down = p.out_at.si == 1 && p.out_at.sj != 1;          // the caller's rows run along the short side
+#pragma unroll 4
+    for (int e = threadIdx.x; e < I * J / 4; e += THREADS) {
+        const int i = down ? e % (I / 4) * 4 : e / (J / 4), j = down ? e / (I / 4) : e % (J / 4) * 4;
+        const int left = i0 + i < p.m && j0 + j < p.n ? down ? p.m - i0 - i : p.n - j0 - j : 0;
+        const float* t = tile + i * pitch + j;
+        const int d = down ? pitch : 1;
+        float4_ v = {t[0] * gain, t[d] * gain, t[2 * d] * gain, t[3 * d] * gain};
+        const int64_t at = b * p.out_at.b + (i0 + i) * p.out_at.si + (j0 + j) * p.out_at.sj, wat = b * p.w_at.b + (i0 + i) * p.w_at.si + (j0 + j) * p.w_at.sj;
+        if (left >= 4) {
+            if (p.w) {
+                const float4_ w = load4(p.w, p.w_type, wat);
+                for (int k = 0; k < 4; ++k) v[k] = fmaf(p.keep, w[k], v[k]);
+            }
+            store4(p.out, p.out_type, at, v);
+        } else {
+            for (int k = 0; k < left; ++k) store_elem(p.out, p.out_type, at + k, p.w ? fmaf(p.keep, load_elem(p.w, p.w_type, wat + k), v[k]) : v[k]);
+        }
+    }
+}
+
+template <int BM, int BN, int WM, int WN> struct staged {
+    static constexpr int WAVES = (BM / WM) * (BN / WN), ROWS = BM / 16 + BN / 16;          // fragments of a step
+    static constexpr int PITCH = BN + 4, STAGE = ROWS * FRAG * 2;                          // bytes
+    static constexpr int BYTES = 2 * STAGE > BM * PITCH * 4 ? 2 * STAGE : BM * PITCH * 4;
+};
+
 template <int BM, int BN, int WM, int WN, int MODE>
-__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void k_orth_product(product p) {
-    constexpr int WAVES = (BM / WM) * (BN / WN), TM = WM / 16, TN = WN / 16;
-    constexpr int ROWS = BM / 16 + BN / 16;                    // fragments of a step
-    constexpr int PITCH = BN + 4;
-    constexpr int STAGE = ROWS * FRAG * 2;                     // bytes
-    constexpr int BYTES = 2 * STAGE > BM * PITCH * 4 ? 2 * STAGE : BM * PITCH * 4;
-    __shared__ __attribute__((aligned(16))) char lds[BYTES];
+__device__ __forceinline__ void product_tile(const product& p, int ti, int tj, char* lds) {
+    typedef staged<BM, BN, WM, WN> L;
+    constexpr int WAVES = L::WAVES, TM = WM / 16, TN = WN / 16, ROWS = L::ROWS, PITCH = L::PITCH, STAGE = L::STAGE;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int64_t b = blockIdx.z;
-    int ti, tj;
-    if (MODE == GRAM || MODE == POLY) {                        // the tiles on and below the diagonal, row by row
-        const int t = blockIdx.x;
-        ti = (int)((sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
-        while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
-        while (ti * (ti + 1) / 2 > t) --ti;
-        tj = t - ti * (ti + 1) / 2;
-    } else {
-        ti = blockIdx.x % p.tiles_i; tj = blockIdx.x / p.tiles_i;
-    }
     const _Float16* P = p.P + b * p.P_b + (int64_t)ti * (BM / 16) * p.kb * FRAG;
     const _Float16* Q = p.Q + b * p.Q_b + (int64_t)tj * (BN / 16) * p.kb * FRAG;
 
@@ -216,16 +293,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void k_orth_product(pro
     __syncthreads();
     const int i0 = ti * BM, j0 = tj * BN, row = lane & 15, k8 = (lane >> 4) * 8;
     if (MODE == LAST) {
-        constexpr int THREADS = WAVES * 64;
-        const bool down = p.out_at.si == 1 && p.out_at.sj != 1;          // the short side runs along the caller's rows
-        for (int e = threadIdx.x; e < BM * BN; e += THREADS) {
-            const int i = down ? e % BM : e / BN, j = down ? e / BM : e % BN;
-            if (i0 + i < p.m && j0 + j < p.n) {
-                float v = tile[i * PITCH + j] * (p.gain / (SCALE * SCALE));
-                if (p.w) v = fmaf(p.keep, load_elem(p.w, p.w_type, b * p.w_at.b + (i0 + i) * p.w_at.si + (j0 + j) * p.w_at.sj), v);
-                store_elem(p.out, p.out_type, b * p.out_at.b + (i0 + i) * p.out_at.si + (j0 + j) * p.out_at.sj, v);
-            }
-        }
+        emit<BM, BN, WAVES * 64>(p, b, tile, PITCH, i0, j0);
         return;
     }
     // rows i, k along j
@@ -268,6 +336,35 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void k_orth_product(pro
     }
 }
 
+// Tiles of 128 x 128, two workgroups per CU; those that would be left for a last round that fills less than two thirds of the chip are
+// cut into four.  Workgroups go round the eight dies by their index: each die gets a run of neighbouring tiles, so that its L2 cache
+// serves their common operands.
+template <int MODE>
+__global__ __launch_bounds__(256) void k_orth_product(product p) {
+    typedef staged<128, 128, 64, 64> big;
+    __shared__ __attribute__((aligned(16))) char lds[big::BYTES];
+    constexpr bool HALF = MODE == GRAM || MODE == POLY;
+    int t = blockIdx.x, quarter = -1, ti, tj;
+    if (t < p.whole) {
+        const int per = p.whole / 8;
+        if (t < per * 8) t = t % 8 * per + t / 8;
+    } else {
+        quarter = (t - p.whole) & 3;
+        t = p.whole + ((t - p.whole) >> 2);
+    }
+    if (HALF) below(t, ti, tj);
+    else {          // in bands of eight rows of tiles
+        const int band = t / (8 * p.tiles_j), r = t - band * 8 * p.tiles_j, rows = min(8, p.tiles_i - band * 8);
+        ti = band * 8 + r % rows; tj = r / rows;
+    }
+    if (quarter < 0) product_tile<128, 128, 64, 64, MODE>(p, ti, tj, lds);
+    else {
+        ti = ti * 2 + (quarter >> 1); tj = tj * 2 + (quarter & 1);
+        if (HALF && tj > ti) return;
+        product_tile<64, 64, 32, 32, MODE>(p, ti, tj, lds);
+    }
+}
+
 // ---- the same products where there are too few tiles, or too few steps along k, to fill the chip with staged ones ----------------------
 // One 32 x 32 tile per workgroup, eight waves take every eighth step along k straight from memory: all their loads are on the way at
 // once, nothing is staged and nothing waited for but the sum over the waves.  Every element comes from the L2 cache 32 times
@@ -280,13 +377,8 @@ __global__ __launch_bounds__(512) void k_orth_direct(product p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int64_t b = blockIdx.z;
     int ti, tj;
-    if (MODE == GRAM || MODE == POLY) {
-        const int t = blockIdx.x;
-        ti = (int)((sqrtf(8.0f * t + 1.0f) - 1.0f) * 0.5f);
-        while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
-        while (ti * (ti + 1) / 2 > t) --ti;
-        tj = t - ti * (ti + 1) / 2;
-    } else {
+    if (MODE == GRAM || MODE == POLY) below(blockIdx.x, ti, tj);
+    else {
         ti = blockIdx.x % p.tiles_i; tj = blockIdx.x / p.tiles_i;
     }
     const _Float16* P = p.P + b * p.P_b + (int64_t)ti * 2 * p.kb * FRAG + lane * 8;
@@ -336,15 +428,7 @@ __global__ __launch_bounds__(512) void k_orth_direct(product p) {
     }
     __syncthreads();
     if (MODE == LAST) {
-        const bool down = p.out_at.si == 1 && p.out_at.sj != 1;
-        for (int e = threadIdx.x; e < 1024; e += 512) {
-            const int i = down ? e & 31 : e >> 5, j = down ? e >> 5 : e & 31;
-            if (i0 + i < p.m && j0 + j < p.n) {
-                float v = tile[i][j] * (p.gain / (SCALE * SCALE));
-                if (p.w) v = fmaf(p.keep, load_elem(p.w, p.w_type, b * p.w_at.b + (i0 + i) * p.w_at.si + (j0 + j) * p.w_at.sj), v);
-                store_elem(p.out, p.out_type, b * p.out_at.b + (i0 + i) * p.out_at.si + (j0 + j) * p.out_at.sj, v);
-            }
-        }
+        emit<32, 32, 512>(p, b, &tile[0][0], 33, i0, j0);
         return;
     }
     if (wave >= 4 || (MODE != STEP && wave >= 2 && ti == tj)) return;
@@ -373,7 +457,7 @@ struct small {
     int32_t m, n, steps, turned;
     float a, b, c;
     void* out; const void* w; int out_type, w_type;
-    matrix out_at, w_at;
+    int64_t out_b, out_r, w_b, w_r;
     float keep, gain;
 };
 
@@ -385,42 +469,42 @@ __global__ __launch_bounds__(512) void k_orth_small(small p) {
     __shared__ __attribute__((aligned(16))) _Float16 am[RB][S][FRAG];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), q = lane >> 4, c = lane & 15;
     const int64_t b = blockIdx.x;
-    float x[JB][RB][4];
+    // in the caller's order, four neighbours a thread, and through LDS (xr's, not needed yet) into the lanes that work on them;
+    // columns swapped by row, so that neither order meets in one bank
+    constexpr int NP = WAVES * JB * 16;
+    float* flat = (float*)&xr[0][0][0][0];
+    auto place = [&](int i, int j) -> float& { return flat[i * NP + (j ^ (i & 31))]; };
+    const int rows = p.turned ? p.n : p.m, cols = p.turned ? p.m : p.n, per = (cols + 3) / 4;
+    const bool padded = p.m < RB * 16 || p.n < NP;
+    if (padded) {
+        for (int e = threadIdx.x; e < RB * 16 * NP; e += 512) flat[e] = 0.0f;
+        __syncthreads();
+    }
     double sum = 0.0;
-#pragma unroll
-    for (int jb = 0; jb < JB; ++jb)
-#pragma unroll
-        for (int I = 0; I < RB; ++I)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * I + 4 * q + r, j = (wave * JB + jb) * 16 + c;
-                float u = 0.0f;
-                if (i < p.m && j < p.n) {
-                    const int64_t row = p.turned ? j : i, col = p.turned ? i : j;
-                    u = load_elem(p.s.g, p.s.dtype, b * p.s.g_b + row * p.s.g_r + col);
-                    if (p.s.m) {
-                        const float v = fmaf(p.s.beta, p.s.m[b * p.s.m_b + row * p.s.m_r + col], u);
-                        p.s.m_out[b * p.s.o_b + row * p.s.o_r + col] = v;
-                        u = p.s.nesterov ? fmaf(p.s.beta, v, u) : v;
-                    }
-                }
-                x[jb][I][r] = u;
-                sum += (double)u * u;
-            }
+#pragma unroll 4
+    for (int e = threadIdx.x; e < rows * per; e += 512) {
+        const int r = e / per, col = (e - r * per) * 4, left = min(4, cols - col);
+        const float4_ u = moved(p.s, b, r, col, left, true);
+        for (int k = 0; k < 4; ++k) {
+            if (k < left) (p.turned ? place(col + k, r) : place(r, col + k)) = u[k];
+            sum += (double)u[k] * u[k];
+        }
+    }
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     double* sums = (double*)red;
     if (lane == 0) sums[wave] = sum;
     __syncthreads();
     sum = 0.0;
     for (int w = 0; w < WAVES; ++w) sum += sums[w];
-    __syncthreads();
+    float x[JB][RB][4];
     const double inv = sum != 0.0 ? (double)SCALE / sqrt(sum) : 0.0;          // (NaN != 0)
 #pragma unroll
     for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
         for (int I = 0; I < RB; ++I)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[jb][I][r] = (float)(x[jb][I][r] * inv);
+            for (int r = 0; r < 4; ++r) x[jb][I][r] = (float)(place(16 * I + 4 * q + r, (wave * JB + jb) * 16 + c) * inv);
+    __syncthreads();
 
     for (int step = 0; step < p.steps; ++step) {
         // X as operands: over rows in registers, over columns through LDS (this wave's part only)
@@ -521,19 +605,31 @@ __global__ __launch_bounds__(512) void k_orth_small(small p) {
                 for (int r = 0; r < 4; ++r) x[jb][I][r] = t[r] * (1.0f / SCALE);
             }
     }
+    __syncthreads();          // (the last reads of xr)
 #pragma unroll
     for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
         for (int I = 0; I < RB; ++I)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = 16 * I + 4 * q + r, j = (wave * JB + jb) * 16 + c;
-                if (i < p.m && j < p.n) {
-                    float v = x[jb][I][r] * (p.gain / SCALE);
-                    if (p.w) v = fmaf(p.keep, load_elem(p.w, p.w_type, b * p.w_at.b + i * p.w_at.si + j * p.w_at.sj), v);
-                    store_elem(p.out, p.out_type, b * p.out_at.b + i * p.out_at.si + j * p.out_at.sj, v);
-                }
+            for (int r = 0; r < 4; ++r) place(16 * I + 4 * q + r, (wave * JB + jb) * 16 + c) = x[jb][I][r];
+    __syncthreads();
+    const float gain = p.gain / SCALE;
+#pragma unroll 4
+    for (int e = threadIdx.x; e < rows * per; e += 512) {
+        const int r = e / per, col = (e - r * per) * 4, left = min(4, cols - col);
+        const int64_t at = b * p.out_b + r * p.out_r + col, wat = b * p.w_b + r * p.w_r + col;
+        float4_ v = {};
+        for (int k = 0; k < 4; ++k) if (k < left) v[k] = (p.turned ? place(col + k, r) : place(r, col + k)) * gain;
+        if (left >= 4) {
+            if (p.w) {
+                const float4_ w = load4(p.w, p.w_type, wat);
+                for (int k = 0; k < 4; ++k) v[k] = fmaf(p.keep, w[k], v[k]);
             }
+            store4(p.out, p.out_type, at, v);
+        } else {
+            for (int k = 0; k < left; ++k) store_elem(p.out, p.out_type, at + k, p.w ? fmaf(p.keep, load_elem(p.w, p.w_type, wat + k), v[k]) : v[k]);
+        }
+    }
 }
 
 }  // namespace dlo
