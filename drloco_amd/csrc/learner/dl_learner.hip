@@ -141,12 +141,27 @@ orth_form orth_plan(const dl_orth_shape* s) {
     return f;
 }
 
-// 512 tiles of 128 fill the chip (two per CU); see k_orth_product
-template <int TILE, int MODE> void launch_product(dlo::product p, int64_t tiles, int64_t batch, hipStream_t st) {
+// How many of `tiles` per matrix run whole when `slots` of them fill the chip: a last round of less than two thirds is cut up.
+int32_t whole_tiles(int64_t tiles, int64_t batch, int64_t slots) {
+    const int64_t rest = tiles * batch % slots;
+    return rest * 3 >= slots * 2 ? (int32_t)tiles : (int32_t)(tiles - std::min(tiles, ceil_div(rest, batch)));
+}
+
+// Tiles of 256 x 128 (a CU each) where they come to at least nine tenths of a round of whole ones and what is left in 64 x 64 to one
+// round at most, else of 128 x 128 (two to a CU).  4096 x 8192 x 4096: 610 instead of 652 us; 2 x 1031 x 4099 x 1031, where 328 of
+// 64 x 64 would be left: 71 and 68 us.
+template <int TILE, int MODE> void launch_product(dlo::product p, int64_t tiles, int64_t batch, const dlo::plan& q, hipStream_t st) {
     if constexpr (TILE == 32) dlo::k_orth_direct<MODE><<<dim3((unsigned)tiles, 1, (unsigned)batch), 512, 0, st>>>(p);
     else {
-        const int64_t all = tiles * batch, rest = all % 512 >= 340 ? 0 : all % 512;
-        p.whole = (int32_t)(tiles - std::min(tiles, ceil_div(rest, batch)));
+        constexpr bool half = MODE == dlo::GRAM || MODE == dlo::POLY;
+        const int64_t wi = q.mp / 256, wj = q.np / 128, wide = half ? wi * (wi + 1) : wi * wj, whole = whole_tiles(wide, batch, 256);
+        const int64_t left = (wide - whole) * 8 + (q.mp % 256 ? 2 * (half ? q.mp / 64 : q.np / 64) : 0);
+        if (whole * batch >= 230 && left * batch <= 256) {
+            p.tiles = (int32_t)wide; p.whole = (int32_t)whole;
+            p.tiles_i = (int32_t)wi; p.tiles_j = (int32_t)wj;
+            return dlo::k_orth_wide<MODE><<<dim3((unsigned)(whole + left), 1, (unsigned)batch), 256, 0, st>>>(p);
+        }
+        p.tiles = (int32_t)tiles; p.whole = whole_tiles(tiles, batch, 512);
         dlo::k_orth_product<MODE><<<dim3((unsigned)(p.whole + (tiles - p.whole) * 4), 1, (unsigned)batch), 256, 0, st>>>(p);
     }
 }
@@ -162,16 +177,16 @@ template <int TILE> void launch_steps(const dl_orth_shape* s, const orth_form& f
         dlo::product p = last;
         p.P = p.Q = xr; p.P_b = p.Q_b = f.p.x_size; p.kb = kn;
         p.out0 = A; p.out0_b = f.p.a_size; p.out0_kb = km;
-        launch_product<TILE, dlo::GRAM>(p, tri, s->batch, st);
+        launch_product<TILE, dlo::GRAM>(p, tri, s->batch, f.p, st);
         p.P = p.Q = A; p.P_b = p.Q_b = f.p.a_size; p.kb = km;
         p.A = A; p.out0 = Q;
-        launch_product<TILE, dlo::POLY>(p, tri, s->batch, st);
+        launch_product<TILE, dlo::POLY>(p, tri, s->batch, f.p, st);
         p.P = Q; p.Q = xc[k & 1]; p.Q_b = f.p.x_size;
         p.tiles_i = (int32_t)ti; p.tiles_j = (int32_t)tj;
         p.out0 = xr; p.out0_b = f.p.x_size; p.out0_kb = kn;
         p.out1 = xc[(k + 1) & 1]; p.out1_b = f.p.x_size; p.out1_kb = km;
-        if (k + 1 < s->steps) launch_product<TILE, dlo::STEP>(p, ti * tj, s->batch, st);
-        else launch_product<TILE, dlo::LAST>(p, ti * tj, s->batch, st);
+        if (k + 1 < s->steps) launch_product<TILE, dlo::STEP>(p, ti * tj, s->batch, f.p, st);
+        else launch_product<TILE, dlo::LAST>(p, ti * tj, s->batch, f.p, st);
     }
 }
 

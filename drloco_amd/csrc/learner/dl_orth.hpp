@@ -178,7 +178,7 @@ struct product {
     const _Float16* P; const _Float16* Q;          // operands, [rows / 16][kb][FRAG]
     int64_t P_b, Q_b;
     int32_t kb;                                    // steps of 32 along k
-    int32_t tiles_i, tiles_j, whole;               // k_orth_product: tiles that are not cut into four
+    int32_t tiles_i, tiles_j, tiles, whole;        // tiles, and those of them that are not cut up
     _Float16* out0; int64_t out0_b, out0_kb;       // GRAM, POLY: the symmetric result;  STEP: XR
     _Float16* out1; int64_t out1_b, out1_kb;       // STEP: XC
     const _Float16* A;                             // POLY: as out0
@@ -222,83 +222,34 @@ __device__ __forceinline__ void emit(const product& p, int64_t b, const float* t
     }
 }
 
-template <int BM, int BN, int WM, int WN> struct staged {
+template <bool V> struct flag { static constexpr bool value = V; };
+template <int N> struct number { static constexpr int value = N; };
+
+// A tile of BM x BN in waves of WM x WN, NS steps of operands in LDS.
+template <int BM, int BN, int WM, int WN, int NS> struct staged {
     static constexpr int WAVES = (BM / WM) * (BN / WN), ROWS = BM / 16 + BN / 16;          // fragments of a step
     static constexpr int PITCH = BN + 4, STAGE = ROWS * FRAG * 2;                          // bytes
-    static constexpr int BYTES = 2 * STAGE > BM * PITCH * 4 ? 2 * STAGE : BM * PITCH * 4;
+    static constexpr int BYTES = NS * STAGE > BM * PITCH * 4 ? NS * STAGE : BM * PITCH * 4;
+    static constexpr int MOVES = ROWS * 2 / WAVES;                                         // copies of a wave and step
+    static_assert(ROWS * 2 % WAVES == 0, "every wave moves the same number of pieces");
 };
 
-template <int BM, int BN, int WM, int WN, int MODE>
-__device__ __forceinline__ void product_tile(const product& p, int ti, int tj, char* lds) {
-    typedef staged<BM, BN, WM, WN> L;
-    constexpr int WAVES = L::WAVES, TM = WM / 16, TN = WN / 16, ROWS = L::ROWS, PITCH = L::PITCH, STAGE = L::STAGE;
+// The finished tile in LDS (BM x BN sums, [i * PITCH + j]) on its way to memory.
+template <int BM, int BN, int WAVES, int MODE>
+__device__ __forceinline__ void finish(const product& p, float* tile, int i0, int j0) {
+    constexpr int PITCH = BN + 4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int64_t b = blockIdx.z;
-    const _Float16* P = p.P + b * p.P_b + (int64_t)ti * (BM / 16) * p.kb * FRAG;
-    const _Float16* Q = p.Q + b * p.Q_b + (int64_t)tj * (BN / 16) * p.kb * FRAG;
-
-    // a step's fragments: one instruction of a wave moves 1 KB, a plane of a fragment
-    auto fetch = [&](int k, int stage) {
-#pragma unroll
-        for (int f = 0; f < ROWS * 2 / WAVES; ++f) {
-            const int piece = f * WAVES + wave, r = piece >> 1, plane = piece & 1;
-            const _Float16* from = (r < BM / 16 ? P + ((int64_t)r * p.kb + k) * FRAG : Q + ((int64_t)(r - BM / 16) * p.kb + k) * FRAG) + plane * 512 + lane * 8;
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)(lds + stage * STAGE + piece * 1024), 16, 0, 0);
-        }
-    };
-    static_assert(ROWS * 2 % WAVES == 0, "every wave moves the same number of pieces");
-
-    float4_ acc[TM][TN] = {};
-    const int wi = wave / (BN / WN), wj = wave % (BN / WN);
-    fetch(0, 0);
-    for (int k = 0; k < p.kb; ++k) {
-        // this wave's copies have arrived, and with the barrier everyone's; everyone is also done reading the other stage
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (k + 1 < p.kb) fetch(k + 1, (k + 1) & 1);
-        const char* stage = lds + (k & 1) * STAGE;
-        half8 ph[TM], pl[TM], qh[TN], ql[TN];
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const char* f = stage + (wi * TM + i) * 2048 + lane * 16;
-            ph[i] = *(const half8*)f; pl[i] = *(const half8*)(f + 1024);
-        }
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const char* f = stage + (BM / 16 + wj * TN + j) * 2048 + lane * 16;
-            qh[j] = *(const half8*)f; ql[j] = *(const half8*)(f + 1024);
-        }
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[i], ql[j], acc[i][j], 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl[i], qh[j], acc[i][j], 0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[i], qh[j], acc[i][j], 0, 0, 0);
-    }
-    __syncthreads();
-    // the tile through LDS, so that both orientations leave in whole fragments.  A lane holds rows 4 (lane / 16) + r of column lane % 16.
-    float* tile = (float*)lds;
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) tile[(wi * WM + i * 16 + (lane >> 4) * 4 + r) * PITCH + wj * WN + j * 16 + (lane & 15)] = acc[i][j][r];
-    __syncthreads();
-    const int i0 = ti * BM, j0 = tj * BN, row = lane & 15, k8 = (lane >> 4) * 8;
+    const int row = lane & 15, k8 = (lane >> 4) * 8;
     if (MODE == LAST) {
         emit<BM, BN, WAVES * 64>(p, b, tile, PITCH, i0, j0);
         return;
     }
-    // rows i, k along j
+    // rows i, k along j.  Of a symmetric result only the blocks of 32 on and below the diagonal count.
+    constexpr bool HALF = MODE == GRAM || MODE == POLY;
     for (int f = wave; f < (BM / 16) * (BN / 32); f += WAVES) {
         const int ri = f / (BN / 32), kj = f % (BN / 32);
+        if (HALF && i0 / 32 + ri / 2 < j0 / 32 + kj) continue;
         const int64_t at = (((int64_t)(i0 / 16 + ri)) * p.out0_kb + j0 / 32 + kj) * FRAG + lane * 8;
         float* src = tile + (ri * 16 + row) * PITCH + kj * 32 + k8;
         half8 hi, lo, ah, al;
@@ -316,32 +267,208 @@ __device__ __forceinline__ void product_tile(const product& p, int ti, int tj, c
         _Float16* to = p.out0 + b * p.out0_b + at;
         *(half8*)to = hi; *(half8*)(to + 512) = lo;
     }
-    if (MODE == STEP || ti != tj) {
-        if (MODE == POLY) __syncthreads();
-        // rows j, k along i: the mirror image of a symmetric result, or X's other orientation
-        _Float16* out = MODE == STEP ? p.out1 + b * p.out1_b : p.out0 + b * p.out0_b;
-        const int64_t kbs = MODE == STEP ? p.out1_kb : p.out0_kb;
-        for (int f = wave; f < (BN / 16) * (BM / 32); f += WAVES) {
-            const int rj = f / (BM / 32), ki = f % (BM / 32);
-            half8 hi, lo;
+    if (MODE == POLY) __syncthreads();
+    // rows j, k along i: the mirror image of a symmetric result, or X's other orientation
+    _Float16* out = HALF ? p.out0 + b * p.out0_b : p.out1 + b * p.out1_b;
+    const int64_t kbs = HALF ? p.out0_kb : p.out1_kb;
+    for (int f = wave; f < (BN / 16) * (BM / 32); f += WAVES) {
+        const int rj = f / (BM / 32), ki = f % (BM / 32);
+        if (HALF && i0 / 32 + ki <= j0 / 32 + rj / 2) continue;
+        half8 hi, lo;
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                _Float16 h, l;
-                split(tile[(ki * 32 + k8 + q) * PITCH + rj * 16 + row] * (1.0f / SCALE), h, l);
-                hi[q] = h; lo[q] = l;
-            }
-            _Float16* to = out + ((int64_t)(j0 / 16 + rj) * kbs + i0 / 32 + ki) * FRAG + lane * 8;
-            *(half8*)to = hi; *(half8*)(to + 512) = lo;
+        for (int q = 0; q < 8; ++q) {
+            _Float16 h, l;
+            split(tile[(ki * 32 + k8 + q) * PITCH + rj * 16 + row] * (1.0f / SCALE), h, l);
+            hi[q] = h; lo[q] = l;
         }
+        _Float16* to = out + ((int64_t)(j0 / 16 + rj) * kbs + i0 / 32 + ki) * FRAG + lane * 8;
+        *(half8*)to = hi; *(half8*)(to + 512) = lo;
     }
+}
+
+// i0, j0: the tile's first row and column
+template <int BM, int BN, int WM, int WN, int NS, int MODE>
+__device__ __forceinline__ void product_tile(const product& p, int i0, int j0, char* lds) {
+    typedef staged<BM, BN, WM, WN, NS> L;
+    constexpr int WAVES = L::WAVES, TM = WM / 16, TN = WN / 16, ROWS = L::ROWS, PITCH = L::PITCH, STAGE = L::STAGE;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int64_t b = blockIdx.z;
+    const _Float16* P = p.P + b * p.P_b + (int64_t)(i0 / 16) * p.kb * FRAG;
+    const _Float16* Q = p.Q + b * p.Q_b + (int64_t)(j0 / 16) * p.kb * FRAG;
+
+    // a step's copies into a stage: one instruction of a wave moves 1 KB, a plane of a fragment
+    auto copy = [&](int f, int k, int stage) {
+        const int piece = f * WAVES + wave, r = piece >> 1, plane = piece & 1;
+        const _Float16* from = (r < BM / 16 ? P + (int64_t)r * p.kb * FRAG : Q + (int64_t)(r - BM / 16) * p.kb * FRAG) + ((int64_t)k * FRAG + plane * 512);
+        auto at = (const __attribute__((address_space(1))) char*)from;
+        asm("" : "+s"(at));          // the same for the wave: stays in scalar registers
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(at + (uint32_t)(lane * 16)), (__attribute__((address_space(3))) void*)(lds + stage * STAGE + piece * 1024), 16, 0, 0);
+    };
+    constexpr int READS = 2 * (TM + TN), PRODUCTS = 3 * TM * TN;
+    float4_ acc[TM][TN] = {};
+    const int wi = wave / (BN / WN), wj = wave % (BN / WN);
+    struct fragments { half8 h[TM + TN], l[TM + TN]; };          // of P, then of Q
+    auto read = [&](fragments& f, int n, int stage) {
+        const int r = n >> 1;
+        const char* from = lds + stage * STAGE + (r < TM ? wi * TM + r : BM / 16 + wj * TN + r - TM) * 2048 + (n & 1) * 1024 + lane * 16;
+        (n & 1 ? f.l : f.h)[r] = *(const half8*)from;
+    };
+    auto multiply = [&](const fragments& f, int n) {          // hi lo for all, lo hi for all, hi hi for all: no sum twice in a row
+        const int kind = n / (TM * TN), i = n / TN % TM, j = n % TN;
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kind == 1 ? f.l[i] : f.h[i], kind == 0 ? f.l[TM + j] : f.h[TM + j], acc[i][j], 0, 0, 0);
+    };
+    int stage = 0;                // of the step to be read
+    // this wave's copies for the step to be read have arrived, and with the barrier everyone's; its reads of the step before are done
+    auto arrived = [&](auto later) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(decltype(later)::value * L::MOVES) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    // While step k is multiplied from registers, step k + 1 is read from LDS and step k + NS is copied into the stage whose last readers
+    // the barrier has seen finish; one read and half a copy to every few products, in this order.
+    auto advance = [&](const fragments& now, fragments& next, int k, auto copies) {
+        const int to = (stage + NS - 1) % NS, from = min(k + NS, p.kb - 1);          // (behind the end: the last step once more)
+#pragma unroll
+        for (int n = 0; n < READS; ++n) {
+            read(next, n, stage);
+            if (decltype(copies)::value && n % (READS / L::MOVES) == 0 && n / (READS / L::MOVES) < L::MOVES) copy(n / (READS / L::MOVES), from, to);
+#pragma unroll
+            for (int e = PRODUCTS * n / READS; e < PRODUCTS * (n + 1) / READS; ++e) multiply(now, e);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        stage = (stage + 1) % NS;
+    };
+    fragments even, odd;
+#pragma unroll
+    for (int k = 0; k < NS - 1; ++k)
+#pragma unroll
+        for (int f = 0; f < L::MOVES; ++f) copy(f, min(k, p.kb - 1), k);
+    arrived(number<NS - 2>());
+#pragma unroll
+    for (int n = 0; n < READS; ++n) read(even, n, 0);
+#pragma unroll
+    for (int f = 0; f < L::MOVES; ++f) copy(f, min(NS - 1, p.kb - 1), NS - 1);
+    stage = 1;
+    for (int k = 0; k + 2 < p.kb; k += 2) {          // (kb is even, and at least 4: sides are padded to 128)
+        arrived(number<NS - 2>());
+        advance(even, odd, k, flag<true>());
+        arrived(number<NS - 2>());
+        advance(odd, even, k + 1, flag<true>());
+    }
+    arrived(number<0>());
+    advance(even, odd, p.kb - 2, flag<false>());
+#pragma unroll
+    for (int e = 0; e < PRODUCTS; ++e) multiply(odd, e);
+    __syncthreads();
+    // the tile through LDS, so that both orientations leave in whole fragments.  A lane holds rows 4 (lane / 16) + r of column lane % 16.
+    float* tile = (float*)lds;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) tile[(wi * WM + i * 16 + (lane >> 4) * 4 + r) * PITCH + wj * WN + j * 16 + (lane & 15)] = acc[i][j][r];
+    __syncthreads();
+    finish<BM, BN, WAVES, MODE>(p, tile, i0, j0);
+}
+
+// 256 x 128 in four waves of 128 x 64: a wave keeps the four column fragments of a step and lets the eight row fragments pass by, two
+// ahead of their products; the next step's column fragments come in during the second half of a step, behind the one barrier.
+// (With all fragments of two steps at hand the sums no longer fit the vector registers, and are carried to and fro.)
+template <int MODE>
+__device__ __forceinline__ void wide_tile(const product& p, int i0, int j0, char* lds) {
+    typedef staged<256, 128, 128, 64, 3> L;
+    constexpr int TM = 8, TN = 4, PITCH = L::PITCH, STAGE = L::STAGE;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), wi = wave >> 1, wj = wave & 1;
+    const int64_t b = blockIdx.z;
+    const _Float16* P = p.P + b * p.P_b + (int64_t)(i0 / 16) * p.kb * FRAG;
+    const _Float16* Q = p.Q + b * p.Q_b + (int64_t)(j0 / 16) * p.kb * FRAG;
+    auto copy = [&](int f, int k, int stage) {
+        const int piece = f * 4 + wave, r = piece >> 1, plane = piece & 1;
+        const _Float16* from = (r < 16 ? P + (int64_t)r * p.kb * FRAG : Q + (int64_t)(r - 16) * p.kb * FRAG) + ((int64_t)k * FRAG + plane * 512);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + lane * 8), (__attribute__((address_space(3))) void*)(lds + stage * STAGE + piece * 1024), 16, 0, 0);
+    };
+    struct fragment { half8 h, l; };
+    auto read = [&](fragment& f, int r, int stage) {
+        const char* from = lds + stage * STAGE + r * 2048 + lane * 16;
+        f.h = *(const half8*)from;
+        f.l = *(const half8*)(from + 1024);
+    };
+    float4_ acc[TM][TN] = {};
+    fragment row[4], even[TN], odd[TN];
+    int now = 0, next = 1, free = 2;          // stages
+    auto step = [&](const fragment (&col)[TN], fragment (&coming)[TN], int k, auto more) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            if (decltype(more)::value && i == TM / 2) {
+                // this wave's copies for step k + 1 have arrived, and with the barrier everyone's; everyone is past step k - 1
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+            }
+            if (i + 2 < TM) read(row[(i + 2) & 3], wi * TM + i + 2, now);
+            else if (decltype(more)::value) read(row[(i + 2) & 3], wi * TM + i + 2 - TM, next);
+            if (decltype(more)::value && i >= TM / 2) {
+                read(coming[i - TM / 2], 16 + wj * TN + i - TM / 2, next);
+#pragma unroll
+                for (int f = 0; f < 3; ++f) copy((i - TM / 2) * 3 + f, min(k + 2, p.kb - 1), free);          // (behind the end: the last step once more)
+            }
+            const fragment& r = row[i & 3];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(r.h, col[j].l, acc[i][j], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(r.l, col[j].h, acc[i][j], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(r.h, col[j].h, acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        const int was = now;
+        now = next; next = free; free = was;
+    };
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int f = 0; f < L::MOVES; ++f) copy(f, k, k);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(L::MOVES) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read(row[0], wi * TM, 0);
+    read(row[1], wi * TM + 1, 0);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) read(even[j], 16 + wj * TN + j, 0);
+    auto pin = [&] {          // the sums stay in accumulation registers
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) asm volatile("" : "+a"(acc[i][j]));
+    };
+    pin();
+    for (int k = 0; k + 2 < p.kb; k += 2) {          // (kb is even, and at least 4: sides are padded to 128)
+        step(even, odd, k, flag<true>());
+        step(odd, even, k + 1, flag<true>());
+        pin();
+    }
+    step(even, odd, p.kb - 2, flag<true>());
+    step(odd, even, p.kb - 1, flag<false>());
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    float* tile = (float*)lds;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) tile[(wi * 128 + i * 16 + (lane >> 4) * 4 + r) * PITCH + wj * 64 + j * 16 + (lane & 15)] = acc[i][j][r];
+    __syncthreads();
+    finish<256, 128, 4, MODE>(p, tile, i0, j0);
 }
 
 // Tiles of 128 x 128, two workgroups per CU; those that would be left for a last round that fills less than two thirds of the chip are
 // cut into four.  Workgroups go round the eight dies by their index: each die gets a run of neighbouring tiles, so that its L2 cache
 // serves their common operands.
 template <int MODE>
-__global__ __launch_bounds__(256) void k_orth_product(product p) {
-    typedef staged<128, 128, 64, 64> big;
+__global__ __launch_bounds__(256, 2) void k_orth_product(product p) {
+    typedef staged<128, 128, 64, 64, 2> big;
     __shared__ __attribute__((aligned(16))) char lds[big::BYTES];
     constexpr bool HALF = MODE == GRAM || MODE == POLY;
     int t = blockIdx.x, quarter = -1, ti, tj;
@@ -357,12 +484,51 @@ __global__ __launch_bounds__(256) void k_orth_product(product p) {
         const int band = t / (8 * p.tiles_j), r = t - band * 8 * p.tiles_j, rows = min(8, p.tiles_i - band * 8);
         ti = band * 8 + r % rows; tj = r / rows;
     }
-    if (quarter < 0) product_tile<128, 128, 64, 64, MODE>(p, ti, tj, lds);
+    if (quarter < 0) product_tile<128, 128, 64, 64, 2, MODE>(p, ti * 128, tj * 128, lds);
     else {
         ti = ti * 2 + (quarter >> 1); tj = tj * 2 + (quarter & 1);
         if (HALF && tj > ti) return;
-        product_tile<64, 64, 32, 32, MODE>(p, ti, tj, lds);
+        product_tile<64, 64, 32, 32, 4, MODE>(p, ti * 64, tj * 64, lds);
     }
+}
+
+// Tiles of 256 x 128, one workgroup per CU, for results that fill the chip with them.  A wave's 128 x 64 need 24 reads of LDS for 96
+// products; with 64 x 64 it is 16 for 48, and LDS is what they wait for.  `whole` tiles, the rest of them in 64 x 64, and 64 x 64 for
+// the last 128 rows where the padded short side is an odd multiple of 128.
+template <int MODE>
+__global__ __launch_bounds__(256, 1) void k_orth_wide(product p) {
+    typedef staged<256, 128, 128, 64, 3> big;
+    __shared__ __attribute__((aligned(16))) char lds[big::BYTES];
+    constexpr bool HALF = MODE == GRAM || MODE == POLY;
+    int t = blockIdx.x, ti, tj;
+    const int cut = (p.tiles - p.whole) * 8;
+    if (t >= p.whole + cut) {          // the last 128 rows
+        t -= p.whole + cut;
+        ti = p.tiles_i * 4 + (t & 1); tj = t >> 1;
+        if (HALF && tj > ti) return;
+        return product_tile<64, 64, 32, 32, 8, MODE>(p, ti * 64, tj * 64, lds);
+    }
+    int part = -1;
+    if (t < p.whole) {
+        const int per = p.whole / 8;
+        if (t < per * 8) t = t % 8 * per + t / 8;
+    } else {
+        part = (t - p.whole) & 7;
+        t = p.whole + ((t - p.whole) >> 3);
+    }
+    if (HALF) {          // row ti of tiles has 2 ti + 2 of them, ti (ti + 1) come before
+        ti = (int)((sqrtf(4.0f * t + 1.0f) - 1.0f) * 0.5f);
+        while ((ti + 1) * (ti + 2) <= t) ++ti;
+        while (ti * (ti + 1) > t) --ti;
+        tj = t - ti * (ti + 1);
+    } else {          // in bands of four rows of tiles
+        const int band = t / (4 * p.tiles_j), r = t - band * 4 * p.tiles_j, rows = min(4, p.tiles_i - band * 4);
+        ti = band * 4 + r % rows; tj = r / rows;
+    }
+    if (part < 0) return wide_tile<MODE>(p, ti * 256, tj * 128, lds);
+    ti = ti * 4 + (part >> 1); tj = tj * 2 + (part & 1);
+    if (HALF && tj > ti) return;
+    product_tile<64, 64, 32, 32, 8, MODE>(p, ti * 64, tj * 64, lds);
 }
 
 // ---- the same products where there are too few tiles, or too few steps along k, to fill the chip with staged ones ----------------------
