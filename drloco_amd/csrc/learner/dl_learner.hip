@@ -73,7 +73,7 @@ form memory_form(const dl_memory_shape* s, int V) {
     f.parts = true;
     int64_t parts = ceil_div(4096, f.blocks);
     parts = std::min(parts, std::max<int64_t>(8, (int64_t)std::sqrt(4.0 * (double)s->T * elem_bytes(s->dtype))));
-    parts = std::max<int64_t>(1, std::min(parts, runs / 2));
+    parts = std::max<int64_t>(1, std::min(parts, runs));
     f.part = ceil_div(runs, parts) * dlm::MARK;
     f.chunks = ceil_div(ceil_div(s->T, f.part), dlm::PARTS);
     return f;
@@ -295,13 +295,17 @@ int dl_orth_update(const dl_orth_shape* s, const void* grad, const float* moment
     if (!aligned(workspace, 16)) return fail(DL_E_INVAL, "dl_orth_update: workspace must be aligned to 16 bytes");
     const orth_form f = orth_plan(s);
     hipStream_t st = (hipStream_t)stream;
+    const bool flat = s->grad_r == s->cols && (!momentum || (s->momentum_r == s->cols && s->momentum_out_r == s->cols));          // one row as good as many
     if (f.small) {
         dlo::small p{{grad, s->grad_type, momentum, momentum_out, (float)s->beta, s->nesterov, s->grad_b, s->grad_r, s->momentum_b, s->momentum_r, s->momentum_out_b, s->momentum_out_r},
-                     f.p.m, f.p.n, s->steps, f.turned, (float)s->a, (float)s->b, (float)s->c, out, weight, s->out_type, s->weight_type,
+                     f.p.m, f.p.n, s->steps, f.turned, flat && (!weight || s->weight_r == s->cols) && s->out_r == s->cols, (float)s->a, (float)s->b, (float)s->c, out, weight, s->out_type, s->weight_type,
                      s->out_b, s->out_r, s->weight_b, s->weight_r,
                      (float)s->weight_keep, (float)s->gain};
         const unsigned batch = (unsigned)s->batch;
         if (f.p.m > 32) dlo::k_orth_small<4, 2><<<batch, 512, 0, st>>>(p);
+        else if (f.p.m <= 16 && f.p.n <= 256) dlo::k_orth_small<1, 2><<<batch, 512, 0, st>>>(p);
+        else if (f.p.m <= 16 && f.p.n <= 512) dlo::k_orth_small<1, 4><<<batch, 512, 0, st>>>(p);
+        else if (f.p.m <= 16) dlo::k_orth_small<1, 8><<<batch, 512, 0, st>>>(p);
         else if (f.p.n <= 256) dlo::k_orth_small<2, 2><<<batch, 512, 0, st>>>(p);
         else if (f.p.n <= 512) dlo::k_orth_small<2, 4><<<batch, 512, 0, st>>>(p);
         else dlo::k_orth_small<2, 8><<<batch, 512, 0, st>>>(p);
@@ -310,7 +314,6 @@ int dl_orth_update(const dl_orth_shape* s, const void* grad, const float* moment
     double* partials = (double*)workspace;
     char* work = (char*)workspace + ceil_div(s->batch * f.p.partials * 8, 256) * 256;
     const dlo::source src{grad, s->grad_type, momentum, momentum_out, (float)s->beta, s->nesterov, s->grad_b, s->grad_r, s->momentum_b, s->momentum_r, s->momentum_out_b, s->momentum_out_r};
-    const bool flat = s->grad_r == s->cols && (!momentum || (s->momentum_r == s->cols && s->momentum_out_r == s->cols));
     dlo::k_orth_norm<<<dim3((unsigned)f.p.partials, (unsigned)s->batch), 256, 0, st>>>(src, flat ? 1 : s->rows, flat ? s->rows * s->cols : s->cols, partials);
     dlo::k_orth_load<<<dim3((unsigned)ceil_div(f.p.np, 64), (unsigned)ceil_div(f.p.mp, 64), (unsigned)s->batch), 256, 0, st>>>(src, f.p, f.turned, partials, (_Float16*)work, (_Float16*)(work + f.x_bytes));
     dlo::product p{};

@@ -20,6 +20,7 @@
 namespace dlo {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float float4_ __attribute__((ext_vector_type(4)));
 
 constexpr float SCALE = 1024.0f;
@@ -79,54 +80,59 @@ struct source {
     int64_t g_b, g_r, m_b, m_r, o_b, o_r;          // strides of g, m, m_out: matrix, row
 };
 
-// u of four neighbours (of `n` of them, where fewer are left), and the momentum on the way
-__device__ __forceinline__ float4_ moved(const source& s, int64_t b, int64_t r, int64_t c, int n, bool first) {
-    const int64_t g = b * s.g_b + r * s.g_r + c;
-    float4_ u = {};
-    if (n >= 4) u = load4(s.g, s.dtype, g);
-    else for (int e = 0; e < n; ++e) u[e] = load_elem(s.g, s.dtype, g + e);
-    if (s.m) {
-        const int64_t o = b * s.o_b + r * s.o_r + c;
-        float4_ v = {};
+// Four neighbours of a row (`n` of them, where fewer are left): everything is loaded, for several places at once, before the first is used.
+struct place {
+    int64_t b, r, c;
+    int n;
+    float4_ u, v;          // gradient and momentum, then what the update is made of
+    __device__ __forceinline__ void load(const source& s, bool first) {
+        u = v = float4_{};
+        const int64_t g = b * s.g_b + r * s.g_r + c;
+        if (n >= 4) u = load4(s.g, s.dtype, g);
+        else for (int e = 0; e < n; ++e) u[e] = load_elem(s.g, s.dtype, g + e);
+        if (s.m && n > 0) {
+            const float* m = first ? s.m + b * s.m_b + r * s.m_r + c : s.m_out + b * s.o_b + r * s.o_r + c;
+            if (n >= 4) v = load4_as<float>(m, 0);
+            else for (int e = 0; e < n; ++e) v[e] = m[e];
+        }
+    }
+    __device__ __forceinline__ void move(const source& s, bool first) {
+        if (!s.m || n <= 0) return;
         if (first) {
-            const int64_t m = b * s.m_b + r * s.m_r + c;
-            if (n >= 4) v = load4_as<float>(s.m, m);
-            else for (int e = 0; e < n; ++e) v[e] = s.m[m + e];
             for (int e = 0; e < 4; ++e) v[e] = fmaf(s.beta, v[e], u[e]);
-            if (n >= 4) store4_as<float>(s.m_out, o, v);
-            else for (int e = 0; e < n; ++e) s.m_out[o + e] = v[e];
-        } else {
-            if (n >= 4) v = load4_as<float>(s.m_out, o);
-            else for (int e = 0; e < n; ++e) v[e] = s.m_out[o + e];
+            float* o = s.m_out + b * s.o_b + r * s.o_r + c;
+            if (n >= 4) store4_as<float>(o, 0, v);
+            else for (int e = 0; e < n; ++e) o[e] = v[e];
         }
         for (int e = 0; e < 4; ++e) u[e] = s.nesterov ? fmaf(s.beta, v[e], u[e]) : v[e];
     }
-    return u;
-}
+};
 
 // rows x cols as they are read: one long row where the rows of all arrays follow each other
 __global__ __launch_bounds__(256) void k_orth_norm(source s, int64_t rows, int64_t cols, double* __restrict__ partials) {
-    const int64_t b = blockIdx.y, per = (cols + 3) / 4, all = rows * per;          // in fours
-    const int64_t step = (int64_t)gridDim.x * 256;
+    constexpr int AT_ONCE = 4;
+    const int64_t per = (cols + 3) / 4, all = rows * per, step = (int64_t)gridDim.x * 256;          // in fours
     double sum = 0.0;
-    if (rows == 1) {
-#pragma unroll 4
-        for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < all; e += step) {
-            const float4_ u = moved(s, b, 0, e * 4, (int)min((int64_t)4, cols - e * 4), true);
-            for (int k = 0; k < 4; ++k) sum += (double)u[k] * u[k];
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < all; e += AT_ONCE * step) {
+        place p[AT_ONCE];
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            const int64_t f = e + k * step, r = rows == 1 ? 0 : f / per;
+            p[k].b = blockIdx.y; p[k].r = r; p[k].c = (f - r * per) * 4;
+            p[k].n = f < all ? (int)min((int64_t)4, cols - p[k].c) : 0;
+            p[k].load(s, true);
         }
-    } else {
-        for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < all; e += step) {
-            const int64_t r = e / per, c = (e - r * per) * 4;
-            const float4_ u = moved(s, b, r, c, (int)min((int64_t)4, cols - c), true);
-            for (int k = 0; k < 4; ++k) sum += (double)u[k] * u[k];
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            p[k].move(s, true);
+            for (int q = 0; q < 4; ++q) sum += (double)p[k].u[q] * p[k].u[q];
         }
     }
     __shared__ double part[4];
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) partials[b * gridDim.x + blockIdx.x] = part[0] + part[1] + part[2] + part[3];
+    if (threadIdx.x == 0) partials[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = part[0] + part[1] + part[2] + part[3];
 }
 
 // ---- X = G / |G| into both orientations: one workgroup per 64 x 64 ---------------------------------------------------------------
@@ -135,24 +141,26 @@ __global__ __launch_bounds__(256) void k_orth_load(source s, plan p, int turned,
     __shared__ float tile[64][65];          // [short side][long side]
     const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;
     const int r0 = turned ? j0 : i0, c0 = turned ? i0 : j0, rows = turned ? p.n : p.m, cols = turned ? p.m : p.n;
-    float4_ u[4];
+    place at[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const int r = r0 + e * 16 + (threadIdx.x >> 4), c = c0 + (threadIdx.x & 15) * 4;
-        u[e] = float4_{};
-        if (r < rows && c < cols) u[e] = moved(s, b, r, c, min(4, cols - c), false);
+        at[e].b = b; at[e].r = r0 + e * 16 + (threadIdx.x >> 4); at[e].c = c0 + (threadIdx.x & 15) * 4;
+        at[e].n = at[e].r < rows ? min(4, cols - (int)at[e].c) : 0;
+        at[e].load(s, false);
     }
     double sum = 0.0;
     for (int k = lane; k < p.partials; k += 64) sum += partials[(int64_t)b * p.partials + k];
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     const double inv = sum != 0.0 ? (double)SCALE / sqrt(sum) : 0.0;          // (NaN != 0)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < 4; ++e) {
+        at[e].move(s, false);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int r = e * 16 + (threadIdx.x >> 4), c = (threadIdx.x & 15) * 4 + k;
-            (turned ? tile[c][r] : tile[r][c]) = (float)(u[e][k] * inv);
+            (turned ? tile[c][r] : tile[r][c]) = (float)(at[e].u[k] * inv);
         }
+    }
     __syncthreads();
     // 4 x 2 fragments with rows i and 4 x 2 with rows j
 #pragma unroll
@@ -615,48 +623,111 @@ __global__ __launch_bounds__(512) void k_orth_direct(product p) {
 // m <= 16 RB rows, n <= 128 JB columns.  Wave w owns 16 JB columns.  A result of the matrix cores leaves lane (q, c) = (lane / 16, lane % 16)
 // with rows 16 I + 4 q + r of column c; as an operand over k = 32 s .. a lane needs eight k's, the same ones in both operands, in
 // any order.  With the order {32 s + 4 q + r, 32 s + 16 + 4 q + r} the results of the blocks I = 2 s and 2 s + 1 are an operand as they
-// stand: X goes from step to step in registers, and Q, being symmetric, is one as it comes out.  Only A = X X', which sums over
-// columns, reads X in its other orientation, from the wave's own part of LDS.  Two barriers per step, where A's parts are summed.
-// 8 x 512 and 29 x 512: bound by the latency of some 150 dependent instructions per step, not by a unit.
+// stand: X goes from step to step in registers, and Q, being symmetric, is one as it comes out (with RB = 1 the products over rows
+// are those of 16 k's, whose operand is a result as it stands, A too).  Only A = X X', which sums over columns, reads X in its other
+// orientation, from the wave's own part of LDS.  Two barriers per step, one with RB = 1, where A's parts are summed.
+// Bound by the instructions of one CU, some 450 per wave and step with RB = 2, JB = 4, and by the way in and out.
 struct small {
     source s;
-    int32_t m, n, steps, turned;
+    int32_t m, n, steps, turned, flat;          // flat: the rows of every array follow each other, they are read as one
     float a, b, c;
     void* out; const void* w; int out_type, w_type;
     int64_t out_b, out_r, w_b, w_r;
     float keep, gain;
 };
 
-template <int RB, int JB>
-__global__ __launch_bounds__(512) void k_orth_small(small p) {
-    constexpr int WAVES = 8, KB = JB / 2, S = RB / 2, TILES = RB * (RB + 1) / 2;
-    __shared__ __attribute__((aligned(16))) _Float16 xr[WAVES][RB][KB][FRAG];
-    __shared__ __attribute__((aligned(16))) float red[WAVES][TILES][256];
-    __shared__ __attribute__((aligned(16))) _Float16 am[RB][S][FRAG];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), q = lane >> 4, c = lane & 15;
+// The way in and out: fours of the caller's rows, and through LDS into the lanes that work on them.  There a row of the short side has
+// NP places, its columns swapped by row, so that neither order meets in one bank.
+template <int NP> struct cells {
+    float* at;
+    int turned, cols;             // the caller's
+    float per_col;
+    __device__ __forceinline__ cells(float* at_, const small& p) : at(at_), turned(p.turned), cols(p.turned ? p.m : p.n), per_col(1.0f / (p.turned ? p.m : p.n)) {}
+    __device__ __forceinline__ float& operator()(int i, int j) const { return at[i * NP + (j ^ (i & 31))]; }
+    template <typename F> __device__ __forceinline__ void four(bool flat, int r, int c, F&& f) const {          // f(k, cell) for c .. c + 3
+        if (flat) { r = (int)((c + 0.5f) * per_col); c -= r * cols; }          // (exact: fewer than 2^16 places)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            f(k, turned ? (*this)(c, r) : (*this)(r, c));
+            if (++c == cols && flat) { c = 0; ++r; }
+        }
+    }
+};
+
+template <int NP, int AT_ONCE>
+__device__ __forceinline__ double way_in(const small& p, const cells<NP>& cell, int rows_used) {
     const int64_t b = blockIdx.x;
-    // in the caller's order, four neighbours a thread, and through LDS (xr's, not needed yet) into the lanes that work on them;
-    // columns swapped by row, so that neither order meets in one bank
-    constexpr int NP = WAVES * JB * 16;
-    float* flat = (float*)&xr[0][0][0][0];
-    auto place = [&](int i, int j) -> float& { return flat[i * NP + (j ^ (i & 31))]; };
-    const int rows = p.turned ? p.n : p.m, cols = p.turned ? p.m : p.n, per = (cols + 3) / 4;
-    const bool padded = p.m < RB * 16 || p.n < NP;
-    if (padded) {
-        for (int e = threadIdx.x; e < RB * 16 * NP; e += 512) flat[e] = 0.0f;
+    const int rows = p.flat ? 1 : p.turned ? p.n : p.m, cols = p.flat ? p.m * p.n : p.turned ? p.m : p.n, per = (cols + 3) / 4;
+    if (p.m < rows_used || p.n < NP) {
+        for (int e = threadIdx.x; e < rows_used * NP / 4; e += 512) ((float4_*)cell.at)[e] = float4_{};
         __syncthreads();
     }
     double sum = 0.0;
-#pragma unroll 4
-    for (int e = threadIdx.x; e < rows * per; e += 512) {
-        const int r = e / per, col = (e - r * per) * 4, left = min(4, cols - col);
-        const float4_ u = moved(p.s, b, r, col, left, true);
-        for (int k = 0; k < 4; ++k) {
-            if (k < left) (p.turned ? place(col + k, r) : place(r, col + k)) = u[k];
-            sum += (double)u[k] * u[k];
+    for (int e = threadIdx.x; e < rows * per; e += AT_ONCE * 512) {
+        place at[AT_ONCE];
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            const int f = e + k * 512, r = p.flat ? 0 : f / per;
+            at[k].b = b; at[k].r = r; at[k].c = (f - r * per) * 4;
+            at[k].n = f < rows * per ? min(4, cols - (int)at[k].c) : 0;
+            at[k].load(p.s, true);
+        }
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            if (at[k].n <= 0) continue;
+            at[k].move(p.s, true);
+            cell.four(p.flat, (int)at[k].r, (int)at[k].c, [&](int t, float& to) {
+                if (t < at[k].n) to = at[k].u[t];
+                sum += (double)at[k].u[t] * at[k].u[t];
+            });
         }
     }
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    return sum;
+}
+
+template <int NP, int AT_ONCE>
+__device__ __forceinline__ void way_out(const small& p, const cells<NP>& cell) {
+    const int64_t b = blockIdx.x;
+    const int rows = p.flat ? 1 : p.turned ? p.n : p.m, cols = p.flat ? p.m * p.n : p.turned ? p.m : p.n, per = (cols + 3) / 4;
+    const float gain = p.gain / SCALE;
+    for (int e = threadIdx.x; e < rows * per; e += AT_ONCE * 512) {
+        float4_ w[AT_ONCE];
+        int row[AT_ONCE], col[AT_ONCE], left[AT_ONCE];
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            const int f = e + k * 512;
+            row[k] = p.flat ? 0 : f / per; col[k] = (f - row[k] * per) * 4;
+            left[k] = f < rows * per ? min(4, cols - col[k]) : 0;
+            w[k] = float4_{};
+            if (p.w) {
+                const int64_t at = b * p.w_b + row[k] * p.w_r + col[k];
+                if (left[k] >= 4) w[k] = load4(p.w, p.w_type, at);
+                else for (int t = 0; t < left[k]; ++t) w[k][t] = load_elem(p.w, p.w_type, at + t);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            if (left[k] <= 0) continue;
+            const int64_t at = b * p.out_b + row[k] * p.out_r + col[k];
+            float4_ v = {};
+            cell.four(p.flat, row[k], col[k], [&](int t, float& from) { if (t < left[k]) v[t] = from * gain; });
+            if (p.w) for (int t = 0; t < 4; ++t) v[t] = fmaf(p.keep, w[k][t], v[t]);
+            if (left[k] >= 4) store4(p.out, p.out_type, at, v);
+            else for (int t = 0; t < left[k]; ++t) store_elem(p.out, p.out_type, at + t, v[t]);
+        }
+    }
+}
+
+template <int RB, int JB>
+__global__ __launch_bounds__(512) void k_orth_small(small p) {
+    constexpr int WAVES = 8, NP = WAVES * JB * 16, KB = JB / 2, S = RB == 1 ? 1 : RB / 2, TILES = RB * (RB + 1) / 2;
+    __shared__ __attribute__((aligned(16))) _Float16 xr[WAVES][RB][KB][FRAG];
+    __shared__ __attribute__((aligned(16))) float red[RB == 1 ? 2 : 1][WAVES][TILES][256];          // (RB = 1: every other step the other one)
+    __shared__ __attribute__((aligned(16))) _Float16 am[RB == 1 ? 1 : RB][S][RB == 1 ? 8 : FRAG];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), q = lane >> 4, c = lane & 15;
+    const cells<NP> cell((float*)&xr[0][0][0][0], p);
+    double sum = way_in<NP, 8>(p, cell, RB * 16);
     double* sums = (double*)red;
     if (lane == 0) sums[wave] = sum;
     __syncthreads();
@@ -669,7 +740,7 @@ __global__ __launch_bounds__(512) void k_orth_small(small p) {
 #pragma unroll
         for (int I = 0; I < RB; ++I)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[jb][I][r] = (float)(place(16 * I + 4 * q + r, (wave * JB + jb) * 16 + c) * inv);
+            for (int r = 0; r < 4; ++r) x[jb][I][r] = (float)(cell(16 * I + 4 * q + r, (wave * JB + jb) * 16 + c) * inv);
     __syncthreads();
 
     for (int step = 0; step < p.steps; ++step) {
@@ -706,11 +777,42 @@ __global__ __launch_bounds__(512) void k_orth_small(small p) {
                 }
         }
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) *(float4_*)&red[wave][t][lane * 4] = acc[t];
+        for (int t = 0; t < TILES; ++t) *(float4_*)&red[RB == 1 ? step & 1 : 0][wave][t][lane * 4] = acc[t];
         __syncthreads();
+        if constexpr (RB == 1) {
+            float4_ a = {};
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) a += *(const float4_*)&red[step & 1][w][0][lane * 4];
+            half4 ah, al, qh, ql;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) { _Float16 h, l; split(a[r] * (1.0f / SCALE), h, l); ah[r] = h; al[r] = l; }
+            float4_ t = {};
+            t = __builtin_amdgcn_mfma_f32_16x16x16f16(ah, al, t, 0, 0, 0);
+            t = __builtin_amdgcn_mfma_f32_16x16x16f16(al, ah, t, 0, 0, 0);
+            t = __builtin_amdgcn_mfma_f32_16x16x16f16(ah, ah, t, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float v = fmaf(p.c, t[r] * (1.0f / SCALE), p.b * (a[r] * (1.0f / SCALE)));
+                if (4 * q + r == c) v += p.a * SCALE;
+                _Float16 h, l;
+                split(v, h, l);
+                qh[r] = h; ql[r] = l;
+            }
+#pragma unroll
+            for (int jb = 0; jb < JB; ++jb) {
+                const half4 h = __builtin_shufflevector(xh[jb][0], xh[jb][0], 0, 1, 2, 3), l = __builtin_shufflevector(xl[jb][0], xl[jb][0], 0, 1, 2, 3);
+                float4_ y = {};
+                y = __builtin_amdgcn_mfma_f32_16x16x16f16(qh, l, y, 0, 0, 0);
+                y = __builtin_amdgcn_mfma_f32_16x16x16f16(ql, h, y, 0, 0, 0);
+                y = __builtin_amdgcn_mfma_f32_16x16x16f16(qh, h, y, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[jb][0][r] = y[r] * (1.0f / SCALE);
+            }
+            continue;
+        } else {
         for (int t = wave; t < TILES; t += WAVES) {          // a wave sums a tile and writes it, and its mirror image, as operands
             float4_ v = {};
-            for (int w = 0; w < WAVES; ++w) v += *(const float4_*)&red[w][t][lane * 4];
+            for (int w = 0; w < WAVES; ++w) v += *(const float4_*)&red[0][w][t][lane * 4];
             int I = 0;
             while ((I + 1) * (I + 2) / 2 <= t) ++I;
             const int J = t - I * (I + 1) / 2;
@@ -770,6 +872,7 @@ __global__ __launch_bounds__(512) void k_orth_small(small p) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) x[jb][I][r] = t[r] * (1.0f / SCALE);
             }
+        }
     }
     __syncthreads();          // (the last reads of xr)
 #pragma unroll
@@ -777,25 +880,9 @@ __global__ __launch_bounds__(512) void k_orth_small(small p) {
 #pragma unroll
         for (int I = 0; I < RB; ++I)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) place(16 * I + 4 * q + r, (wave * JB + jb) * 16 + c) = x[jb][I][r];
+            for (int r = 0; r < 4; ++r) cell(16 * I + 4 * q + r, (wave * JB + jb) * 16 + c) = x[jb][I][r];
     __syncthreads();
-    const float gain = p.gain / SCALE;
-#pragma unroll 4
-    for (int e = threadIdx.x; e < rows * per; e += 512) {
-        const int r = e / per, col = (e - r * per) * 4, left = min(4, cols - col);
-        const int64_t at = b * p.out_b + r * p.out_r + col, wat = b * p.w_b + r * p.w_r + col;
-        float4_ v = {};
-        for (int k = 0; k < 4; ++k) if (k < left) v[k] = (p.turned ? place(col + k, r) : place(r, col + k)) * gain;
-        if (left >= 4) {
-            if (p.w) {
-                const float4_ w = load4(p.w, p.w_type, wat);
-                for (int k = 0; k < 4; ++k) v[k] = fmaf(p.keep, w[k], v[k]);
-            }
-            store4(p.out, p.out_type, at, v);
-        } else {
-            for (int k = 0; k < left; ++k) store_elem(p.out, p.out_type, at + k, p.w ? fmaf(p.keep, load_elem(p.w, p.w_type, wat + k), v[k]) : v[k]);
-        }
-    }
+    way_out<NP, 8>(p, cell);
 }
 
 }  // namespace dlo
