@@ -46,7 +46,7 @@ const char* memory_shape_error(const dl_memory_shape* s) {
 }
 
 // The form of a launch (dl_memory.hpp): V columns per lane, `blocks` waves across the columns, W waves of a workgroup along time.
-struct form { int V, W; bool parts; int64_t part, chunks, blocks; };
+struct form { int V, W; bool parts, chain; int64_t part, chunks, blocks; };
 
 // Columns per lane: eight bytes forward, four backward, where three arrays and the states of a run are held; fewer where the lanes
 // behind the last column of a row and of the last wave would be more than a seventh of all.
@@ -61,8 +61,10 @@ int widest_back(int dtype) { return dtype == DL_F32 ? 1 : 2; }
 
 // With a wave for every SIMD unit of the chip (1024) a wave runs through all of time.  Parts: 4096 waves; at least two runs each, and not
 // so many that the maps before a part (parts / 16 bytes for each of its columns, on average) weigh more than an eighth of its elements.
+constexpr int64_t CHAIN_MOST = 64;
+
 form memory_form(const dl_memory_shape* s, int V) {
-    form f{V, 1, false, s->T, 1, ceil_div(s->N * ceil_div(s->D, V), 64)};
+    form f{V, 1, false, false, s->T, 1, ceil_div(s->N * ceil_div(s->D, V), 64)};
     const int64_t runs = ceil_div(s->T, dlm::MARK);
     if (f.blocks >= 1024 || runs <= 1) return f;
     if (runs <= 8) {
@@ -70,6 +72,12 @@ form memory_form(const dl_memory_shape* s, int V) {
         return f;
     }
     f.W = dlm::PARTS;
+    if (runs <= dlm::PARTS * CHAIN_MOST) {
+        f.chain = true;
+        f.part = dlm::MARK;
+        f.chunks = ceil_div(runs, dlm::PARTS);
+        return f;
+    }
     f.parts = true;
     int64_t parts = ceil_div(4096, f.blocks);
     parts = std::min(parts, std::max<int64_t>(8, (int64_t)std::sqrt(4.0 * (double)s->T * elem_bytes(s->dtype))));
@@ -78,7 +86,21 @@ form memory_form(const dl_memory_shape* s, int V) {
     f.chunks = ceil_div(ceil_div(s->T, f.part), dlm::PARTS);
     return f;
 }
-int64_t maps_bytes(const dl_memory_shape* s, const form& f) { return f.parts ? f.chunks * (1 + dlm::PARTS) * 2 * s->N * s->D * 4 : 0; }
+// The form with the widest loads of its kernel; a chain's hold a whole run in registers, and wait: four bytes there, for twice the waves.
+form memory_plan(const dl_memory_shape* s, int most) {
+    form f = memory_form(s, memory_width(s, most));
+    const int narrow = s->dtype == DL_F32 ? 1 : 2;
+    return f.chain && f.V > narrow ? memory_form(s, memory_width(s, narrow)) : f;
+}
+// (a chain: its ticket, and a link of two floats per chunk and column)
+int64_t maps_bytes(const dl_memory_shape* s, const form& f) { return f.chain ? 64 + f.chunks * s->N * s->D * 8 : f.parts ? f.chunks * (1 + dlm::PARTS) * 2 * s->N * s->D * 4 : 0; }
+
+dlm::chain start_chain(const dl_memory_shape* s, const form& f, void* workspace, hipStream_t st) {
+    const dlm::chain ch{(uint32_t*)workspace, (uint64_t*)((char*)workspace + 64), (uint32_t)f.blocks};
+    const int64_t links = f.chunks * s->N * s->D;
+    dlm::k_memory_unlink<<<(unsigned)std::min<int64_t>(1024, ceil_div(links, 1024)), 256, 0, st>>>(ch, links);
+    return ch;
+}
 
 dlm::shape device_shape(const dl_memory_shape* s, const form& f) {
     return dlm::shape{s->N, s->D, s->x_t, s->x_n, s->gate_t, s->gate_n, s->starts_t, s->starts_n, s->grad_t, s->grad_n, (int32_t)s->T, (int32_t)f.part, (int32_t)f.chunks};
@@ -201,7 +223,7 @@ int64_t dl_memory_workspace_bytes(const dl_memory_shape* s) {
     if (const char* e = memory_shape_error(s)) return fail(DL_E_INVAL, e);
     if (s->T == 0 || s->N == 0 || s->D == 0) return 0;
     int64_t most = 0;
-    for (int V : {widest_forward(s->dtype), widest_back(s->dtype)}) most = std::max(most, maps_bytes(s, memory_form(s, memory_width(s, V))));
+    for (int V : {widest_forward(s->dtype), widest_back(s->dtype)}) most = std::max(most, maps_bytes(s, memory_plan(s, V)));
     return most;
 }
 
@@ -211,8 +233,9 @@ int dl_memory_forward(const dl_memory_shape* s, const void* x, const void* gate,
     if (s->T == 0) return fail(DL_E_INVAL, "dl_memory_forward: T = 0 (there is no step: the state stays as it is)");
     if (!x || !gate || !h) return fail(DL_E_INVAL, "dl_memory_forward: x, gate and h must not be NULL");
     if (state && state == state_out) return fail(DL_E_INVAL, "dl_memory_forward: state_out may not be state");
-    const form f = memory_form(s, memory_width(s, widest_forward(s->dtype)));
-    if (f.parts && !workspace) return fail(DL_E_INVAL, "dl_memory_forward: workspace must not be NULL (dl_memory_workspace_bytes)");
+    const form f = memory_plan(s, widest_forward(s->dtype));
+    if ((f.parts || f.chain) && !workspace) return fail(DL_E_INVAL, "dl_memory_forward: workspace must not be NULL (dl_memory_workspace_bytes)");
+    if (!aligned(workspace, 16)) return fail(DL_E_INVAL, "dl_memory_forward: workspace must be aligned to 16 bytes");
     if (f.blocks > 0x7fffffff) return fail(DL_E_INVAL, "dl_memory_forward: N * D too large");
     const dlm::shape d = device_shape(s, f);
     const dim3 grid((unsigned)f.blocks, (unsigned)f.chunks);
@@ -225,9 +248,12 @@ int dl_memory_forward(const dl_memory_shape* s, const void* x, const void* gate,
             dlm::k_memory_run<E, V, dlm::PARTS><<<grid, 64 * dlm::PARTS, 0, st>>>(d, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks, (const float*)workspace);
         } else if (f.W == 1) {
             dlm::k_memory_run<E, V, 1><<<grid, 64, 0, st>>>(d, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks, nullptr);
+        } else if (f.chain) {
+            const dlm::chain ch = start_chain(s, f, workspace, st);
+            dlm::k_memory_short<E, V, dlm::PARTS, true><<<(unsigned)(f.blocks * f.chunks), 64 * dlm::PARTS, 0, st>>>(d, ch, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks);
         } else with_waves(f.W, [&](auto w) {
             constexpr int W = decltype(w)::value;
-            dlm::k_memory_short<E, V, W><<<grid, 64 * W, 0, st>>>(d, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks);
+            dlm::k_memory_short<E, V, W, false><<<grid, 64 * W, 0, st>>>(d, dlm::chain{}, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks);
         });
     }); });
     return launched("dl_memory_forward");
@@ -240,8 +266,9 @@ int dl_memory_backward(const dl_memory_shape* s, const void* x, const void* gate
     if (s->T == 0) return fail(DL_E_INVAL, "dl_memory_backward: T = 0 (there is no step: the gradient of the state is grad_state)");
     if (!x || !gate || !marks || !dx || !dgate) return fail(DL_E_INVAL, "dl_memory_backward: x, gate, marks, dx and dgate must not be NULL");
     if (grad_state && grad_state == dstate) return fail(DL_E_INVAL, "dl_memory_backward: dstate may not be grad_state");
-    const form f = memory_form(s, memory_width(s, widest_back(s->dtype)));
-    if (f.parts && !workspace) return fail(DL_E_INVAL, "dl_memory_backward: workspace must not be NULL (dl_memory_workspace_bytes)");
+    const form f = memory_plan(s, widest_back(s->dtype));
+    if ((f.parts || f.chain) && !workspace) return fail(DL_E_INVAL, "dl_memory_backward: workspace must not be NULL (dl_memory_workspace_bytes)");
+    if (!aligned(workspace, 16)) return fail(DL_E_INVAL, "dl_memory_backward: workspace must be aligned to 16 bytes");
     if (f.blocks > 0x7fffffff) return fail(DL_E_INVAL, "dl_memory_backward: N * D too large");
     const dlm::shape d = device_shape(s, f);
     const dim3 grid((unsigned)f.blocks, (unsigned)f.chunks);
@@ -254,9 +281,12 @@ int dl_memory_backward(const dl_memory_shape* s, const void* x, const void* gate
             dlm::k_memory_run_back<E, V, dlm::PARTS><<<grid, 64 * dlm::PARTS, 0, st>>>(d, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, grad_state, (E*)dx, (E*)dgate, dstate, (const float*)workspace);
         } else if (f.W == 1) {
             dlm::k_memory_run_back<E, V, 1><<<grid, 64, 0, st>>>(d, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, grad_state, (E*)dx, (E*)dgate, dstate, nullptr);
+        } else if (f.chain) {
+            const dlm::chain ch = start_chain(s, f, workspace, st);
+            dlm::k_memory_short_back<E, V, dlm::PARTS, true><<<(unsigned)(f.blocks * f.chunks), 64 * dlm::PARTS, 0, st>>>(d, ch, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, grad_state, (E*)dx, (E*)dgate, dstate);
         } else with_waves(f.W, [&](auto w) {
             constexpr int W = decltype(w)::value;
-            dlm::k_memory_short_back<E, V, W><<<grid, 64 * W, 0, st>>>(d, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, grad_state, (E*)dx, (E*)dgate, dstate);
+            dlm::k_memory_short_back<E, V, W, false><<<grid, 64 * W, 0, st>>>(d, dlm::chain{}, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, grad_state, (E*)dx, (E*)dgate, dstate);
         });
     }); });
     return launched("dl_memory_backward");

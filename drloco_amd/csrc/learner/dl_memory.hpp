@@ -5,11 +5,13 @@
 //
 // Bound by memory (three elements moved per step forward, five backward) with the arithmetic, 20 to 40 operations per element, close
 // behind.  A wave takes 64 x V columns through time, MARK steps (a run) in registers and the loads of the next ones under way.
-// Three forms, by the number of such waves ("blocks") and of steps:
+// Four forms, by the number of such waves ("blocks") and of steps:
 //   whole   enough blocks for the chip: a wave runs through all of time, every element is loaded once;
 //   short   few blocks, at most eight runs: the waves of a workgroup take a run each, reduce it to its affine map, exchange the maps
 //           through LDS and finish their steps from the registers: every element is loaded once here too;
-//   parts   few blocks, many steps: the time axis is cut into parts.  A first kernel reduces every part to its map (two of three
+//   chain   the same with a row of workgroups along time, eight runs each: a workgroup leaves its map in memory as soon as it has it and
+//           picks up those before it while its own elements wait in registers: once again every element is loaded once;
+//   parts   few blocks, still more steps: the time axis is cut into parts.  A first kernel reduces every part to its map (two of three
 //           elements are read, in the backward direction two of five), the second starts each part from the maps before it.
 //
 // Rounding.  The smaller of a and s is computed as e / (1 + e), e = exp(-|g|), and both products go through it:
@@ -95,9 +97,9 @@ template <int V> struct columns {
     int64_t n0;
     uint32_t dn, d;               // walkers after n0, channel
     bool valid, few;              // few: the wave spans at most four walkers
-    __device__ columns(int64_t N, int64_t D) {
+    __device__ columns(int64_t N, int64_t D, uint32_t block = blockIdx.x) {
         const int64_t per = (D + V - 1) / V;
-        const int64_t q0 = (int64_t)blockIdx.x * 64, q = q0 + (threadIdx.x & 63);
+        const int64_t q0 = (int64_t)block * 64, q = q0 + (threadIdx.x & 63);
         n0 = uniform(q0 / per);
         valid = q < N * per;
         dn = valid ? (uint32_t)(q / per - n0) : 0;
@@ -403,21 +405,104 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 4) void k_memory_run(shape s, 
     if (state_out && c.valid && last == s.T) store_floats<V>(state_out + corner, floats, now);
 }
 
+// ---- chain: the maps of workgroups on their way to later ones ---------------------------------------------------------------------------
+// A link is a map (m, b) in one 64-bit word, written and read whole, so that there is nothing to order; EMPTY (no map has that m)
+// until it is written.  Workgroups take their place in the chain by a ticket, in the order in which they start: those a workgroup waits
+// for have started before it and write their links without waiting for anyone, so every wait ends.  All links before a chunk are
+// joined in the same order however late they come: results do not depend on timing.
+constexpr uint32_t EMPTY = 0xffffffffu;
+struct chain { uint32_t* ticket; uint64_t* links; uint32_t blocks; };          // links: [chunks][N * D]
+
+__global__ __launch_bounds__(256) void k_memory_unlink(chain ch, int64_t links) {
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < links; e += (int64_t)gridDim.x * 256) ch.links[e] = ~0ull;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *ch.ticket = 0;
+}
+
+template <int V> __device__ __forceinline__ void link(uint64_t* at, const float (&m)[V], const float (&b)[V]) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        const uint32_t lo = m[v] != m[v] ? 0x7fc00000u : __float_as_uint(m[v]);
+        __hip_atomic_store(at + v, (uint64_t)__float_as_uint(b[v]) << 32 | lo, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+}
+// m, b: joined with the links of the chunks first, first + way, .. (`count` of them)
+template <int V> __device__ __forceinline__ void follow(const uint64_t* links, int64_t plane, int first, int way, int count, float (&m)[V], float (&b)[V]) {
+    constexpr int AT_ONCE = 4;
+    for (int i = 0; i < count; i += AT_ONCE) {
+        uint64_t l[AT_ONCE][V];
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k)
+#pragma unroll
+            for (int v = 0; v < V; ++v) l[k][v] = __hip_atomic_load(links + (int64_t)(first + way * min(i + k, count - 1)) * plane + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            if (i + k >= count) break;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                while ((uint32_t)l[k][v] == EMPTY) {
+                    __builtin_amdgcn_s_sleep(1);
+                    l[k][v] = __hip_atomic_load(links + (int64_t)(first + way * (i + k)) * plane + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+                const float n = __uint_as_float((uint32_t)l[k][v]), c = __uint_as_float((uint32_t)(l[k][v] >> 32));
+                b[v] = apply(n, c, b[v]);
+                m[v] = after(m[v], n);
+            }
+        }
+    }
+}
+// The workgroup's place, and then: its link (from its waves' maps la, lb) and the value that enters it (carry: the one that enters the chain).
+__device__ __forceinline__ uint32_t take_ticket(const chain& ch) {
+    __shared__ uint32_t mine;
+    if (threadIdx.x == 0) mine = __hip_atomic_fetch_add(ch.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane((int)mine);
+}
+template <int V, bool BACK>
+__device__ __forceinline__ void pass_on(const chain& ch, int k, int chunks, int64_t plane, int64_t col, bool valid, int wave, int lane, const float (*la)[64 * V], const float (*lb)[64 * V],
+                                        float (*lc)[64 * V], float (*ld)[64 * V], float (&carry)[V]) {
+    float m[V], b[V], zero[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) m[v] = b[v] = zero[v] = 0.0f;
+    if (wave == 0 && (BACK ? k > 0 : k + 1 < chunks)) {          // (nobody waits for the last one's)
+        float mine[V], next[V];
+        join<V, BACK>(la, lb, lane, PARTS, 0, zero, mine, next);
+        for (int w = 0; w < PARTS; ++w) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) m[v] = after(m[v], la[w][v * 64 + lane]);
+        }
+        if (valid) link<V>(ch.links + (int64_t)k * plane + col, m, next);
+    }
+    const int before = BACK ? chunks - 1 - k : k;
+    if (before == 0) return;
+#pragma unroll
+    for (int v = 0; v < V; ++v) m[v] = b[v] = 0.0f;
+    const int lo = before * wave / PARTS, hi = before * (wave + 1) / PARTS;
+    follow<V>(ch.links + col, plane, BACK ? chunks - 1 - lo : lo, BACK ? -1 : 1, hi - lo, m, b);
+#pragma unroll
+    for (int v = 0; v < V; ++v) { lc[wave][v * 64 + lane] = m[v]; ld[wave][v * 64 + lane] = b[v]; }
+    __syncthreads();
+    float mine[V], next[V];
+    join<V, false>(lc, ld, lane, PARTS, 0, carry, mine, next);
+#pragma unroll
+    for (int v = 0; v < V; ++v) carry[v] = next[v];
+}
+
 // ---- short: W waves of a workgroup take one run each ----------------------------------------------------------------------------------
-template <typename E, int V, int W>
-__global__ __launch_bounds__(64 * W) void k_memory_short(shape s, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ state,
+template <typename E, int V, int W, bool CHAIN>
+__global__ __launch_bounds__(64 * W) void k_memory_short(shape s, chain ch, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ state,
                                                          E* __restrict__ h, float* __restrict__ state_out, float* __restrict__ marks) {
     typedef vec_t<E, V> vec;
     __shared__ float la[W][64 * V], lb[W][64 * V];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const columns<V> c(s.N, s.D);
+    const uint32_t place = CHAIN ? take_ticket(ch) : blockIdx.x, k = CHAIN ? place / ch.blocks : 0;
+    const columns<V> c(s.N, s.D, CHAIN ? place - k * ch.blocks : place);
     const int64_t plane = s.N * s.D, corner = c.n0 * s.D;
     const uint32_t elems = c.template bytes<E>(s.D), floats = c.template bytes<float>(s.D);
     float carry[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) carry[v] = 0.0f;
     if (state) load_floats<V>(carry, state + corner, floats);
-    const int t0 = wave * MARK, len = max(0, min(MARK, s.T - t0));
+    const int t0 = ((int)k * W + wave) * MARK, len = max(0, min(MARK, s.T - t0));
     rows<E, V, MARK, true, false> r;
     r.load(s, c, t0, s.T, x, gate, nullptr, starts);
     float m[MARK][V];
@@ -439,9 +524,13 @@ __global__ __launch_bounds__(64 * W) void k_memory_short(shape s, const E* __res
     for (int v = 0; v < V; ++v) { la[wave][v * 64 + lane] = A[v].held(begin != 0); lb[wave][v * 64 + lane] = B[v]; }
     forget<V>(m, begin); r.forget();
     __syncthreads();
+    if constexpr (CHAIN) {
+        __shared__ float lc[W][64 * V], ld[W][64 * V];
+        pass_on<V, false>(ch, (int)k, s.chunks, plane, corner + floats / 4, c.valid, wave, lane, la, lb, lc, ld, carry);
+    }
     float in[V], next[V];
     join<V, false>(la, lb, lane, W, wave, carry, in, next);
-    if (marks && c.valid && len > 0) store_floats<V>(marks + (int64_t)wave * plane + corner, floats, in);
+    if (marks && c.valid && len > 0) store_floats<V>(marks + (int64_t)(t0 / MARK) * plane + corner, floats, in);
     E* ph = h + (int64_t)t0 * plane + corner;
 #pragma unroll
     for (int t = 0; t < MARK; ++t) {
@@ -456,7 +545,7 @@ __global__ __launch_bounds__(64 * W) void k_memory_short(shape s, const E* __res
             ph += plane;
         }
     }
-    if (state_out && wave == 0 && c.valid) store_floats<V>(state_out + corner, floats, next);
+    if (state_out && wave == 0 && c.valid && (!CHAIN || (int)k + 1 == s.chunks)) store_floats<V>(state_out + corner, floats, next);
 }
 
 // ---- gradients of a run.  hs: the states before each step, recomputed from the saved one --------------------------------------------------
@@ -549,19 +638,21 @@ __global__ __launch_bounds__(64 * W) void k_memory_run_back(shape s, const E* __
     if (dstate && c.valid && first == 0) store_floats<V>(dstate + corner, floats, in);
 }
 
-template <typename E, int V, int W>
-__global__ __launch_bounds__(64 * W) void k_memory_short_back(shape s, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ marks,
+template <typename E, int V, int W, bool CHAIN>
+__global__ __launch_bounds__(64 * W) void k_memory_short_back(shape s, chain ch, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ marks,
                                                               const E* __restrict__ grad_h, const float* __restrict__ grad_state, E* __restrict__ dx, E* __restrict__ dgate, float* __restrict__ dstate) {
     __shared__ float la[W][64 * V], lb[W][64 * V];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const columns<V> c(s.N, s.D);
+    const uint32_t place = CHAIN ? take_ticket(ch) : blockIdx.x, back = CHAIN ? place / ch.blocks : 0;
+    const columns<V> c(s.N, s.D, CHAIN ? place - back * ch.blocks : place);
+    const int k = CHAIN ? s.chunks - 1 - (int)back : 0;
     const int64_t plane = s.N * s.D, corner = c.n0 * s.D;
     const uint32_t elems = c.template bytes<E>(s.D), floats = c.template bytes<float>(s.D);
     float carry[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) carry[v] = 0.0f;
     if (grad_state) load_floats<V>(carry, grad_state + corner, floats);
-    const int t0 = wave * MARK, len = max(0, min(MARK, s.T - t0));
+    const int t0 = (k * W + wave) * MARK, len = max(0, min(MARK, s.T - t0));
     run_back<E, V> b;
     b.load(s, c, t0, s.T, x, gate, grad_h, starts, marks, plane, corner, floats);
     float m[MARK][V], hs[MARK][V];
@@ -582,10 +673,14 @@ __global__ __launch_bounds__(64 * W) void k_memory_short_back(shape s, const E* 
     for (int v = 0; v < V; ++v) { la[wave][v * 64 + lane] = A[v].held(begin != 0); lb[wave][v * 64 + lane] = B[v]; }
     forget<V>(m, begin); b.r.forget();
     __syncthreads();
+    if constexpr (CHAIN) {
+        __shared__ float lc[W][64 * V], ld[W][64 * V];
+        pass_on<V, true>(ch, k, s.chunks, plane, corner + floats / 4, c.valid, wave, lane, la, lb, lc, ld, carry);
+    }
     float in[V], next[V];
     join<V, true>(la, lb, lane, W, W - 1 - wave, carry, in, next);
     if (len > 0) b.finish(c, t0, len, begin, m, hs, in, dx, dgate, plane, corner, elems);
-    if (dstate && wave == 0 && c.valid) store_floats<V>(dstate + corner, floats, next);
+    if (dstate && wave == 0 && c.valid && k == 0) store_floats<V>(dstate + corner, floats, next);
 }
 
 // One control step.  state_out may be state: a thread reads its own columns, which are no other's, before it writes them.

@@ -61,7 +61,8 @@ typedef struct dl_memory_shape {
  * [ceil(T / DL_MEMORY_MARK), N, D]; dl_memory_backward recomputes the steps between from x and gate in 32 bits. */
 #define DL_MEMORY_MARK 16
 
-/* Bytes of device workspace dl_memory_forward / dl_memory_backward need for this shape (0 is possible), or a DL_E_ code. */
+/* Bytes of device workspace dl_memory_forward / dl_memory_backward need for this shape (0 is possible), or a DL_E_ code.  Aligned to 16 bytes;
+ * what it holds before a call does not matter. */
 int64_t dl_memory_workspace_bytes(const dl_memory_shape* shape);
 
 /* h: [T, N, D]; state_out: float [N, D] = h[T-1] before rounding (may be NULL; may not overlap state); marks may be NULL. */

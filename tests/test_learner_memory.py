@@ -107,7 +107,7 @@ def test_empty_shapes_are_done_at_once(L):
 def test_the_workspace_stays_small(L, T, N, D):
     size = L.dl_memory_workspace_bytes(C.byref(shape(T, N, D, x_t=N * D, gate_t=N * D)))
     # a map (two floats) per part of at least 32 steps, and one per eight parts
-    assert 0 <= size <= 72 * N * D * (T // 256 + 2)
+    assert 0 <= size <= 72 * N * D * (T // 256 + 2) + 64
 
 
 t3 = lambda *s, dtype=torch.float32: torch.zeros(*s, dtype=dtype)
