@@ -2,7 +2,6 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <algorithm>
-#include <cmath>
 #include <string>
 
 #include "drloco_learner.h"
@@ -45,8 +44,9 @@ const char* memory_shape_error(const dl_memory_shape* s) {
     return nullptr;
 }
 
-// The form of a launch (dl_memory.hpp): V columns per lane, `blocks` waves across the columns, W waves of a workgroup along time.
-struct form { int V, W; bool parts, chain; int64_t part, chunks, blocks; };
+// The form of a launch (dl_memory.hpp): V columns per lane, `blocks` waves across the columns, W waves of a workgroup along time and
+// `chunks` such workgroups in a chain.
+struct form { int V, W; int64_t chunks, blocks; };
 
 // Columns per lane: eight bytes forward, four backward, where three arrays and the states of a run are held; fewer where the lanes
 // behind the last column of a row and of the last wave would be more than a seventh of all.
@@ -59,51 +59,35 @@ int memory_width(const dl_memory_shape* s, int most) {
 int widest_forward(int dtype) { return dtype == DL_F32 ? 2 : 4; }
 int widest_back(int dtype) { return dtype == DL_F32 ? 1 : 2; }
 
-// With a wave for every SIMD unit of the chip (1024) a wave runs through all of time.  Parts: 4096 waves; at least two runs each, and not
-// so many that the maps before a part (parts / 16 bytes for each of its columns, on average) weigh more than an eighth of its elements.
-constexpr int64_t CHAIN_MOST = 64;
-
+// With a wave for every SIMD unit of the chip (1024) a wave runs through all of time.
 form memory_form(const dl_memory_shape* s, int V) {
-    form f{V, 1, false, false, s->T, 1, ceil_div(s->N * ceil_div(s->D, V), 64)};
+    form f{V, 1, 1, ceil_div(s->N * ceil_div(s->D, V), 64)};
     const int64_t runs = ceil_div(s->T, dlm::MARK);
-    if (f.blocks >= 1024 || runs <= 1) return f;
-    if (runs <= 8) {
-        while (f.W < runs) f.W *= 2;
-        return f;
-    }
-    f.W = dlm::PARTS;
-    if (runs <= dlm::PARTS * CHAIN_MOST) {
-        f.chain = true;
-        f.part = dlm::MARK;
-        f.chunks = ceil_div(runs, dlm::PARTS);
-        return f;
-    }
-    f.parts = true;
-    int64_t parts = ceil_div(4096, f.blocks);
-    parts = std::min(parts, std::max<int64_t>(8, (int64_t)std::sqrt(4.0 * (double)s->T * elem_bytes(s->dtype))));
-    parts = std::max<int64_t>(1, std::min(parts, runs));
-    f.part = ceil_div(runs, parts) * dlm::MARK;
-    f.chunks = ceil_div(ceil_div(s->T, f.part), dlm::PARTS);
+    if (f.blocks >= 1024) return f;
+    while (f.W < runs && f.W < dlm::WAVES) f.W *= 2;
+    f.chunks = ceil_div(runs, f.W);
     return f;
 }
 // The form with the widest loads of its kernel; a chain's hold a whole run in registers, and wait: four bytes there, for twice the waves.
 form memory_plan(const dl_memory_shape* s, int most) {
     form f = memory_form(s, memory_width(s, most));
-    const int narrow = s->dtype == DL_F32 ? 1 : 2;
-    return f.chain && f.V > narrow ? memory_form(s, memory_width(s, narrow)) : f;
+    const int narrow = 4 / elem_bytes(s->dtype);
+    return f.chunks > 1 && f.V > narrow ? memory_form(s, memory_width(s, narrow)) : f;
 }
-// (a chain: its ticket, and a link of two floats per chunk and column)
-int64_t maps_bytes(const dl_memory_shape* s, const form& f) { return f.chain ? 64 + f.chunks * s->N * s->D * 8 : f.parts ? f.chunks * (1 + dlm::PARTS) * 2 * s->N * s->D * 4 : 0; }
+// A chain: its ticket, a link of two floats per chunk and column, a value per group of chunks.
+int64_t chain_words(const dl_memory_shape* s, const form& f) { return (f.chunks + ceil_div(f.chunks, dlm::GROUP)) * s->N * s->D; }
+int64_t chain_bytes(const dl_memory_shape* s, const form& f) { return f.chunks > 1 ? 64 + chain_words(s, f) * 8 : 0; }
 
 dlm::chain start_chain(const dl_memory_shape* s, const form& f, void* workspace, hipStream_t st) {
-    const dlm::chain ch{(uint32_t*)workspace, (uint64_t*)((char*)workspace + 64), (uint32_t)f.blocks};
-    const int64_t links = f.chunks * s->N * s->D;
-    dlm::k_memory_unlink<<<(unsigned)std::min<int64_t>(1024, ceil_div(links, 1024)), 256, 0, st>>>(ch, links);
+    uint64_t* links = (uint64_t*)((char*)workspace + 64);
+    const dlm::chain ch{(uint32_t*)workspace, links, links + f.chunks * s->N * s->D, (uint32_t)f.blocks};
+    const int64_t words = chain_words(s, f);
+    dlm::k_memory_unlink<<<(unsigned)std::min<int64_t>(1024, ceil_div(words, 1024)), 256, 0, st>>>(ch, words);
     return ch;
 }
 
 dlm::shape device_shape(const dl_memory_shape* s, const form& f) {
-    return dlm::shape{s->N, s->D, s->x_t, s->x_n, s->gate_t, s->gate_n, s->starts_t, s->starts_n, s->grad_t, s->grad_n, (int32_t)s->T, (int32_t)f.part, (int32_t)f.chunks};
+    return dlm::shape{s->N, s->D, s->x_t, s->x_n, s->gate_t, s->gate_n, s->starts_t, s->starts_n, s->grad_t, s->grad_n, (int32_t)s->T, (int32_t)f.chunks};
 }
 
 template <int N> struct Int { static constexpr int value = N; };
@@ -223,7 +207,7 @@ int64_t dl_memory_workspace_bytes(const dl_memory_shape* s) {
     if (const char* e = memory_shape_error(s)) return fail(DL_E_INVAL, e);
     if (s->T == 0 || s->N == 0 || s->D == 0) return 0;
     int64_t most = 0;
-    for (int V : {widest_forward(s->dtype), widest_back(s->dtype)}) most = std::max(most, maps_bytes(s, memory_plan(s, V)));
+    for (int V : {widest_forward(s->dtype), widest_back(s->dtype)}) most = std::max(most, chain_bytes(s, memory_plan(s, V)));
     return most;
 }
 
@@ -234,23 +218,22 @@ int dl_memory_forward(const dl_memory_shape* s, const void* x, const void* gate,
     if (!x || !gate || !h) return fail(DL_E_INVAL, "dl_memory_forward: x, gate and h must not be NULL");
     if (state && state == state_out) return fail(DL_E_INVAL, "dl_memory_forward: state_out may not be state");
     const form f = memory_plan(s, widest_forward(s->dtype));
-    if ((f.parts || f.chain) && !workspace) return fail(DL_E_INVAL, "dl_memory_forward: workspace must not be NULL (dl_memory_workspace_bytes)");
+    if (f.chunks > 1 && !workspace) return fail(DL_E_INVAL, "dl_memory_forward: workspace must not be NULL (dl_memory_workspace_bytes)");
     if (!aligned(workspace, 16)) return fail(DL_E_INVAL, "dl_memory_forward: workspace must be aligned to 16 bytes");
-    if (f.blocks > 0x7fffffff) return fail(DL_E_INVAL, "dl_memory_forward: N * D too large");
+    if (f.blocks * f.chunks > 0x7fffffff) return fail(DL_E_INVAL, "dl_memory_forward: T * N * D too large");
     const dlm::shape d = device_shape(s, f);
-    const dim3 grid((unsigned)f.blocks, (unsigned)f.chunks);
+    const unsigned grid = (unsigned)(f.blocks * f.chunks);
     hipStream_t st = (hipStream_t)stream;
     with_type(s->dtype, [&](auto e) { with_width<widest<decltype(e)>()>(f.V, [&](auto v) {
         using E = decltype(e);
         constexpr int V = decltype(v)::value;
-        if (f.parts) {
-            dlm::k_memory_maps<E, V, false><<<grid, 64 * dlm::PARTS, 0, st>>>(d, (const E*)x, (const E*)gate, nullptr, starts, (float*)workspace);
-            dlm::k_memory_run<E, V, dlm::PARTS><<<grid, 64 * dlm::PARTS, 0, st>>>(d, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks, (const float*)workspace);
-        } else if (f.W == 1) {
-            dlm::k_memory_run<E, V, 1><<<grid, 64, 0, st>>>(d, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks, nullptr);
-        } else if (f.chain) {
-            const dlm::chain ch = start_chain(s, f, workspace, st);
-            dlm::k_memory_short<E, V, dlm::PARTS, true><<<(unsigned)(f.blocks * f.chunks), 64 * dlm::PARTS, 0, st>>>(d, ch, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks);
+        if (f.W == 1) {
+            dlm::k_memory_run<E, V><<<grid, 64, 0, st>>>(d, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks);
+        } else if (f.chunks > 1) {
+            if constexpr (V * sizeof(E) <= 4) {
+                const dlm::chain ch = start_chain(s, f, workspace, st);
+                dlm::k_memory_short<E, V, dlm::WAVES, true><<<grid, 64 * dlm::WAVES, 0, st>>>(d, ch, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks);
+            }
         } else with_waves(f.W, [&](auto w) {
             constexpr int W = decltype(w)::value;
             dlm::k_memory_short<E, V, W, false><<<grid, 64 * W, 0, st>>>(d, dlm::chain{}, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks);
@@ -267,23 +250,20 @@ int dl_memory_backward(const dl_memory_shape* s, const void* x, const void* gate
     if (!x || !gate || !marks || !dx || !dgate) return fail(DL_E_INVAL, "dl_memory_backward: x, gate, marks, dx and dgate must not be NULL");
     if (grad_state && grad_state == dstate) return fail(DL_E_INVAL, "dl_memory_backward: dstate may not be grad_state");
     const form f = memory_plan(s, widest_back(s->dtype));
-    if ((f.parts || f.chain) && !workspace) return fail(DL_E_INVAL, "dl_memory_backward: workspace must not be NULL (dl_memory_workspace_bytes)");
+    if (f.chunks > 1 && !workspace) return fail(DL_E_INVAL, "dl_memory_backward: workspace must not be NULL (dl_memory_workspace_bytes)");
     if (!aligned(workspace, 16)) return fail(DL_E_INVAL, "dl_memory_backward: workspace must be aligned to 16 bytes");
-    if (f.blocks > 0x7fffffff) return fail(DL_E_INVAL, "dl_memory_backward: N * D too large");
+    if (f.blocks * f.chunks > 0x7fffffff) return fail(DL_E_INVAL, "dl_memory_backward: T * N * D too large");
     const dlm::shape d = device_shape(s, f);
-    const dim3 grid((unsigned)f.blocks, (unsigned)f.chunks);
+    const unsigned grid = (unsigned)(f.blocks * f.chunks);
     hipStream_t st = (hipStream_t)stream;
     with_type(s->dtype, [&](auto e) { with_width<widest<decltype(e)>() / 2>(f.V, [&](auto v) {
         using E = decltype(e);
         constexpr int V = decltype(v)::value;
-        if (f.parts) {
-            dlm::k_memory_maps<E, V, true><<<grid, 64 * dlm::PARTS, 0, st>>>(d, (const E*)x, (const E*)gate, (const E*)grad_h, starts, (float*)workspace);
-            dlm::k_memory_run_back<E, V, dlm::PARTS><<<grid, 64 * dlm::PARTS, 0, st>>>(d, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, grad_state, (E*)dx, (E*)dgate, dstate, (const float*)workspace);
-        } else if (f.W == 1) {
-            dlm::k_memory_run_back<E, V, 1><<<grid, 64, 0, st>>>(d, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, grad_state, (E*)dx, (E*)dgate, dstate, nullptr);
-        } else if (f.chain) {
+        if (f.W == 1) {
+            dlm::k_memory_run_back<E, V><<<grid, 64, 0, st>>>(d, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, grad_state, (E*)dx, (E*)dgate, dstate);
+        } else if (f.chunks > 1) {
             const dlm::chain ch = start_chain(s, f, workspace, st);
-            dlm::k_memory_short_back<E, V, dlm::PARTS, true><<<(unsigned)(f.blocks * f.chunks), 64 * dlm::PARTS, 0, st>>>(d, ch, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, grad_state, (E*)dx, (E*)dgate, dstate);
+            dlm::k_memory_short_back<E, V, dlm::WAVES, true><<<grid, 64 * dlm::WAVES, 0, st>>>(d, ch, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, grad_state, (E*)dx, (E*)dgate, dstate);
         } else with_waves(f.W, [&](auto w) {
             constexpr int W = decltype(w)::value;
             dlm::k_memory_short_back<E, V, W, false><<<grid, 64 * W, 0, st>>>(d, dlm::chain{}, (const E*)x, (const E*)gate, starts, marks, (const E*)grad_h, grad_state, (E*)dx, (E*)dgate, dstate);

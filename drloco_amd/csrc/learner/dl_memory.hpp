@@ -5,14 +5,12 @@
 //
 // Bound by memory (three elements moved per step forward, five backward) with the arithmetic, 20 to 40 operations per element, close
 // behind.  A wave takes 64 x V columns through time, MARK steps (a run) in registers and the loads of the next ones under way.
-// Four forms, by the number of such waves ("blocks") and of steps:
+// Three forms, by the number of such waves ("blocks") and of steps:
 //   whole   enough blocks for the chip: a wave runs through all of time, every element is loaded once;
 //   short   few blocks, at most eight runs: the waves of a workgroup take a run each, reduce it to its affine map, exchange the maps
 //           through LDS and finish their steps from the registers: every element is loaded once here too;
-//   chain   the same with a row of workgroups along time, eight runs each: a workgroup leaves its map in memory as soon as it has it and
-//           picks up those before it while its own elements wait in registers: once again every element is loaded once;
-//   parts   few blocks, still more steps: the time axis is cut into parts.  A first kernel reduces every part to its map (two of three
-//           elements are read, in the backward direction two of five), the second starts each part from the maps before it.
+//   chain   few blocks, more runs: a row of such workgroups along time.  Each leaves its map in memory as soon as it has it and picks
+//           up those before it while its own elements wait in registers: once again every element is loaded once.
 //
 // Rounding.  The smaller of a and s is computed as e / (1 + e), e = exp(-|g|), and both products go through it:
 //     g >= 0:  h = h' + s (x - h'),  c = l - s l        g < 0:  h = x + a (h' - x),  c = a l
@@ -28,7 +26,7 @@
 namespace dlm {
 
 constexpr int MARK = 16;          // steps of a wave's run, and between two saved states
-constexpr int PARTS = 8;          // waves of a workgroup that shares the time axis
+constexpr int WAVES = 8;          // waves of a chain's workgroup, a run each
 
 template <typename E, int V> struct vec { typedef E type __attribute__((ext_vector_type(V), aligned(sizeof(E)))); };
 template <typename E> struct vec<E, 1> { typedef E type; };
@@ -46,8 +44,7 @@ template <typename E, int V> __device__ __forceinline__ void put(vec_t<E, V>& v,
 struct shape {
     int64_t N, D;
     int64_t x_t, x_n, gate_t, gate_n, starts_t, starts_n, grad_t, grad_n;
-    int32_t T;
-    int32_t part, chunks;         // steps of a part (a multiple of MARK), workgroups of PARTS parts along time
+    int32_t T, chunks;            // steps; workgroups along time
 };
 
 // min(a, s) with the sign of the gate.
@@ -149,48 +146,6 @@ template <int V> __device__ __forceinline__ void store_floats(float* base, uint3
     store_at<vec_t<float, V>>(base, bytes, f);
 }
 
-// Maps in memory: float [chunks][2][N * D] of the chunks, behind them [chunks * PARTS][2][N * D] of the parts; `maps` is at channel 0 of
-// the first walker.  The value that enters a wave's part: the workgroup joins the chunks before, a share per wave, and then
-// each wave the parts before its own.
-template <int V, bool BACK>
-__device__ __forceinline__ void enter(const float* maps, int64_t plane, int k, int chunks, uint32_t floats, int wave, int lane, float (*la)[64 * V], float (*lb)[64 * V], float (&carry)[V]) {
-    const int before = BACK ? chunks - 1 - k : k;
-    if (before > 0) {
-        float A[V], B[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) { A[v] = 0.0f; B[v] = 0.0f; }
-        const int lo = before * wave / PARTS, hi = before * (wave + 1) / PARTS;
-#pragma unroll 4
-        for (int i = lo; i < hi; ++i) {
-            const float* p = maps + (int64_t)(BACK ? chunks - 1 - i : i) * 2 * plane;
-            float a[V], b[V];
-            load_floats<V>(a, p, floats);
-            load_floats<V>(b, p + plane, floats);
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                B[v] = apply(a[v], b[v], B[v]);
-                A[v] = after(A[v], a[v]);
-            }
-        }
-#pragma unroll
-        for (int v = 0; v < V; ++v) { la[wave][v * 64 + lane] = A[v]; lb[wave][v * 64 + lane] = B[v]; }
-        __syncthreads();
-        float mine[V], next[V];
-        join<V, false>(la, lb, lane, PARTS, 0, carry, mine, next);
-#pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = next[v];
-    }
-    const float* parts = maps + ((int64_t)chunks + (int64_t)k * PARTS) * 2 * plane;
-    for (int i = 0; i < (BACK ? PARTS - 1 - wave : wave); ++i) {
-        const float* p = parts + (int64_t)(BACK ? PARTS - 1 - i : i) * 2 * plane;
-        float a[V], b[V];
-        load_floats<V>(a, p, floats);
-        load_floats<V>(b, p + plane, floats);
-#pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = apply(a[v], b[v], carry[v]);
-    }
-}
-
 // Between the passes over a run: the comparisons of the first are made again instead of being kept, a pair of scalar registers each.
 template <int V> __device__ __forceinline__ void forget(float (&m)[MARK][V], uint32_t& begin) {
 #pragma unroll
@@ -270,88 +225,10 @@ template <typename E, int V, int R, bool X, bool G> struct rows {
 struct yes { static constexpr bool value = true; };
 struct no { static constexpr bool value = false; };
 
-// ---- parts: every part and every chunk of PARTS of them to its map ---------------------------------------------------------------
-template <typename E, int V, bool BACK>
-__global__ __launch_bounds__(64 * PARTS, 4) void k_memory_maps(shape s, const E* __restrict__ x, const E* __restrict__ gate, const E* __restrict__ grad_h, const uint8_t* __restrict__ starts, float* __restrict__ maps) {
-    __shared__ float la[PARTS][64 * V], lb[PARTS][64 * V];
-    constexpr int R = MARK / 2;
-    typedef rows<E, V, R, !BACK, BACK> half;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), k = blockIdx.y;
-    const columns<V> c(s.N, s.D);
-    const int64_t plane = s.N * s.D, corner = c.n0 * s.D;
-    const uint32_t floats = c.template bytes<float>(s.D);
-    const int first = (k * PARTS + wave) * s.part, last = min(first + s.part, s.T);
-    factor A[V];
-    float B[V];
-    uint32_t begun = 0;
-#pragma unroll
-    for (int v = 0; v < V; ++v) B[v] = 0.0f;
-    auto run = [&](half& r, int t0) {
-        const int len = max(0, min(R, last - t0));
-        const uint32_t begin = r.begins(c);
-        begun |= begin;
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            const int t = BACK ? R - 1 - i : i;
-            if (t < len) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const float m = gate_of(get<E, V>(r.g[t], v));
-                    if (BACK) B[v] = (begin >> t) & 1 ? 0.0f : decay_of(m, get<E, V>(r.d[t], v) + B[v]);
-                    else B[v] = step_of(m, get<E, V>(r.x[t], v), (begin >> t) & 1 ? 0.0f : B[v]);
-                    A[v].step(m);
-                }
-            }
-        }
-    };
-    if (first < last) {
-        half p, q;
-        if (BACK) {
-            int t0 = first + (last - first - 1) / R * R;
-            p.load(s, c, t0, last, x, gate, grad_h, starts);
-            for (;;) {
-                q.load(s, c, max(t0 - R, first), last, x, gate, grad_h, starts);
-                run(p, t0);
-                if ((t0 -= R) < first) break;
-                p.load(s, c, max(t0 - R, first), last, x, gate, grad_h, starts);
-                run(q, t0);
-                if ((t0 -= R) < first) break;
-            }
-        } else {
-            p.load(s, c, first, last, x, gate, grad_h, starts);
-            for (int t0 = first; t0 < last; t0 += MARK) {
-                q.load(s, c, t0 + R, last, x, gate, grad_h, starts);
-                run(p, t0);
-                p.load(s, c, t0 + MARK, last, x, gate, grad_h, starts);
-                run(q, t0 + R);
-            }
-        }
-    }
-    float held[V], zero[V], mine[V], next[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) { held[v] = A[v].held(begun != 0); zero[v] = 0.0f; }
-#pragma unroll
-    for (int v = 0; v < V; ++v) { la[wave][v * 64 + lane] = held[v]; lb[wave][v * 64 + lane] = B[v]; }
-    __syncthreads();
-    float* part = maps + ((int64_t)s.chunks + (int64_t)k * PARTS + wave) * 2 * plane + corner;
-    if (c.valid) { store_floats<V>(part, floats, held); store_floats<V>(part + plane, floats, B); }
-    if (wave == 0) {
-        join<V, BACK>(la, lb, lane, PARTS, 0, zero, mine, next);
-#pragma unroll
-        for (int v = 0; v < V; ++v) held[v] = 0.0f;
-        for (int w = 0; w < PARTS; ++w) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) held[v] = after(held[v], la[w][v * 64 + lane]);
-        }
-        float* chunk = maps + (int64_t)k * 2 * plane + corner;
-        if (c.valid) { store_floats<V>(chunk, floats, held); store_floats<V>(chunk + plane, floats, next); }
-    }
-}
-
-// ---- whole (W = 1) and parts (W = PARTS): a wave runs through its steps, half a run ahead with its loads --------------------------------
-template <typename E, int V, int W>
-__global__ __launch_bounds__(64 * W, W == 1 ? 1 : 4) void k_memory_run(shape s, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ state,
-                                                                       E* __restrict__ h, float* __restrict__ state_out, float* __restrict__ marks, const float* __restrict__ maps) {
+// ---- whole: a wave runs through all steps, half a run ahead with its loads --------------------------------------------------------------
+template <typename E, int V>
+__global__ __launch_bounds__(64) void k_memory_run(shape s, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ state,
+                                                   E* __restrict__ h, float* __restrict__ state_out, float* __restrict__ marks) {
     typedef vec_t<E, V> vec;
     constexpr int R = MARK / 2;
     typedef rows<E, V, R, true, false> half;
@@ -362,15 +239,6 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 4) void k_memory_run(shape s, 
 #pragma unroll
     for (int v = 0; v < V; ++v) now[v] = 0.0f;
     if (state) load_floats<V>(now, state + corner, floats);
-    int first = 0, last = s.T;
-    if constexpr (W > 1) {
-        __shared__ float la[W][64 * V], lb[W][64 * V];
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), k = blockIdx.y;
-        enter<V, false>(maps + corner, plane, k, s.chunks, floats, wave, lane, la, lb, now);
-        first = (k * W + wave) * s.part;
-        last = min(first + s.part, s.T);
-        if (first >= last) return;
-    }
     auto steps = [&](const half& r, int t0, int len, auto all, uint32_t begin) {
         E* ph = h + (int64_t)t0 * plane + corner;
 #pragma unroll
@@ -389,32 +257,34 @@ __global__ __launch_bounds__(64 * W, W == 1 ? 1 : 4) void k_memory_run(shape s, 
         }
     };
     auto run = [&](const half& r, int t0) {          // whole and without a beginning, as nearly always, or not
-        const int len = max(0, min(R, last - t0));
+        const int len = max(0, min(R, s.T - t0));
         const uint32_t begin = r.begins(c);
         if (len == R && __ballot(begin != 0) == 0) steps(r, t0, len, yes(), 0u); else steps(r, t0, len, no(), begin);
     };
     half p, q;
-    p.load(s, c, first, last, x, gate, nullptr, starts);
-    for (int t0 = first; t0 < last; t0 += MARK) {
-        q.load(s, c, t0 + R, last, x, gate, nullptr, starts);
+    p.load(s, c, 0, s.T, x, gate, nullptr, starts);
+    for (int t0 = 0; t0 < s.T; t0 += MARK) {
+        q.load(s, c, t0 + R, s.T, x, gate, nullptr, starts);
         if (marks && c.valid) store_floats<V>(marks + (int64_t)(t0 / MARK) * plane + corner, floats, now);
         run(p, t0);
-        p.load(s, c, t0 + MARK, last, x, gate, nullptr, starts);
+        p.load(s, c, t0 + MARK, s.T, x, gate, nullptr, starts);
         run(q, t0 + R);
     }
-    if (state_out && c.valid && last == s.T) store_floats<V>(state_out + corner, floats, now);
+    if (state_out && c.valid) store_floats<V>(state_out + corner, floats, now);
 }
 
 // ---- chain: the maps of workgroups on their way to later ones ---------------------------------------------------------------------------
-// A link is a map (m, b) in one 64-bit word, written and read whole, so that there is nothing to order; EMPTY (no map has that m)
-// until it is written.  Workgroups take their place in the chain by a ticket, in the order in which they start: those a workgroup waits
-// for have started before it and write their links without waiting for anyone, so every wait ends.  All links before a chunk are
-// joined in the same order however late they come: results do not depend on timing.
+// A link is the map (m, b) of a workgroup in one 64-bit word, written and read whole, so that there is nothing to order; EMPTY (no map
+// has that m) until it is written.  Of every GROUP workgroups the last also leaves the value behind it, so that the next group starts
+// from that and no workgroup joins more than GROUP - 1 links.  Workgroups take their place in the chain by a ticket, in the order in
+// which they start: those a workgroup waits for have started before it, and wait only for earlier ones in turn, the first for nobody,
+// so every wait ends.  What is joined, and in which order, does not depend on who comes late, nor do results.
+constexpr int GROUP = 64;
 constexpr uint32_t EMPTY = 0xffffffffu;
-struct chain { uint32_t* ticket; uint64_t* links; uint32_t blocks; };          // links: [chunks][N * D]
+struct chain { uint32_t* ticket; uint64_t *links, *values; uint32_t blocks; };          // links: [chunks][N * D], values: [groups][N * D] (behind them)
 
-__global__ __launch_bounds__(256) void k_memory_unlink(chain ch, int64_t links) {
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < links; e += (int64_t)gridDim.x * 256) ch.links[e] = ~0ull;
+__global__ __launch_bounds__(256) void k_memory_unlink(chain ch, int64_t words) {
+    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < words; e += (int64_t)gridDim.x * 256) ch.links[e] = ~0ull;
     if (blockIdx.x == 0 && threadIdx.x == 0) *ch.ticket = 0;
 }
 
@@ -450,41 +320,61 @@ template <int V> __device__ __forceinline__ void follow(const uint64_t* links, i
         }
     }
 }
-// The workgroup's place, and then: its link (from its waves' maps la, lb) and the value that enters it (carry: the one that enters the chain).
 __device__ __forceinline__ uint32_t take_ticket(const chain& ch) {
     __shared__ uint32_t mine;
     if (threadIdx.x == 0) mine = __hip_atomic_fetch_add(ch.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     return __builtin_amdgcn_readfirstlane((int)mine);
 }
+// Leaves the workgroup's link (from its waves' maps la, lb) and finds the value that enters it; carry: the one that enters the chain.
 template <int V, bool BACK>
 __device__ __forceinline__ void pass_on(const chain& ch, int k, int chunks, int64_t plane, int64_t col, bool valid, int wave, int lane, const float (*la)[64 * V], const float (*lb)[64 * V],
                                         float (*lc)[64 * V], float (*ld)[64 * V], float (&carry)[V]) {
-    float m[V], b[V], zero[V];
+    const int order = BACK ? chunks - 1 - k : k, before = order % GROUP;
+    float m[V], b[V], zero[V], mine[V], next[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) m[v] = b[v] = zero[v] = 0.0f;
-    if (wave == 0 && (BACK ? k > 0 : k + 1 < chunks)) {          // (nobody waits for the last one's)
-        float mine[V], next[V];
-        join<V, BACK>(la, lb, lane, PARTS, 0, zero, mine, next);
-        for (int w = 0; w < PARTS; ++w) {
+    if (wave == 0 && before + 1 < GROUP && order + 1 < chunks) {          // (of the last one of a group nobody takes the link)
+        join<V, BACK>(la, lb, lane, WAVES, 0, zero, mine, next);
+        for (int w = 0; w < WAVES; ++w) {
 #pragma unroll
             for (int v = 0; v < V; ++v) m[v] = after(m[v], la[w][v * 64 + lane]);
         }
         if (valid) link<V>(ch.links + (int64_t)k * plane + col, m, next);
     }
-    const int before = BACK ? chunks - 1 - k : k;
-    if (before == 0) return;
+    if (before > 0) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) m[v] = b[v] = 0.0f;
-    const int lo = before * wave / PARTS, hi = before * (wave + 1) / PARTS;
-    follow<V>(ch.links + col, plane, BACK ? chunks - 1 - lo : lo, BACK ? -1 : 1, hi - lo, m, b);
+        for (int v = 0; v < V; ++v) m[v] = b[v] = 0.0f;
+        const int lo = before * wave / WAVES, hi = before * (wave + 1) / WAVES, way = BACK ? -1 : 1;
+        follow<V>(ch.links + col, plane, k - way * (before - lo), way, hi - lo, m, b);
 #pragma unroll
-    for (int v = 0; v < V; ++v) { lc[wave][v * 64 + lane] = m[v]; ld[wave][v * 64 + lane] = b[v]; }
-    __syncthreads();
-    float mine[V], next[V];
-    join<V, false>(lc, ld, lane, PARTS, 0, carry, mine, next);
+        for (int v = 0; v < V; ++v) { lc[wave][v * 64 + lane] = m[v]; ld[wave][v * 64 + lane] = b[v]; }
+    }
+    if (order >= GROUP) {
+        const uint64_t* from = ch.values + (int64_t)(order / GROUP) * plane + col;
 #pragma unroll
-    for (int v = 0; v < V; ++v) carry[v] = next[v];
+        for (int v = 0; v < V; ++v) {
+            uint64_t l = __hip_atomic_load(from + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            while ((uint32_t)(l >> 32) == EMPTY) {
+                __builtin_amdgcn_s_sleep(1);
+                l = __hip_atomic_load(from + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            carry[v] = __uint_as_float((uint32_t)l);
+        }
+    }
+    if (before > 0) {
+        __syncthreads();
+        join<V, false>(lc, ld, lane, WAVES, 0, carry, mine, next);
+#pragma unroll
+        for (int v = 0; v < V; ++v) carry[v] = next[v];
+    }
+}
+// The value behind the last workgroup of a group.
+template <int V, bool BACK> __device__ __forceinline__ void leave(const chain& ch, int k, int chunks, int64_t plane, int64_t col, bool valid, int wave, const float (&next)[V]) {
+    const int order = BACK ? chunks - 1 - k : k;
+    if (wave != 0 || !valid || (order + 1) % GROUP != 0 || order + 1 == chunks) return;
+#pragma unroll
+    for (int v = 0; v < V; ++v) __hip_atomic_store(ch.values + (int64_t)((order + 1) / GROUP) * plane + col + v, (uint64_t)__float_as_uint(next[v]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // ---- short: W waves of a workgroup take one run each ----------------------------------------------------------------------------------
@@ -530,6 +420,7 @@ __global__ __launch_bounds__(64 * W) void k_memory_short(shape s, chain ch, cons
     }
     float in[V], next[V];
     join<V, false>(la, lb, lane, W, wave, carry, in, next);
+    if constexpr (CHAIN) leave<V, false>(ch, (int)k, s.chunks, plane, corner + floats / 4, c.valid, wave, next);
     if (marks && c.valid && len > 0) store_floats<V>(marks + (int64_t)(t0 / MARK) * plane + corner, floats, in);
     E* ph = h + (int64_t)t0 * plane + corner;
 #pragma unroll
@@ -596,11 +487,10 @@ template <typename E, int V> struct run_back {
     }
 };
 
-// whole (W = 1) and parts (W = PARTS): a wave runs back through its steps, a run ahead with its loads
-template <typename E, int V, int W>
-__global__ __launch_bounds__(64 * W) void k_memory_run_back(shape s, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ marks,
-                                                            const E* __restrict__ grad_h, const float* __restrict__ grad_state, E* __restrict__ dx, E* __restrict__ dgate, float* __restrict__ dstate,
-                                                            const float* __restrict__ maps) {
+// whole: a wave runs back through all steps, a run ahead with its loads
+template <typename E, int V>
+__global__ __launch_bounds__(64) void k_memory_run_back(shape s, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ marks,
+                                                            const E* __restrict__ grad_h, const float* __restrict__ grad_state, E* __restrict__ dx, E* __restrict__ dgate, float* __restrict__ dstate) {
     const columns<V> c(s.N, s.D);
     const int64_t plane = s.N * s.D, corner = c.n0 * s.D;
     const uint32_t elems = c.template bytes<E>(s.D), floats = c.template bytes<float>(s.D);
@@ -608,34 +498,25 @@ __global__ __launch_bounds__(64 * W) void k_memory_run_back(shape s, const E* __
 #pragma unroll
     for (int v = 0; v < V; ++v) in[v] = 0.0f;
     if (grad_state) load_floats<V>(in, grad_state + corner, floats);
-    int first = 0, last = s.T;
-    if constexpr (W > 1) {
-        __shared__ float la[W][64 * V], lb[W][64 * V];
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), k = blockIdx.y;
-        enter<V, true>(maps + corner, plane, k, s.chunks, floats, wave, lane, la, lb, in);
-        first = (k * W + wave) * s.part;
-        last = min(first + s.part, s.T);
-        if (first >= last) return;
-    }
-    auto load = [&](run_back<E, V>& b, int t0) { b.load(s, c, max(t0, first), last, x, gate, grad_h, starts, marks, plane, corner, floats); };          // (in front of the first run: that again)
+    auto load = [&](run_back<E, V>& b, int t0) { b.load(s, c, max(t0, 0), s.T, x, gate, grad_h, starts, marks, plane, corner, floats); };          // (in front of the first run: that again)
     auto one = [&](run_back<E, V>& b, int t0) {
-        const int len = min(MARK, last - t0);
+        const int len = min(MARK, s.T - t0);
         float m[MARK][V], hs[MARK][V];
         const uint32_t begin = b.states(c, len, m, hs);
         b.finish(c, t0, len, begin, m, hs, in, dx, dgate, plane, corner, elems);
     };
     run_back<E, V> p, q;
-    int t0 = first + (last - first - 1) / MARK * MARK;
+    int t0 = (s.T - 1) / MARK * MARK;
     load(p, t0);
     for (;;) {
         load(q, t0 - MARK);
         one(p, t0);
-        if ((t0 -= MARK) < first) break;
+        if ((t0 -= MARK) < 0) break;
         load(p, t0 - MARK);
         one(q, t0);
-        if ((t0 -= MARK) < first) break;
+        if ((t0 -= MARK) < 0) break;
     }
-    if (dstate && c.valid && first == 0) store_floats<V>(dstate + corner, floats, in);
+    if (dstate && c.valid) store_floats<V>(dstate + corner, floats, in);
 }
 
 template <typename E, int V, int W, bool CHAIN>
@@ -679,6 +560,7 @@ __global__ __launch_bounds__(64 * W) void k_memory_short_back(shape s, chain ch,
     }
     float in[V], next[V];
     join<V, true>(la, lb, lane, W, W - 1 - wave, carry, in, next);
+    if constexpr (CHAIN) leave<V, true>(ch, k, s.chunks, plane, corner + floats / 4, c.valid, wave, next);
     if (len > 0) b.finish(c, t0, len, begin, m, hs, in, dx, dgate, plane, corner, elems);
     if (dstate && wave == 0 && c.valid && k == 0) store_floats<V>(dstate + corner, floats, next);
 }

@@ -93,6 +93,20 @@ def test_long_rollouts_of_few_walkers(T, N, D, dtype):
     check_all(x, gate, None, st, gh, gl)
 
 
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+@pytest.mark.parametrize('T', [8191, 8192, 8193, 8320, 8321, 16385, 25000])
+def test_chains_of_several_groups(T, dtype):
+    """64 workgroups of 128 steps each hand a value to the next 64: rollouts around and over multiples of 8192 steps, episodes that
+    begin right there, and none at all"""
+    x, gate, _, st, gh, gl = make(T, 2, 5, dtype, seed=T, shift=4.0)
+    b = torch.zeros(T, 2, dtype=torch.uint8)
+    b[[0, 127, 128, 8190, T - 1], 0] = 1
+    if T > 8192:
+        b[8192, 1] = 1
+    check_all(x, gate, b, st, gh, gl)
+    check_all(x, gate, None, st, gh, gl)
+
+
 @pytest.mark.parametrize('T,N,D', [(20, 513, 256), (40, 2100, 66), (129, 300, 512)])
 def test_many_walkers(T, N, D):
     check_all(*make(T, N, D, torch.bfloat16, seed=5))
