@@ -68,11 +68,12 @@ form memory_form(const dl_memory_shape* s, int V) {
     f.chunks = ceil_div(runs, f.W);
     return f;
 }
-// The form with the widest loads of its kernel; a chain's hold a whole run in registers, and wait: four bytes there, for twice the waves.
+// The form with the widest loads of its kernel.  The kernels that share the time axis hold a whole run in registers, and wait: four
+// bytes there, for twice the waves (128 x 128 x 512 bf16: 17.4 instead of 18.0 us).
 form memory_plan(const dl_memory_shape* s, int most) {
     form f = memory_form(s, memory_width(s, most));
     const int narrow = 4 / elem_bytes(s->dtype);
-    return f.chunks > 1 && f.V > narrow ? memory_form(s, memory_width(s, narrow)) : f;
+    return f.W > 1 && f.V > narrow ? memory_form(s, memory_width(s, narrow)) : f;
 }
 // A chain: its ticket, a link of two floats per chunk and column, a value per group of chunks.
 int64_t chain_words(const dl_memory_shape* s, const form& f) { return (f.chunks + ceil_div(f.chunks, dlm::GROUP)) * s->N * s->D; }
@@ -156,19 +157,20 @@ int32_t whole_tiles(int64_t tiles, int64_t batch, int64_t slots) {
 // Tiles of 256 x 128 (a CU each) where they come to at least nine tenths of a round of whole ones and what is left in 64 x 64 to one
 // round at most, else of 128 x 128 (two to a CU).  4096 x 8192 x 4096: 610 instead of 652 us; 2 x 1031 x 4099 x 1031, where 328 of
 // 64 x 64 would be left: 71 and 68 us.
-template <int TILE, int MODE> void launch_product(dlo::product p, int64_t tiles, int64_t batch, const dlo::plan& q, hipStream_t st) {
+template <int TILE, int MODE, bool COARSE> void launch_product(dlo::product p, int64_t tiles, int64_t batch, const dlo::plan& q, hipStream_t st) {
     if constexpr (TILE == 32) dlo::k_orth_direct<MODE><<<dim3((unsigned)tiles, 1, (unsigned)batch), 512, 0, st>>>(p);
     else {
+        if (COARSE) p.kb /= 2;          // two at once
         constexpr bool half = MODE == dlo::GRAM || MODE == dlo::POLY;
         const int64_t wi = q.mp / 256, wj = q.np / 128, wide = half ? wi * (wi + 1) : wi * wj, whole = whole_tiles(wide, batch, 256);
         const int64_t left = (wide - whole) * 8 + (q.mp % 256 ? 2 * (half ? q.mp / 64 : q.np / 64) : 0);
         if (whole * batch >= 230 && left * batch <= 256) {
             p.tiles = (int32_t)wide; p.whole = (int32_t)whole;
             p.tiles_i = (int32_t)wi; p.tiles_j = (int32_t)wj;
-            return dlo::k_orth_wide<MODE><<<dim3((unsigned)(whole + left), 1, (unsigned)batch), 256, 0, st>>>(p);
+            return dlo::k_orth_wide<MODE, COARSE><<<dim3((unsigned)(whole + left), 1, (unsigned)batch), 256, 0, st>>>(p);
         }
         p.tiles = (int32_t)tiles; p.whole = whole_tiles(tiles, batch, 512);
-        dlo::k_orth_product<MODE><<<dim3((unsigned)(p.whole + (tiles - p.whole) * 4), 1, (unsigned)batch), 256, 0, st>>>(p);
+        dlo::k_orth_product<MODE, COARSE><<<dim3((unsigned)(p.whole + (tiles - p.whole) * 4), 1, (unsigned)batch), 256, 0, st>>>(p);
     }
 }
 
@@ -180,19 +182,21 @@ template <int TILE> void launch_steps(const dl_orth_shape* s, const orth_form& f
     const int64_t ti = f.p.mp / TILE, tj = f.p.np / TILE, tri = ti * (ti + 1) / 2;
     const int32_t km = f.p.mp / 32, kn = f.p.np / 32;
     for (int k = 0; k < s->steps; ++k) {
+        const bool end = k + 1 == s->steps, coarse = TILE != 32 && end && s->out_type == DL_BF16;
         dlo::product p = last;
         p.P = p.Q = xr; p.P_b = p.Q_b = f.p.x_size; p.kb = kn;
         p.out0 = A; p.out0_b = f.p.a_size; p.out0_kb = km;
-        launch_product<TILE, dlo::GRAM>(p, tri, s->batch, f.p, st);
+        if (coarse) launch_product<TILE, dlo::GRAM, TILE != 32>(p, tri, s->batch, f.p, st); else launch_product<TILE, dlo::GRAM, false>(p, tri, s->batch, f.p, st);
         p.P = p.Q = A; p.P_b = p.Q_b = f.p.a_size; p.kb = km;
         p.A = A; p.out0 = Q;
-        launch_product<TILE, dlo::POLY>(p, tri, s->batch, f.p, st);
+        if (coarse) launch_product<TILE, dlo::POLY, TILE != 32>(p, tri, s->batch, f.p, st); else launch_product<TILE, dlo::POLY, false>(p, tri, s->batch, f.p, st);
         p.P = Q; p.Q = xc[k & 1]; p.Q_b = f.p.x_size;
         p.tiles_i = (int32_t)ti; p.tiles_j = (int32_t)tj;
         p.out0 = xr; p.out0_b = f.p.x_size; p.out0_kb = kn;
         p.out1 = xc[(k + 1) & 1]; p.out1_b = f.p.x_size; p.out1_kb = km;
-        if (k + 1 < s->steps) launch_product<TILE, dlo::STEP>(p, ti * tj, s->batch, f.p, st);
-        else launch_product<TILE, dlo::LAST>(p, ti * tj, s->batch, f.p, st);
+        if (!end) launch_product<TILE, dlo::STEP, false>(p, ti * tj, s->batch, f.p, st);
+        else if (coarse) launch_product<TILE, dlo::LAST, TILE != 32>(p, ti * tj, s->batch, f.p, st);
+        else launch_product<TILE, dlo::LAST, false>(p, ti * tj, s->batch, f.p, st);
     }
 }
 
@@ -229,15 +233,15 @@ int dl_memory_forward(const dl_memory_shape* s, const void* x, const void* gate,
         constexpr int V = decltype(v)::value;
         if (f.W == 1) {
             dlm::k_memory_run<E, V><<<grid, 64, 0, st>>>(d, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks);
-        } else if (f.chunks > 1) {
-            if constexpr (V * sizeof(E) <= 4) {
+        } else if constexpr (V * sizeof(E) <= 4) {
+            if (f.chunks > 1) {
                 const dlm::chain ch = start_chain(s, f, workspace, st);
                 dlm::k_memory_short<E, V, dlm::WAVES, true><<<grid, 64 * dlm::WAVES, 0, st>>>(d, ch, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks);
-            }
-        } else with_waves(f.W, [&](auto w) {
-            constexpr int W = decltype(w)::value;
-            dlm::k_memory_short<E, V, W, false><<<grid, 64 * W, 0, st>>>(d, dlm::chain{}, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks);
-        });
+            } else with_waves(f.W, [&](auto w) {
+                constexpr int W = decltype(w)::value;
+                dlm::k_memory_short<E, V, W, false><<<grid, 64 * W, 0, st>>>(d, dlm::chain{}, (const E*)x, (const E*)gate, starts, state, (E*)h, state_out, marks);
+            });
+        }
     }); });
     return launched("dl_memory_forward");
 }

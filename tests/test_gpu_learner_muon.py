@@ -75,6 +75,40 @@ def test_large_matrices(rows, cols):
     check_orthogonal(orthogonalise(g.cuda()), g)
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize('rows,cols,steps', [(1500, 1700, 5), (1300, 2300, 1), (2050, 1300, 2)])
+def test_large_matrices_of_16_bits(rows, cols, steps, dtype):
+    """bfloat16: the last step has operands of 11 bits.  Its products are off by 2^-11 / sqrt(3) per operand at random, two operands
+    in each of three products: below 2.5 * 2^-11 / sqrt(3) = 2^-10.5 of the norm where singular values differ (2^-9.3 of the norm at most), next to the half step 2^-8
+    that check_orthogonal allows.  float16: as exact as float32, one rounding."""
+    from drloco_amd.muon import orthogonalise
+    g = gradient(rows, cols, seed=2, dtype=dtype)
+    check_orthogonal(orthogonalise(g.cuda(), steps), g, steps)
+
+
+def orthogonal_on_device(g, dtype, steps=5, coefficients=(3.4445, -4.7750, 2.0315)):
+    a, b, c = coefficients
+    x = g.double()
+    x = (x / x.norm()).to(dtype)
+    for _ in range(steps):
+        p = x @ x.t() if x.shape[0] <= x.shape[1] else x.t() @ x
+        q = b * p + c * (p @ p)
+        x = a * x + (q @ x if x.shape[0] <= x.shape[1] else x @ q)
+    return x.double()
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize('rows,cols', [(2170, 4090), (3904, 4000), (4200, 4096), (700, 20000)])
+def test_matrices_that_fill_the_chip(rows, cols, dtype):
+    """256 x 128 tiles, whole rounds of them, cut-up rests and a short side that is an odd multiple of 128; 64-bit and float32 products on the
+    device, and the second rule of check_orthogonal; bfloat16: next to the half step of the result, 2^-8."""
+    from drloco_amd.muon import orthogonalise
+    g = gradient(rows, cols, seed=3, dtype=dtype).cuda()
+    o, want = orthogonalise(g), orthogonal_on_device(g, torch.float64)
+    err, err32, norm = (float(t.norm()) for t in (o.double() - want, orthogonal_on_device(g, torch.float32) - want, want))
+    assert err <= 8 * err32 + 2.0 ** -20 * norm + (0 if dtype == torch.float32 else 2.0 ** -8) * norm, (err, err32, norm)
+
+
 @pytest.mark.parametrize('steps', [1, 2, 3, 8])
 @pytest.mark.parametrize('name', ['COEFFICIENTS', 'CUBIC'])
 @pytest.mark.parametrize('rows,cols', [(40, 72), (200, 130)])
