@@ -123,8 +123,9 @@ const char* orth_shape_error(const dl_orth_shape* s) {
 struct orth_form {
     dlo::plan p;
     int tile;
-    bool turned, small;
-    int64_t x_bytes, a_bytes, bytes;          // of the whole batch; the workspace: partials, XR, XC, XC', A, Q
+    bool turned, small, gram_direct, poly_direct;          // direct: k_orth_direct for this product
+    int64_t splits, counters;                 // of a Gram tile along its sum, and the counters of all tiles
+    int64_t head, x_bytes, a_bytes, bytes;    // the workspace: partials, counters and split sums (together head), XR, XC, XC', A, Q of the whole batch
 };
 
 constexpr int64_t DIRECT = (int64_t)640 * 640 * 640;
@@ -144,7 +145,20 @@ orth_form orth_plan(const dl_orth_shape* s) {
     f.p.partials = (int32_t)std::min<int64_t>(1024, ceil_div(s->rows * s->cols, 4096));
     f.x_bytes = s->batch * f.p.x_size * 2;
     f.a_bytes = s->batch * f.p.a_size * 2;
-    f.bytes = ceil_div(s->batch * f.p.partials * 8, 256) * 256 + 3 * f.x_bytes + 2 * f.a_bytes;
+    // Of a product with few tiles in the staged kernels the direct one may be the faster: 0.27 us a step of 64 x 64 tiles against 64 rows
+    // from the caches for every 32 x 32 tile, at 10 TB/s, and 3 us more where the sum is split.
+    auto direct = [&](int64_t k) {
+        const int64_t t64 = f.p.mp / 64 * (f.p.mp / 64 + 1) / 2 * s->batch, t32 = f.p.mp / 32 * (f.p.mp / 32 + 1) / 2 * s->batch;
+        return f.tile == 32 || (double)ceil_div(t64, 512) * (double)(k / 32) * 0.27 > (double)t32 * 64 * (double)k * 4 * 1e-7 + 3;
+    };
+    f.gram_direct = direct(f.p.np);
+    f.poly_direct = direct(f.p.mp);
+    // A workgroup per CU and two steps for each of its eight waves; not worth the way through memory below some hundred steps.
+    const int64_t tri = f.p.mp / 32 * (f.p.mp / 32 + 1) / 2 * s->batch, steps = f.p.np / 32;
+    f.splits = f.gram_direct && steps >= 128 ? std::max<int64_t>(1, std::min<int64_t>({ceil_div(256, tri), steps / 16, 64})) : 1;
+    f.counters = f.splits > 1 ? tri : 0;
+    f.head = ceil_div(s->batch * f.p.partials * 8 + f.counters * 4, 256) * 256;
+    f.bytes = f.head + f.counters * f.splits * 4096 + 3 * f.x_bytes + 2 * f.a_bytes;
     return f;
 }
 
@@ -157,9 +171,12 @@ int32_t whole_tiles(int64_t tiles, int64_t batch, int64_t slots) {
 // Tiles of 256 x 128 (a CU each) where they come to at least nine tenths of a round of whole ones and what is left in 64 x 64 to one
 // round at most, else of 128 x 128 (two to a CU).  4096 x 8192 x 4096: 610 instead of 652 us; 2 x 1031 x 4099 x 1031, where 328 of
 // 64 x 64 would be left: 71 and 68 us.
-template <int TILE, int MODE, bool COARSE> void launch_product(dlo::product p, int64_t tiles, int64_t batch, const dlo::plan& q, hipStream_t st) {
-    if constexpr (TILE == 32) dlo::k_orth_direct<MODE><<<dim3((unsigned)tiles, 1, (unsigned)batch), 512, 0, st>>>(p);
-    else {
+template <int TILE, int MODE, bool COARSE> void launch_product(dlo::product p, int64_t tiles, int64_t batch, const orth_form& f, hipStream_t st) {
+    const dlo::plan& q = f.p;
+    if (TILE == 32 || (MODE == dlo::GRAM && f.gram_direct) || (MODE == dlo::POLY && f.poly_direct)) {
+        if (TILE != 32) tiles = (int64_t)(q.mp / 32) * (q.mp / 32 + 1) / 2;
+        dlo::k_orth_direct<MODE><<<dim3((unsigned)(MODE == dlo::GRAM ? tiles * p.splits : tiles), 1, (unsigned)batch), 512, 0, st>>>(p);
+    } else if constexpr (TILE != 32) {
         if (COARSE) p.kb /= 2;          // two at once
         constexpr bool half = MODE == dlo::GRAM || MODE == dlo::POLY;
         const int64_t wi = q.mp / 256, wj = q.np / 128, wide = half ? wi * (wi + 1) : wi * wj, whole = whole_tiles(wide, batch, 256);
@@ -186,17 +203,17 @@ template <int TILE> void launch_steps(const dl_orth_shape* s, const orth_form& f
         dlo::product p = last;
         p.P = p.Q = xr; p.P_b = p.Q_b = f.p.x_size; p.kb = kn;
         p.out0 = A; p.out0_b = f.p.a_size; p.out0_kb = km;
-        if (coarse) launch_product<TILE, dlo::GRAM, TILE != 32>(p, tri, s->batch, f.p, st); else launch_product<TILE, dlo::GRAM, false>(p, tri, s->batch, f.p, st);
+        if (coarse) launch_product<TILE, dlo::GRAM, TILE != 32>(p, tri, s->batch, f, st); else launch_product<TILE, dlo::GRAM, false>(p, tri, s->batch, f, st);
         p.P = p.Q = A; p.P_b = p.Q_b = f.p.a_size; p.kb = km;
         p.A = A; p.out0 = Q;
-        if (coarse) launch_product<TILE, dlo::POLY, TILE != 32>(p, tri, s->batch, f.p, st); else launch_product<TILE, dlo::POLY, false>(p, tri, s->batch, f.p, st);
+        if (coarse) launch_product<TILE, dlo::POLY, TILE != 32>(p, tri, s->batch, f, st); else launch_product<TILE, dlo::POLY, false>(p, tri, s->batch, f, st);
         p.P = Q; p.Q = xc[k & 1]; p.Q_b = f.p.x_size;
         p.tiles_i = (int32_t)ti; p.tiles_j = (int32_t)tj;
         p.out0 = xr; p.out0_b = f.p.x_size; p.out0_kb = kn;
         p.out1 = xc[(k + 1) & 1]; p.out1_b = f.p.x_size; p.out1_kb = km;
-        if (!end) launch_product<TILE, dlo::STEP, false>(p, ti * tj, s->batch, f.p, st);
-        else if (coarse) launch_product<TILE, dlo::LAST, TILE != 32>(p, ti * tj, s->batch, f.p, st);
-        else launch_product<TILE, dlo::LAST, false>(p, ti * tj, s->batch, f.p, st);
+        if (!end) launch_product<TILE, dlo::STEP, false>(p, ti * tj, s->batch, f, st);
+        else if (coarse) launch_product<TILE, dlo::LAST, TILE != 32>(p, ti * tj, s->batch, f, st);
+        else launch_product<TILE, dlo::LAST, false>(p, ti * tj, s->batch, f, st);
     }
 }
 
@@ -326,15 +343,18 @@ int dl_orth_update(const dl_orth_shape* s, const void* grad, const float* moment
         return launched("dl_orth_update");
     }
     double* partials = (double*)workspace;
-    char* work = (char*)workspace + ceil_div(s->batch * f.p.partials * 8, 256) * 256;
+    uint32_t* counters = (uint32_t*)(partials + s->batch * f.p.partials);
+    float* parts = (float*)((char*)workspace + f.head);
+    char* work = (char*)parts + f.counters * f.splits * 4096;
     const dlo::source src{grad, s->grad_type, momentum, momentum_out, (float)s->beta, s->nesterov, s->grad_b, s->grad_r, s->momentum_b, s->momentum_r, s->momentum_out_b, s->momentum_out_r};
-    dlo::k_orth_norm<<<dim3((unsigned)f.p.partials, (unsigned)s->batch), 256, 0, st>>>(src, flat ? 1 : s->rows, flat ? s->rows * s->cols : s->cols, partials);
+    dlo::k_orth_norm<<<dim3((unsigned)f.p.partials, (unsigned)s->batch), 256, 0, st>>>(src, flat ? 1 : s->rows, flat ? s->rows * s->cols : s->cols, partials, counters, (int)f.counters);
     dlo::k_orth_load<<<dim3((unsigned)ceil_div(f.p.np, 64), (unsigned)ceil_div(f.p.mp, 64), (unsigned)s->batch), 256, 0, st>>>(src, f.p, f.turned, partials, (_Float16*)work, (_Float16*)(work + f.x_bytes));
     dlo::product p{};
     p.a = (float)s->a; p.b = (float)s->b; p.c = (float)s->c;
     p.out = out; p.w = weight; p.out_type = s->out_type; p.w_type = s->weight_type;
     p.out_at = f.turned ? dlo::matrix{s->out_b, 1, s->out_r} : dlo::matrix{s->out_b, s->out_r, 1};
     p.w_at = f.turned ? dlo::matrix{s->weight_b, 1, s->weight_r} : dlo::matrix{s->weight_b, s->weight_r, 1};
+    p.splits = (int32_t)f.splits; p.parts = parts; p.arrived = counters;
     p.keep = (float)s->weight_keep; p.gain = (float)s->gain;
     p.m = f.p.m; p.n = f.p.n;
     if (f.tile == 32) launch_steps<32>(s, f, p, work, st); else launch_steps<128>(s, f, p, work, st);

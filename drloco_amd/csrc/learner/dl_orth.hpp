@@ -112,7 +112,9 @@ struct place {
 };
 
 // rows x cols as they are read: one long row where the rows of all arrays follow each other
-__global__ __launch_bounds__(256) void k_orth_norm(source s, int64_t rows, int64_t cols, double* __restrict__ partials) {
+// (and counters for later kernels to zero)
+__global__ __launch_bounds__(256) void k_orth_norm(source s, int64_t rows, int64_t cols, double* __restrict__ partials, uint32_t* __restrict__ counters, int n_counters) {
+    if (blockIdx.x == 0 && blockIdx.y == 0) for (int k = threadIdx.x; k < n_counters; k += 256) counters[k] = 0;
     constexpr int AT_ONCE = 4;
     const int64_t per = (cols + 3) / 4, all = rows * per, step = (int64_t)gridDim.x * 256;          // in fours
     double sum = 0.0;
@@ -194,6 +196,9 @@ struct product {
     _Float16* out1; int64_t out1_b, out1_kb;       // STEP: XC
     const _Float16* A;                             // POLY: as out0
     float a, b, c;
+    // GRAM of k_orth_direct with `splits` workgroups per tile along k: their sums, and a counter per tile that is zero before and after
+    int32_t splits;
+    float* parts; uint32_t* arrived;
     // LAST: out = keep * w + gain * X
     void* out; const void* w; int out_type, w_type;
     matrix out_at, w_at;
@@ -561,6 +566,8 @@ __global__ __launch_bounds__(256, 1) void k_orth_wide(product p) {
 // One 32 x 32 tile per workgroup, eight waves take every eighth step along k straight from memory: all their loads are on the way at
 // once, nothing is staged and nothing waited for but the sum over the waves.  Every element comes from the L2 cache 32 times
 // (m n k / 4 bytes in all), which is what bounds it from some 600^3 on.
+// A = X X' of a short and long X has few tiles and many steps: they are split over workgroups, and the last of a tile's to finish sums
+// what all have left, in their order, not in that of their coming (8 x 8000, all five steps: 157 -> @@ us).
 template <int MODE>
 __global__ __launch_bounds__(512) void k_orth_direct(product p) {
     constexpr int WAVES = 8;
@@ -569,15 +576,17 @@ __global__ __launch_bounds__(512) void k_orth_direct(product p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int64_t b = blockIdx.z;
     int ti, tj;
-    if (MODE == GRAM || MODE == POLY) below(blockIdx.x, ti, tj);
+    const int tile_ = MODE == GRAM ? blockIdx.x / p.splits : blockIdx.x, share = MODE == GRAM ? blockIdx.x % p.splits : 0;
+    if (MODE == GRAM || MODE == POLY) below(tile_, ti, tj);
     else {
-        ti = blockIdx.x % p.tiles_i; tj = blockIdx.x / p.tiles_i;
+        ti = tile_ % p.tiles_i; tj = tile_ / p.tiles_i;
     }
+    const int first = MODE == GRAM ? (int)((int64_t)p.kb * share / p.splits) : 0, last = MODE == GRAM ? (int)((int64_t)p.kb * (share + 1) / p.splits) : p.kb;
     const _Float16* P = p.P + b * p.P_b + (int64_t)ti * 2 * p.kb * FRAG + lane * 8;
     const _Float16* Q = p.Q + b * p.Q_b + (int64_t)tj * 2 * p.kb * FRAG + lane * 8;
     float4_ acc[2][2] = {};
 #pragma unroll 4
-    for (int k = wave; k < p.kb; k += WAVES) {
+    for (int k = first + wave; k < last; k += WAVES) {
         half8 ph[2], pl[2], qh[2], ql[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -601,10 +610,36 @@ __global__ __launch_bounds__(512) void k_orth_direct(product p) {
         for (int j = 0; j < 2; ++j) *(float4_*)&part[wave][i * 2 + j][lane * 4] = acc[i][j];
     const int i0 = ti * 32, j0 = tj * 32;
     __syncthreads();
+    float4_ v = {};
     if (wave < 4) {          // a wave sums a quarter
-        float4_ v = {};
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) v += *(const float4_*)&part[w][wave][lane * 4];
+    }
+    if (MODE == GRAM && p.splits > 1) {
+        // left where every die sees it (a die's L2 cache does not hold it back), 8 bytes at a time
+        const int64_t at = b * (gridDim.x / p.splits) + tile_;
+        uint64_t* mine = (uint64_t*)p.parts + ((at * p.splits + share) * 4 + wave) * 128 + lane * 2;
+        if (wave < 4) {
+            __hip_atomic_store(mine, (uint64_t)__float_as_uint(v[1]) << 32 | __float_as_uint(v[0]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(mine + 1, (uint64_t)__float_as_uint(v[3]) << 32 | __float_as_uint(v[2]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __shared__ uint32_t before;
+        __syncthreads();          // (waits for the stores too)
+        if (threadIdx.x == 0) before = __hip_atomic_fetch_add(p.arrived + at, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if ((int)before + 1 < p.splits) return;
+        if (threadIdx.x == 0) __hip_atomic_store(p.arrived + at, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (wave < 4) {
+            v = float4_{};
+            mine -= (int64_t)share * 512;
+#pragma unroll 8
+            for (int k = 0; k < p.splits; ++k) {
+                const uint64_t lo = __hip_atomic_load(mine + k * 512, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), hi = __hip_atomic_load(mine + k * 512 + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                v += float4_{__uint_as_float((uint32_t)lo), __uint_as_float((uint32_t)(lo >> 32)), __uint_as_float((uint32_t)hi), __uint_as_float((uint32_t)(hi >> 32))};
+            }
+        }
+    }
+    if (wave < 4) {
         const int i = (wave >> 1) * 16 + (lane >> 4) * 4, j = (wave & 1) * 16 + (lane & 15);
         if (MODE == POLY) {
             // A[i + r][j] lies in the fragment of row j (A is symmetric): four neighbours

@@ -11,6 +11,7 @@ The default is 128 walkers x 128-step rollouts (the reference: 8 x 2048); rollou
 with thousands of walkers.  Everything of the rollout runs through the C-ABI:
 dl_policy_forward -> dl_step -> dl_vecnormalize_step -> dl_gae; torch autograd only evaluates the PPO loss.
 
+  python examples/train_ppo.py --optimizer muon # the trunk's matrices by orthogonalised updates (drloco_amd.muon)
   python examples/train_ppo.py --mio 8          # the reference's budget: 8 M env-steps, ~30 s on one MI355X, walks 23 m per episode (3 of 4 seeds)
   python -m torch.distributed.run --nnodes=1 --nproc-per-node 8 --master-addr 127.0.0.1 examples/train_ppo.py --envs 1024
                                                 # data parallel: walkers shard by global index (--envs is the GLOBAL count), one rank per GPU over RCCL;
@@ -28,12 +29,13 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 import torch
 
 from drloco_amd import collectives
+from drloco_amd.muon import HipMuon
 from drloco_amd.policy import HipPolicy
 from drloco_amd.rollout import HipRolloutBuffer
 from drloco_amd.vec_env import HipVecEnv, HipVecNormalize
 
 
-def train(mio=2.0, n_envs=128, batch=16384, minibatch=2048, epochs=4, seed=0, log_every=25, quiet=False, norm_reward=True, evaluate=False, save_path=None, moments='per_step', return_objects=False):
+def train(mio=2.0, n_envs=128, batch=16384, minibatch=2048, epochs=4, seed=0, log_every=25, quiet=False, norm_reward=True, evaluate=False, save_path=None, moments='per_step', return_objects=False, optimizer='adam', muon_lr=0.01):
     # one process per GPU under torch.distributed.run (backend nccl = RCCL); a single process otherwise
     import torch.distributed as dist
     world, rank, local_rank = int(os.environ.get('WORLD_SIZE', '1')), int(os.environ.get('RANK', '0')), int(os.environ.get('LOCAL_RANK', '0'))
@@ -65,7 +67,13 @@ def train(mio=2.0, n_envs=128, batch=16384, minibatch=2048, epochs=4, seed=0, lo
     wd = dict(zip(names, params))
     bucket = collectives.FlatGradAllReducer(params)      # C2: one all-reduce of the flat gradient per optimiser step
     perm_gen = torch.Generator().manual_seed(seed + 1000)    # minibatch permutations: the same on every rank
-    opt = torch.optim.Adam(params, lr=5e-4, eps=1e-5)
+    if optimizer == 'muon':          # the trunk's matrices by orthogonalised updates, heads, biases and log_std by Adam
+        matrices = [wd[n_] for n_ in ('w1', 'w2')]
+        muon = HipMuon(matrices, lr=muon_lr)
+        opt = torch.optim.Adam([p for n_, p in wd.items() if n_ not in ('w1', 'w2')], lr=5e-4, eps=1e-5)
+    else:
+        muon = None
+        opt = torch.optim.Adam(params, lr=5e-4, eps=1e-5)
     clip, ent_coef, vf_coef = 0.15, -0.0075, 0.5
     total = int(mio * 1e6)
     n_updates = max(1, total // batch)
@@ -79,6 +87,9 @@ def train(mio=2.0, n_envs=128, batch=16384, minibatch=2048, epochs=4, seed=0, lo
         lr = max(5e-4 + (upd / n_updates) * (1e-6 - 5e-4), 1e-6)             # LinearDecay(5e-4 -> 1e-6)
         for gp in opt.param_groups:
             gp['lr'] = lr
+        if muon is not None:
+            for gp in muon.param_groups:
+                gp['lr'] = muon_lr * lr / 5e-4
         # ---- collect_rollouts
         with torch.no_grad():
             buf.collect_rollouts(vn, pol, obs, start, moments=moments)        # dl_collect_rollouts: T x (policy -> step -> normalise) in one call -- one persistent launch where that form exists
@@ -97,10 +108,14 @@ def train(mio=2.0, n_envs=128, batch=16384, minibatch=2048, epochs=4, seed=0, lo
                 adv, n_mb = collectives.minibatch_adv_normalize(b_adv[idx])                          # C1: statistics of the global minibatch
                 loss = collectives.ppo_minibatch_loss(wd, b_obs[idx], b_act[idx], adv, b_ret[idx], b_val[idx], b_lp[idx], n_mb, clip, ent_coef, vf_coef)
                 opt.zero_grad(set_to_none=True)
+                if muon is not None:
+                    muon.zero_grad(set_to_none=True)
                 loss.backward()
                 bucket.reduce()
                 torch.nn.utils.clip_grad_norm_(params, 0.5)
                 opt.step()
+                if muon is not None:
+                    muon.step()
         if upd % log_every == 0 or upd == n_updates - 1:
             torch.cuda.synchronize()
             ep_len = torch.tensor(venv.get_attr('ep_len_smoothed')).mean().item()
@@ -137,7 +152,7 @@ def train(mio=2.0, n_envs=128, batch=16384, minibatch=2048, epochs=4, seed=0, lo
         os.makedirs(os.path.join(save_path, 'models'), exist_ok=True); os.makedirs(os.path.join(save_path, 'envs'), exist_ok=True)
         ckpt = f'{int(total / 1e5)}'
         # SB3 1.0's save_to_zip_file layout: data (spaces, policy class, hyperparameters), policy.pth, policy.optimizer.pth (Adam's moments)
-        checkpoint.write_model_zip(pol, os.path.join(save_path, 'models', f'model_{ckpt}.zip'), observation_space=venv.observation_space, action_space=venv.action_space, optimizer=opt,
+        checkpoint.write_model_zip(pol, os.path.join(save_path, 'models', f'model_{ckpt}.zip'), observation_space=venv.observation_space, action_space=venv.action_space, optimizer=opt if muon is None else None,
                                    hyper=dict(n_envs=n_envs, num_timesteps=int(total), n_steps=batch // n_envs, batch_size=minibatch, n_epochs=epochs, learning_rate=float(lr)))
         vn.save(os.path.join(save_path, 'envs', f'env_{ckpt}'), sb3_format=True)
         if not quiet:
@@ -157,5 +172,7 @@ if __name__ == '__main__':
     ap.add_argument('--save', default=None, help='directory for models/model_<ckpt>.zip (policy.pth with SB3 1.0 key names) and envs/env_<ckpt> (VecNormalize statistics), drloco_amd/checkpoint.py')
     ap.add_argument('--no-norm-reward', action='store_true', help='VecNormalize(norm_reward=False)')
     ap.add_argument('--moments', choices=['per_step', 'per_rollout'], default='per_step', help="VecNormalize moments inside a rollout: SB3's per-step update (default) or the opt-in per-rollout relaxation of the persistent rollout kernel")
+    ap.add_argument('--optimizer', choices=['adam', 'muon'], default='adam', help="the reference's Adam (default), or Muon (drloco_amd.muon.HipMuon) for the trunk's two matrices and Adam for the rest; a saved model then has no optimiser state")
+    ap.add_argument('--muon-lr', type=float, default=0.01, help='Muon: learning rate of the matrices at the start, decays as the other')
     args = ap.parse_args()
-    train(args.mio, args.envs, batch=args.batch, minibatch=args.minibatch, seed=args.seed, norm_reward=not args.no_norm_reward, evaluate=True, save_path=args.save, moments=args.moments)
+    train(args.mio, args.envs, batch=args.batch, minibatch=args.minibatch, seed=args.seed, norm_reward=not args.no_norm_reward, evaluate=True, save_path=args.save, moments=args.moments, optimizer=args.optimizer, muon_lr=args.muon_lr)
