@@ -123,21 +123,32 @@ const char* orth_shape_error(const dl_orth_shape* s) {
 struct orth_form {
     dlo::plan p;
     int tile;
-    bool turned, small, gram_direct, poly_direct;          // direct: k_orth_direct for this product
+    bool turned, small, slab, gram_direct, poly_direct;          // direct: k_orth_direct for this product
+    int64_t slab_rows, slab_cols, n_slabs;    // 16 rows, columns and number of slabs
     int64_t splits, counters;                 // of a Gram tile along its sum, and the counters of all tiles
     int64_t head, x_bytes, a_bytes, bytes;    // the workspace: partials, counters and split sums (together head), XR, XC, XC', A, Q of the whole batch
 };
 
-constexpr int64_t DIRECT = (int64_t)640 * 640 * 640;
+constexpr int64_t DIRECT = (int64_t)800 * 800 * 800;
 
 orth_form orth_plan(const dl_orth_shape* s) {
     orth_form f;
     f.turned = s->rows > s->cols;
     f.p.m = (int32_t)std::min(s->rows, s->cols);
     f.p.n = (int32_t)std::max(s->rows, s->cols);
-    f.small = f.p.m <= 32 ? f.p.n <= 1024 : f.p.m <= 64 && f.p.n <= 256;          // what a workgroup's LDS holds
+    f.small = f.p.n <= (f.p.m <= 16 ? 1024 : f.p.m <= 32 ? 512 : f.p.m <= 64 ? 256 : 0);          // what a workgroup's LDS and registers hold
+    // Short sides of up to 64: a slab of 512 columns (up to 32 rows) or 256 per workgroup; from 256 slabs on the sums over them weigh more
+    // than the launches they save.
+    f.slab_rows = f.p.m <= 16 ? 1 : f.p.m <= 32 ? 2 : 4;
+    f.slab_cols = f.slab_rows == 4 ? 256 : 512;
+    f.n_slabs = ceil_div(f.p.n, f.slab_cols);
+    f.slab = !f.small && f.p.m <= 64 && f.n_slabs < 256;
     const int64_t m32 = ceil_div(f.p.m, 32) * 32, n32 = ceil_div(f.p.n, 32) * 32;
-    f.tile = s->batch * m32 * m32 * n32 <= DIRECT ? 32 : 128;
+    // Whatever sets the order of a matrix's sums (tile, direct or staged, splits) follows from that matrix alone, never from how many come
+    // with it: a matrix has the same result, bit for bit, by itself and in any stack.
+    // What that costs where a rule on the whole stack would have taken the staged kernels: 16 x 512 x 512 404 instead of 359 us, 64 x 512 x
+    // 512 1515 instead of 1154, 8 x 100 x 8000 509 instead of 262; 4 x 700 x 700 gains, 241 instead of 274.
+    f.tile = m32 * m32 * n32 <= DIRECT ? 32 : 128;
     f.p.mp = (int32_t)(ceil_div(f.p.m, f.tile) * f.tile);
     f.p.np = (int32_t)(ceil_div(f.p.n, f.tile) * f.tile);
     f.p.x_size = (int64_t)f.p.mp * f.p.np * 2;
@@ -148,16 +159,22 @@ orth_form orth_plan(const dl_orth_shape* s) {
     // Of a product with few tiles in the staged kernels the direct one may be the faster: 0.27 us a step of 64 x 64 tiles against 64 rows
     // from the caches for every 32 x 32 tile, at 10 TB/s, and 3 us more where the sum is split.
     auto direct = [&](int64_t k) {
-        const int64_t t64 = f.p.mp / 64 * (f.p.mp / 64 + 1) / 2 * s->batch, t32 = f.p.mp / 32 * (f.p.mp / 32 + 1) / 2 * s->batch;
+        const int64_t t64 = f.p.mp / 64 * (f.p.mp / 64 + 1) / 2, t32 = f.p.mp / 32 * (f.p.mp / 32 + 1) / 2;
         return f.tile == 32 || (double)ceil_div(t64, 512) * (double)(k / 32) * 0.27 > (double)t32 * 64 * (double)k * 4 * 1e-7 + 3;
     };
     f.gram_direct = direct(f.p.np);
     f.poly_direct = direct(f.p.mp);
     // A workgroup per CU and two steps for each of its eight waves; not worth the way through memory below some hundred steps.
-    const int64_t tri = f.p.mp / 32 * (f.p.mp / 32 + 1) / 2 * s->batch, steps = f.p.np / 32;
+    const int64_t tri = f.p.mp / 32 * (f.p.mp / 32 + 1) / 2, steps = f.p.np / 32;
     f.splits = f.gram_direct && steps >= 128 ? std::max<int64_t>(1, std::min<int64_t>({ceil_div(256, tri), steps / 16, 64})) : 1;
-    f.counters = f.splits > 1 ? tri : 0;
+    f.counters = f.splits > 1 ? s->batch * tri : 0;
     f.head = ceil_div(s->batch * f.p.partials * 8 + f.counters * 4, 256) * 256;
+    if (f.slab) {          // the head, X and two sets of sums
+        f.x_bytes = s->batch * f.n_slabs * f.slab_rows * 16 * f.slab_cols * 4;
+        f.a_bytes = s->batch * f.n_slabs * (f.slab_rows * (f.slab_rows + 1) / 2) * 1024;
+        f.bytes = f.head + f.x_bytes + 2 * f.a_bytes;
+        return f;
+    }
     f.bytes = f.head + f.counters * f.splits * 4096 + 3 * f.x_bytes + 2 * f.a_bytes;
     return f;
 }
@@ -327,27 +344,37 @@ int dl_orth_update(const dl_orth_shape* s, const void* grad, const float* moment
     const orth_form f = orth_plan(s);
     hipStream_t st = (hipStream_t)stream;
     const bool flat = s->grad_r == s->cols && (!momentum || (s->momentum_r == s->cols && s->momentum_out_r == s->cols));          // one row as good as many
+    const dlo::source src{grad, s->grad_type, momentum, momentum_out, (float)s->beta, s->nesterov, s->grad_b, s->grad_r, s->momentum_b, s->momentum_r, s->momentum_out_b, s->momentum_out_r};
+    const dlo::small sp{src, f.p.m, f.p.n, s->steps, f.turned, flat && (!weight || s->weight_r == s->cols) && s->out_r == s->cols, (float)s->a, (float)s->b, (float)s->c,
+                        out, weight, s->out_type, s->weight_type, s->out_b, s->out_r, s->weight_b, s->weight_r, (float)s->weight_keep, (float)s->gain};
     if (f.small) {
-        dlo::small p{{grad, s->grad_type, momentum, momentum_out, (float)s->beta, s->nesterov, s->grad_b, s->grad_r, s->momentum_b, s->momentum_r, s->momentum_out_b, s->momentum_out_r},
-                     f.p.m, f.p.n, s->steps, f.turned, flat && (!weight || s->weight_r == s->cols) && s->out_r == s->cols, (float)s->a, (float)s->b, (float)s->c, out, weight, s->out_type, s->weight_type,
-                     s->out_b, s->out_r, s->weight_b, s->weight_r,
-                     (float)s->weight_keep, (float)s->gain};
         const unsigned batch = (unsigned)s->batch;
-        if (f.p.m > 32) dlo::k_orth_small<4, 2><<<batch, 512, 0, st>>>(p);
-        else if (f.p.m <= 16 && f.p.n <= 256) dlo::k_orth_small<1, 2><<<batch, 512, 0, st>>>(p);
-        else if (f.p.m <= 16 && f.p.n <= 512) dlo::k_orth_small<1, 4><<<batch, 512, 0, st>>>(p);
-        else if (f.p.m <= 16) dlo::k_orth_small<1, 8><<<batch, 512, 0, st>>>(p);
-        else if (f.p.n <= 256) dlo::k_orth_small<2, 2><<<batch, 512, 0, st>>>(p);
-        else if (f.p.n <= 512) dlo::k_orth_small<2, 4><<<batch, 512, 0, st>>>(p);
-        else dlo::k_orth_small<2, 8><<<batch, 512, 0, st>>>(p);
+        if (f.p.m > 32) dlo::k_orth_small<4, 2><<<batch, 512, 0, st>>>(sp);
+        else if (f.p.m <= 16 && f.p.n <= 256) dlo::k_orth_small<1, 2><<<batch, 512, 0, st>>>(sp);
+        else if (f.p.m <= 16 && f.p.n <= 512) dlo::k_orth_small<1, 4><<<batch, 512, 0, st>>>(sp);
+        else if (f.p.m <= 16) dlo::k_orth_small<1, 8><<<batch, 512, 0, st>>>(sp);
+        else if (f.p.n <= 256) dlo::k_orth_small<2, 2><<<batch, 512, 0, st>>>(sp);
+        else dlo::k_orth_small<2, 4><<<batch, 512, 0, st>>>(sp);
         return launched("dl_orth_update");
     }
     double* partials = (double*)workspace;
     uint32_t* counters = (uint32_t*)(partials + s->batch * f.p.partials);
     float* parts = (float*)((char*)workspace + f.head);
     char* work = (char*)parts + f.counters * f.splits * 4096;
-    const dlo::source src{grad, s->grad_type, momentum, momentum_out, (float)s->beta, s->nesterov, s->grad_b, s->grad_r, s->momentum_b, s->momentum_r, s->momentum_out_b, s->momentum_out_r};
     dlo::k_orth_norm<<<dim3((unsigned)f.p.partials, (unsigned)s->batch), 256, 0, st>>>(src, flat ? 1 : s->rows, flat ? s->rows * s->cols : s->cols, partials, counters, (int)f.counters);
+    if (f.slab) {
+        char* at = (char*)workspace + f.head;
+        dlo::slabs sl{partials, f.p.partials, (float*)at, {(float*)(at + f.x_bytes), (float*)(at + f.x_bytes + f.a_bytes)}, 0};
+        dlo::small p = sp;
+        p.flat = f.turned && sp.flat;          // (a slab of the caller's rows is one piece, one of columns is not)
+        const dim3 grid((unsigned)s->batch, (unsigned)f.n_slabs);
+        for (; sl.step <= s->steps; ++sl.step) {
+            if (f.slab_rows == 1) dlo::k_orth_slab<1, 4><<<grid, 512, 0, st>>>(p, sl);
+            else if (f.slab_rows == 2) dlo::k_orth_slab<2, 4><<<grid, 512, 0, st>>>(p, sl);
+            else dlo::k_orth_slab<4, 2><<<grid, 512, 0, st>>>(p, sl);
+        }
+        return launched("dl_orth_update");
+    }
     dlo::k_orth_load<<<dim3((unsigned)ceil_div(f.p.np, 64), (unsigned)ceil_div(f.p.mp, 64), (unsigned)s->batch), 256, 0, st>>>(src, f.p, f.turned, partials, (_Float16*)work, (_Float16*)(work + f.x_bytes));
     dlo::product p{};
     p.a = (float)s->a; p.b = (float)s->b; p.c = (float)s->c;

@@ -565,9 +565,9 @@ __global__ __launch_bounds__(256, 1) void k_orth_wide(product p) {
 // ---- the same products where there are too few tiles, or too few steps along k, to fill the chip with staged ones ----------------------
 // One 32 x 32 tile per workgroup, eight waves take every eighth step along k straight from memory: all their loads are on the way at
 // once, nothing is staged and nothing waited for but the sum over the waves.  Every element comes from the L2 cache 32 times
-// (m n k / 4 bytes in all), which is what bounds it from some 600^3 on.
+// (m n k / 4 bytes in all), which is what bounds it from some 800^3 on.
 // A = X X' of a short and long X has few tiles and many steps: they are split over workgroups, and the last of a tile's to finish sums
-// what all have left, in their order, not in that of their coming (8 x 8000, all five steps: 157 -> @@ us).
+// what all have left, in their order, not in that of their coming (100 x 8000, all five steps: 208 -> 126 us).
 template <int MODE>
 __global__ __launch_bounds__(512) void k_orth_direct(product p) {
     constexpr int WAVES = 8;
@@ -708,7 +708,7 @@ template <int NP> struct cells {
 };
 
 template <int NP, int AT_ONCE>
-__device__ __forceinline__ double way_in(const small& p, const cells<NP>& cell, int rows_used) {
+__device__ __forceinline__ double way_in(const small& p, const cells<NP>& cell, int rows_used, bool first) {
     const int64_t b = blockIdx.x;
     const int rows = p.flat ? 1 : p.turned ? p.n : p.m, cols = p.flat ? p.m * p.n : p.turned ? p.m : p.n, per = (cols + 3) / 4;
     if (p.m < rows_used || p.n < NP) {
@@ -723,12 +723,12 @@ __device__ __forceinline__ double way_in(const small& p, const cells<NP>& cell, 
             const int f = e + k * 512, r = p.flat ? 0 : f / per;
             at[k].b = b; at[k].r = r; at[k].c = (f - r * per) * 4;
             at[k].n = f < rows * per ? min(4, cols - (int)at[k].c) : 0;
-            at[k].load(p.s, true);
+            at[k].load(p.s, first);
         }
 #pragma unroll
         for (int k = 0; k < AT_ONCE; ++k) {
             if (at[k].n <= 0) continue;
-            at[k].move(p.s, true);
+            at[k].move(p.s, first);
             cell.four(p.flat, (int)at[k].r, (int)at[k].c, [&](int t, float& to) {
                 if (t < at[k].n) to = at[k].u[t];
                 sum += (double)at[k].u[t] * at[k].u[t];
@@ -772,33 +772,15 @@ __device__ __forceinline__ void way_out(const small& p, const cells<NP>& cell) {
     }
 }
 
-template <int RB, int JB>
-__global__ __launch_bounds__(512) void k_orth_small(small p) {
-    constexpr int WAVES = 8, NP = WAVES * JB * 16, KB = JB / 2, S = RB == 1 ? 1 : RB / 2, TILES = RB * (RB + 1) / 2;
-    __shared__ __attribute__((aligned(16))) _Float16 xr[WAVES][RB][KB][FRAG];
-    __shared__ __attribute__((aligned(16))) float red[RB == 1 ? 2 : 1][WAVES][TILES][256];          // (RB = 1: every other step the other one)
-    __shared__ __attribute__((aligned(16))) _Float16 am[RB == 1 ? 1 : RB][S][RB == 1 ? 8 : FRAG];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), q = lane >> 4, c = lane & 15;
-    const cells<NP> cell((float*)&xr[0][0][0][0], p);
-    double sum = way_in<NP, 8>(p, cell, RB * 16);
-    double* sums = (double*)red;
-    if (lane == 0) sums[wave] = sum;
-    __syncthreads();
-    sum = 0.0;
-    for (int w = 0; w < WAVES; ++w) sum += sums[w];
-    float x[JB][RB][4];
-    const double inv = sum != 0.0 ? (double)SCALE / sqrt(sum) : 0.0;          // (NaN != 0)
-#pragma unroll
-    for (int jb = 0; jb < JB; ++jb)
-#pragma unroll
-        for (int I = 0; I < RB; ++I)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) x[jb][I][r] = (float)(cell(16 * I + 4 * q + r, (wave * JB + jb) * 16 + c) * inv);
-    __syncthreads();
+// The arithmetic of a step on x, a lane's part of X (times SCALE) in the layout of the results.
+template <int RB, int JB> struct rowwise {
+    static constexpr int NWAVES = 8, NP = NWAVES * JB * 16, KB = JB / 2, S = RB == 1 ? 1 : RB / 2, TILES = RB * (RB + 1) / 2;
+    typedef _Float16 columns[NWAVES][RB][KB][FRAG];          // X over columns, a part for each wave
+    typedef float sums[NWAVES][TILES][256];                  // the tiles of A, as each wave has them
+    typedef _Float16 matrix_[RB == 1 ? 1 : RB][S][RB == 1 ? 8 : FRAG];
+    struct operand { half8 h[JB][S], l[JB][S]; };            // X over rows
 
-    for (int step = 0; step < p.steps; ++step) {
-        // X as operands: over rows in registers, over columns through LDS (this wave's part only)
-        half8 xh[JB][S], xl[JB][S];
+    template <bool STORE> static __device__ __forceinline__ void operands(const float (&x)[JB][RB][4], operand& o, columns& xr, int wave, int q, int c) {
 #pragma unroll
         for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
@@ -807,13 +789,19 @@ __global__ __launch_bounds__(512) void k_orth_small(small p) {
                 for (int r = 0; r < 4; ++r) {
                     _Float16 h, l;
                     split(x[jb][I][r], h, l);
-                    xh[jb][I / 2][(I & 1) * 4 + r] = h;
-                    xl[jb][I / 2][(I & 1) * 4 + r] = l;
-                    _Float16* to = &xr[wave][I][jb / 2][(4 * q + r + 16 * ((jb & 1) * 2 + (c >> 3))) * 8 + (c & 7)];
-                    to[0] = h;
-                    to[512] = l;
+                    o.h[jb][I / 2][(I & 1) * 4 + r] = h;
+                    o.l[jb][I / 2][(I & 1) * 4 + r] = l;
+                    if constexpr (STORE) {
+                        _Float16* to = &xr[wave][I][jb / 2][(4 * q + r + 16 * ((jb & 1) * 2 + (c >> 3))) * 8 + (c & 7)];
+                        to[0] = h;
+                        to[512] = l;
+                    }
                 }
-        float4_ acc[TILES] = {};
+    }
+    // this wave's part of A, from its own part of xr
+    static __device__ __forceinline__ void gram(float4_ (&acc)[TILES], const columns& xr, int wave, int lane) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) acc[t] = float4_{};
 #pragma unroll
         for (int k = 0; k < KB; ++k) {
             half8 ph[RB], pl[RB];
@@ -829,13 +817,21 @@ __global__ __launch_bounds__(512) void k_orth_small(small p) {
                     t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph[I], ph[J], t, 0, 0, 0);
                 }
         }
+    }
+    static __device__ __forceinline__ float4_ total(const sums& red, int t, int lane) {
+        float4_ v = {};
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) *(float4_*)&red[RB == 1 ? step & 1 : 0][wave][t][lane * 4] = acc[t];
+        for (int w = 0; w < NWAVES; ++w) v += *(const float4_*)&red[w][t][lane * 4];
+        return v;
+    }
+    // X = a X + (b A + c A A) X, A from everyone's sums: one barrier, and with RB > 1 a second one inside
+    static __device__ __forceinline__ void update(const small& p, float (&x)[JB][RB][4], const operand& o, const float4_ (&acc)[TILES], sums& red, matrix_& am, int wave, int lane) {
+        const int q = lane >> 4, c = lane & 15;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) *(float4_*)&red[wave][t][lane * 4] = acc[t];
         __syncthreads();
         if constexpr (RB == 1) {
-            float4_ a = {};
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) a += *(const float4_*)&red[step & 1][w][0][lane * 4];
+            const float4_ a = total(red, 0, lane);
             half4 ah, al, qh, ql;
 #pragma unroll
             for (int r = 0; r < 4; ++r) { _Float16 h, l; split(a[r] * (1.0f / SCALE), h, l); ah[r] = h; al[r] = l; }
@@ -851,7 +847,7 @@ __global__ __launch_bounds__(512) void k_orth_small(small p) {
             }
 #pragma unroll
             for (int jb = 0; jb < JB; ++jb) {
-                const half4 h = __builtin_shufflevector(xh[jb][0], xh[jb][0], 0, 1, 2, 3), l = __builtin_shufflevector(xl[jb][0], xl[jb][0], 0, 1, 2, 3);
+                const half4 h = __builtin_shufflevector(o.h[jb][0], o.h[jb][0], 0, 1, 2, 3), l = __builtin_shufflevector(o.l[jb][0], o.l[jb][0], 0, 1, 2, 3);
                 float4_ y = {};
                 y = __builtin_amdgcn_mfma_f32_16x16x16f16(qh, l, y, 0, 0, 0);
                 y = __builtin_amdgcn_mfma_f32_16x16x16f16(ql, h, y, 0, 0, 0);
@@ -859,79 +855,189 @@ __global__ __launch_bounds__(512) void k_orth_small(small p) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) x[jb][0][r] = fmaf(p.a, x[jb][0][r], y[r] * (1.0f / SCALE));
             }
-            continue;
         } else {
-        for (int t = wave; t < TILES; t += WAVES) {          // a wave sums a tile and writes it, and its mirror image, as operands
-            float4_ v = {};
-            for (int w = 0; w < WAVES; ++w) v += *(const float4_*)&red[0][w][t][lane * 4];
-            int I = 0;
-            while ((I + 1) * (I + 2) / 2 <= t) ++I;
-            const int J = t - I * (I + 1) / 2;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                _Float16 h, l;
-                split(v[r] * (1.0f / SCALE), h, l);
-                const int i = 16 * I + 4 * q + r, j = 16 * J + c;
-                _Float16* to = &am[J][i >> 5][(c + 16 * ((i & 31) >> 3)) * 8 + (i & 7)];
-                to[0] = h; to[512] = l;
-                if (I != J) {
-                    to = &am[I][j >> 5][(4 * q + r + 16 * ((j & 31) >> 3)) * 8 + (j & 7)];
-                    to[0] = h; to[512] = l;
-                }
-            }
-        }
-        __syncthreads();
-        half8 ah[RB][S], al[RB][S], qh[RB][S], ql[RB][S];
-#pragma unroll
-        for (int I = 0; I < RB; ++I)
-#pragma unroll
-            for (int k = 0; k < S; ++k) { ah[I][k] = *(const half8*)&am[I][k][lane * 8]; al[I][k] = *(const half8*)&am[I][k][512 + lane * 8]; }
-#pragma unroll
-        for (int J = 0; J < RB; ++J)
-#pragma unroll
-            for (int I = 0; I < RB; ++I) {
-                float4_ t = {};
-#pragma unroll
-                for (int k = 0; k < S; ++k) {
-                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[I][k], al[J][k], t, 0, 0, 0);
-                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[I][k], ah[J][k], t, 0, 0, 0);
-                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[I][k], ah[J][k], t, 0, 0, 0);
-                }
-                const int i = 16 * I + 4 * q;          // A[i + r][16 J + c] lies as row 16 J + c, columns i + r
-                const _Float16* from = &am[J][i >> 5][(c + 16 * ((i & 31) >> 3)) * 8 + (i & 7)];
+            for (int t = wave; t < TILES; t += NWAVES) {          // a wave sums a tile and writes it, and its mirror image, as operands
+                const float4_ v = total(red, t, lane);
+                int I = 0;
+                while ((I + 1) * (I + 2) / 2 <= t) ++I;
+                const int J = t - I * (I + 1) / 2;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     _Float16 h, l;
-                    split(fmaf(p.c, t[r] * (1.0f / SCALE), p.b * ((float)from[r] + (float)from[512 + r])), h, l);
-                    qh[J][I / 2][(I & 1) * 4 + r] = h;
-                    ql[J][I / 2][(I & 1) * 4 + r] = l;
+                    split(v[r] * (1.0f / SCALE), h, l);
+                    const int i = 16 * I + 4 * q + r, j = 16 * J + c;
+                    _Float16* to = &am[J][i >> 5][(c + 16 * ((i & 31) >> 3)) * 8 + (i & 7)];
+                    to[0] = h; to[512] = l;
+                    if (I != J) {
+                        to = &am[I][j >> 5][(4 * q + r + 16 * ((j & 31) >> 3)) * 8 + (j & 7)];
+                        to[0] = h; to[512] = l;
+                    }
                 }
             }
+            __syncthreads();
+            half8 ah[RB][S], al[RB][S], qh[RB][S], ql[RB][S];
+#pragma unroll
+            for (int I = 0; I < RB; ++I)
+#pragma unroll
+                for (int k = 0; k < S; ++k) { ah[I][k] = *(const half8*)&am[I][k][lane * 8]; al[I][k] = *(const half8*)&am[I][k][512 + lane * 8]; }
+#pragma unroll
+            for (int J = 0; J < RB; ++J)
+#pragma unroll
+                for (int I = 0; I < RB; ++I) {
+                    float4_ t = {};
+#pragma unroll
+                    for (int k = 0; k < S; ++k) {
+                        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[I][k], al[J][k], t, 0, 0, 0);
+                        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[I][k], ah[J][k], t, 0, 0, 0);
+                        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[I][k], ah[J][k], t, 0, 0, 0);
+                    }
+                    const int i = 16 * I + 4 * q;          // A[i + r][16 J + c] lies as row 16 J + c, columns i + r
+                    const _Float16* from = &am[J][i >> 5][(c + 16 * ((i & 31) >> 3)) * 8 + (i & 7)];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        _Float16 h, l;
+                        split(fmaf(p.c, t[r] * (1.0f / SCALE), p.b * ((float)from[r] + (float)from[512 + r])), h, l);
+                        qh[J][I / 2][(I & 1) * 4 + r] = h;
+                        ql[J][I / 2][(I & 1) * 4 + r] = l;
+                    }
+                }
+#pragma unroll
+            for (int jb = 0; jb < JB; ++jb)
+#pragma unroll
+                for (int I = 0; I < RB; ++I) {
+                    float4_ t = {};
+#pragma unroll
+                    for (int k = 0; k < S; ++k) {
+                        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[I][k], o.l[jb][k], t, 0, 0, 0);
+                        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[I][k], o.h[jb][k], t, 0, 0, 0);
+                        t = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[I][k], o.h[jb][k], t, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[jb][I][r] = fmaf(p.a, x[jb][I][r], t[r] * (1.0f / SCALE));
+                }
+        }
+    }
+    // between the caller's order and the lanes'
+    static __device__ __forceinline__ void pick(float (&x)[JB][RB][4], const cells<NP>& cell, double inv, int wave, int q, int c) {
 #pragma unroll
         for (int jb = 0; jb < JB; ++jb)
 #pragma unroll
-            for (int I = 0; I < RB; ++I) {
-                float4_ t = {};
+            for (int I = 0; I < RB; ++I)
 #pragma unroll
-                for (int k = 0; k < S; ++k) {
-                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[I][k], xl[jb][k], t, 0, 0, 0);
-                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[I][k], xh[jb][k], t, 0, 0, 0);
-                    t = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[I][k], xh[jb][k], t, 0, 0, 0);
-                }
+                for (int r = 0; r < 4; ++r) x[jb][I][r] = (float)(cell(16 * I + 4 * q + r, (wave * JB + jb) * 16 + c) * inv);
+    }
+    static __device__ __forceinline__ void put(const float (&x)[JB][RB][4], const cells<NP>& cell, int wave, int q, int c) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[jb][I][r] = fmaf(p.a, x[jb][I][r], t[r] * (1.0f / SCALE));
-            }
-        }
+        for (int jb = 0; jb < JB; ++jb)
+#pragma unroll
+            for (int I = 0; I < RB; ++I)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) cell(16 * I + 4 * q + r, (wave * JB + jb) * 16 + c) = x[jb][I][r];
+    }
+};
+
+template <int RB, int JB>
+__global__ __launch_bounds__(512) void k_orth_small(small p) {
+    typedef rowwise<RB, JB> R;
+    __shared__ __attribute__((aligned(16))) typename R::columns xr;
+    __shared__ __attribute__((aligned(16))) typename R::sums red[RB == 1 ? 2 : 1];          // (RB = 1, one barrier: every other step the other one)
+    __shared__ __attribute__((aligned(16))) typename R::matrix_ am;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), q = lane >> 4, c = lane & 15;
+    const cells<R::NP> cell((float*)&xr[0][0][0][0], p);
+    double sum = way_in<R::NP, 8>(p, cell, RB * 16, true);
+    double* sums = (double*)red;
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+    for (int w = 0; w < R::NWAVES; ++w) sum += sums[w];
+    float x[JB][RB][4];
+    R::pick(x, cell, sum != 0.0 ? (double)SCALE / sqrt(sum) : 0.0, wave, q, c);          // (NaN != 0)
+    __syncthreads();
+    for (int step = 0; step < p.steps; ++step) {
+        typename R::operand o;
+        float4_ acc[R::TILES];
+        R::template operands<true>(x, o, xr, wave, q, c);
+        R::gram(acc, xr, wave, lane);
+        R::update(p, x, o, acc, red[RB == 1 ? step & 1 : 0], am, wave, lane);
     }
     __syncthreads();          // (the last reads of xr)
-#pragma unroll
-    for (int jb = 0; jb < JB; ++jb)
-#pragma unroll
-        for (int I = 0; I < RB; ++I)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) cell(16 * I + 4 * q + r, (wave * JB + jb) * 16 + c) = x[jb][I][r];
+    R::put(x, cell, wave, q, c);
     __syncthreads();
-    way_out<NP, 8>(p, cell);
+    way_out<R::NP, 8>(p, cell);
+}
+
+// ---- short sides of up to 64 with a long one: a workgroup per 128 JB columns ("slab"), a launch per step ---------------------------------------
+// Slab s leaves its part of A behind each launch; the next one sums all slabs' parts for itself, makes Q, moves its part of X on.
+// X waits in memory between the launches, in 32 bits and in the order of the lanes.  Seven launches instead of seventeen, each bound by
+// its way to the caches and back.
+struct slabs {
+    const double* partials; int32_t n_partials;
+    float* x;                     // [batch][slab][JB * RB][512 lanes][4]
+    float* parts[2];              // [batch][slab][TILES][256]: read and written in turn
+    int32_t step;                 // 0: X from the gradient;  p.steps: the result
+};
+
+template <int RB, int JB>
+__global__ __launch_bounds__(512) void k_orth_slab(small p, slabs sl) {
+    typedef rowwise<RB, JB> R;
+    __shared__ __attribute__((aligned(16))) typename R::columns xr;
+    __shared__ __attribute__((aligned(16))) typename R::sums red;
+    __shared__ __attribute__((aligned(16))) typename R::matrix_ am;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), q = lane >> 4, c = lane & 15;
+    const int slab = blockIdx.y, n_slabs = gridDim.y, j0 = slab * R::NP;
+    const int64_t b = blockIdx.x, part = (b * n_slabs + slab) * R::TILES * 256;
+    // from here on the slab is a matrix of its own
+    p.n = min(p.n - j0, R::NP);
+    const auto at = [&](int64_t row) { return p.turned ? j0 * row : j0; };
+    const int size = p.s.dtype == 0 ? 4 : 2, w_size = p.w_type == 0 ? 4 : 2, out_size = p.out_type == 0 ? 4 : 2;
+    p.s.g = (const char*)p.s.g + at(p.s.g_r) * size;
+    if (p.s.m) p.s.m_out += at(p.s.o_r);
+    if (p.w) p.w = (const char*)p.w + at(p.w_r) * w_size;
+    p.out = (char*)p.out + at(p.out_r) * out_size;
+    const cells<R::NP> cell((float*)&xr[0][0][0][0], p);
+    float x[JB][RB][4];
+    float4_* mine = (float4_*)sl.x + (b * n_slabs + slab) * (JB * RB) * 512 + threadIdx.x;
+    typename R::operand o;
+    float4_ acc[R::TILES];
+    if (sl.step == 0) {
+        way_in<R::NP, 8>(p, cell, RB * 16, false);
+        double sum = 0.0;
+        for (int k = lane; k < sl.n_partials; k += 64) sum += sl.partials[b * sl.n_partials + k];
+        for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+        __syncthreads();
+        R::pick(x, cell, sum != 0.0 ? (double)SCALE / sqrt(sum) : 0.0, wave, q, c);
+        __syncthreads();
+    } else {
+#pragma unroll
+        for (int e = 0; e < JB * RB; ++e) {
+            const float4_ v = mine[e * 512];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[e / RB][e % RB][r] = v[r];
+        }
+        const float* from = sl.parts[(sl.step + 1) & 1] + b * n_slabs * R::TILES * 256 + lane * 4;
+#pragma unroll
+        for (int t = 0; t < R::TILES; ++t) acc[t] = float4_{};
+        for (int k = wave; k < n_slabs; k += R::NWAVES) {
+#pragma unroll
+            for (int t = 0; t < R::TILES; ++t) acc[t] += *(const float4_*)(from + ((int64_t)k * R::TILES + t) * 256);
+        }
+        R::template operands<false>(x, o, xr, wave, q, c);
+        R::update(p, x, o, acc, red, am, wave, lane);
+        if (sl.step == p.steps) {
+            R::put(x, cell, wave, q, c);
+            __syncthreads();
+            return way_out<R::NP, 8>(p, cell);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < JB * RB; ++e) mine[e * 512] = float4_{x[e / RB][e % RB][0], x[e / RB][e % RB][1], x[e / RB][e % RB][2], x[e / RB][e % RB][3]};
+    R::template operands<true>(x, o, xr, wave, q, c);
+    R::gram(acc, xr, wave, lane);
+    __syncthreads();          // (the last reads of red)
+#pragma unroll
+    for (int t = 0; t < R::TILES; ++t) *(float4_*)&red[wave][t][lane * 4] = acc[t];
+    __syncthreads();
+    for (int t = wave; t < R::TILES; t += R::NWAVES) *(float4_*)(sl.parts[sl.step & 1] + part + t * 256 + lane * 4) = R::total(red, t, lane);
 }
 
 }  // namespace dlo

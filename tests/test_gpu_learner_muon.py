@@ -59,7 +59,8 @@ def check_orthogonal(got, g, steps=5, coefficients=(3.4445, -4.7750, 2.0315), ha
 
 @pytest.mark.parametrize('dtype', TYPES, ids=str)
 @pytest.mark.parametrize('rows,cols', [(1, 1), (1, 7), (7, 1), (1, 512), (8, 512), (512, 8), (29, 512), (512, 29), (16, 16), (31, 33), (32, 32), (64, 64), (65, 63), (33, 129), (127, 128), (130, 257),
-                                       (512, 512), (300, 1000), (1000, 300)])
+                                       (512, 512), (300, 1000), (1000, 300),
+                                       (1, 5000), (5000, 1), (15, 1025), (16, 2049), (17, 513), (4000, 30), (32, 1024), (33, 257), (2500, 50), (64, 1000), (63, 9000), (90, 7000), (5000, 130)])
 def test_shapes(rows, cols, dtype):
     from drloco_amd.muon import orthogonalise
     g = gradient(rows, cols, seed=rows * 7 + cols, dtype=dtype)
@@ -119,7 +120,7 @@ def test_steps_and_coefficients(rows, cols, steps, name):
 
 
 @pytest.mark.parametrize('lead', [(3,), (2, 3), (1,), (17,)])
-@pytest.mark.parametrize('rows,cols', [(40, 70), (70, 40), (8, 300)])
+@pytest.mark.parametrize('rows,cols', [(40, 70), (70, 40), (8, 300), (20, 1100), (1100, 50), (70, 5000)])
 def test_batches(lead, rows, cols):
     from drloco_amd.muon import orthogonalise
     g = gradient(*lead, rows, cols, seed=4) * torch.logspace(-3, 3, int(np.prod(lead))).reshape(*lead, 1, 1)
@@ -137,7 +138,7 @@ def test_the_size_of_a_gradient_does_not_matter(scale):
     check_orthogonal(orthogonalise(g.cuda()), g)
 
 
-@pytest.mark.parametrize('rows,cols', [(20, 30), (30, 20), (200, 300), (1, 5)])
+@pytest.mark.parametrize('rows,cols', [(20, 30), (30, 20), (200, 300), (1, 5), (1500, 20), (100, 5000)])
 def test_zeros_stay_zero_and_bad_matrices_keep_to_themselves(rows, cols):
     from drloco_amd.muon import orthogonalise
     g = gradient(5, rows, cols, seed=6).cuda()
@@ -169,7 +170,7 @@ LAYOUTS = {'transposed': lambda g: g.t().contiguous().cuda().t(), 'wider rows': 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.float16], ids=str)
 def test_layouts(layout, dtype):
     from drloco_amd.muon import orthogonalise
-    for shape in ((45, 77), (77, 45)):
+    for shape in ((45, 77), (77, 45), (20, 1300), (1300, 40), (130, 200)):
         g = gradient(*shape, seed=7, dtype=dtype)
         placed = LAYOUTS[layout](g)
         want = orthogonalise(g.cuda())
@@ -196,7 +197,7 @@ def test_in_place_and_destinations():
 
 @pytest.mark.parametrize('wt', TYPES, ids=str)
 @pytest.mark.parametrize('gt', TYPES, ids=str)
-@pytest.mark.parametrize('rows,cols', [(29, 40), (512, 29), (130, 200)])
+@pytest.mark.parametrize('rows,cols', [(29, 40), (512, 29), (130, 200), (29, 1500), (2000, 50)])
 def test_the_update(rows, cols, wt, gt):
     from drloco_amd.muon import muon_update
     w, g, m = gradient(rows, cols, seed=1, dtype=wt, scale=0.1), gradient(rows, cols, seed=2, dtype=gt), gradient(rows, cols, seed=3)
@@ -275,7 +276,7 @@ def test_the_policy_sees_updated_weights():
     assert (a - ra).abs().max() < 1e-4 and (v - rv).abs().max() < 1e-4
 
 
-@pytest.mark.parametrize('rows,cols', [(8, 40), (130, 200)])
+@pytest.mark.parametrize('rows,cols', [(8, 40), (130, 200), (20, 1500), (100, 6000)])
 def test_a_captured_update_replays(rows, cols):
     from drloco_amd.muon import muon_update
     w, g, m = (gradient(rows, cols, seed=s).cuda() for s in (1, 2, 3))
@@ -299,7 +300,7 @@ def test_a_captured_update_replays(rows, cols):
 
 def test_two_updates_on_two_streams():
     from drloco_amd.muon import orthogonalise
-    g = [gradient(300, 500, seed=s).cuda() for s in (1, 2)]
+    g = [gradient(*shape, seed=s).cuda() for s, shape in ((1, (100, 6000)), (2, (110, 7000)))]          # (sums split over workgroups)
     want = [orthogonalise(t) for t in g]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream(), torch.cuda.Stream()]
