@@ -25,6 +25,8 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 bool aligned(const void* p, int64_t bytes) { return ((uintptr_t)p % (uintptr_t)bytes) == 0; }
 int elem_bytes(int dtype) { return dtype == DL_F32 ? 4 : 2; }
 
+bool fits(int64_t blocks, int64_t threads) { return blocks <= 0xffffffff / threads; }          // a launch has less than 2^32 threads
+
 // ---- gated memory ----
 constexpr int64_t MAX_DIM = (int64_t)1 << 40;
 
@@ -258,7 +260,7 @@ int dl_memory_forward(const dl_memory_shape* s, const void* x, const void* gate,
     const form f = memory_plan(s, widest_forward(s->dtype));
     if (f.chunks > 1 && !workspace) return fail(DL_E_INVAL, "dl_memory_forward: workspace must not be NULL (dl_memory_workspace_bytes)");
     if (!aligned(workspace, 16)) return fail(DL_E_INVAL, "dl_memory_forward: workspace must be aligned to 16 bytes");
-    if (f.blocks * f.chunks > 0x7fffffff) return fail(DL_E_INVAL, "dl_memory_forward: T * N * D too large");
+    if (!fits(f.blocks * f.chunks, 64 * f.W)) return fail(DL_E_INVAL, "dl_memory_forward: T * N * D too large");
     const dlm::shape d = device_shape(s, f);
     const unsigned grid = (unsigned)(f.blocks * f.chunks);
     hipStream_t st = (hipStream_t)stream;
@@ -290,7 +292,7 @@ int dl_memory_backward(const dl_memory_shape* s, const void* x, const void* gate
     const form f = memory_plan(s, widest_back(s->dtype));
     if (f.chunks > 1 && !workspace) return fail(DL_E_INVAL, "dl_memory_backward: workspace must not be NULL (dl_memory_workspace_bytes)");
     if (!aligned(workspace, 16)) return fail(DL_E_INVAL, "dl_memory_backward: workspace must be aligned to 16 bytes");
-    if (f.blocks * f.chunks > 0x7fffffff) return fail(DL_E_INVAL, "dl_memory_backward: T * N * D too large");
+    if (!fits(f.blocks * f.chunks, 64 * f.W)) return fail(DL_E_INVAL, "dl_memory_backward: T * N * D too large");
     const dlm::shape d = device_shape(s, f);
     const unsigned grid = (unsigned)(f.blocks * f.chunks);
     hipStream_t st = (hipStream_t)stream;
@@ -318,7 +320,7 @@ int dl_memory_step(const dl_memory_shape* s, const void* x, const void* gate, co
     int V = widest_forward(s->dtype);
     while (s->D % V) V /= 2;
     const int64_t blocks = ceil_div(s->N * (s->D / V), 256);
-    if (blocks > 0x7fffffff) return fail(DL_E_INVAL, "dl_memory_step: N * D too large");
+    if (!fits(blocks, 256)) return fail(DL_E_INVAL, "dl_memory_step: N * D too large");
     with_type(s->dtype, [&](auto e) { with_width<widest<decltype(e)>()>(V, [&](auto v) {
         using E = decltype(e);
         constexpr int V_ = decltype(v)::value;

@@ -68,6 +68,16 @@ def test_bad_shapes_are_refused_by_every_c_entry(L, bad):
     assert len(L.dl_learner_last_error()) > 5
 
 
+def test_launches_of_too_many_threads_are_refused(L):
+    p = 4096          # never read: the checks come first
+    for n in (1 << 33, (1 << 32) + 256, 1 << 40):          # a lane per walker: 2^32 and more of them
+        s = C.byref(shape(T=1, N=n, D=1, x_t=0, x_n=1, gate_t=0, gate_n=1, starts_t=0, grad_t=0, grad_n=1))
+        assert L.dl_memory_forward(s, p, p, None, None, p, None, None, p, None) == -1
+        assert L.dl_memory_backward(s, p, p, None, p, p, None, p, p, None, p, None) == -1
+        assert L.dl_memory_step(s, p, p, None, p, p, p, None) == -1
+        assert b'too large' in L.dl_learner_last_error()
+
+
 def test_null_pointers_are_refused(L):
     s, p = C.byref(shape()), 4096
     assert L.dl_memory_workspace_bytes(None) == -1
