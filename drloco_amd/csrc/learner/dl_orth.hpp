@@ -440,14 +440,14 @@ __device__ __forceinline__ void wide_tile(const product& p, int i0, int j0, char
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
                 float4_& sum = COARSE ? acc[i][j] : small[i][j];
-                sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(COARSE ? r.l : r.h, col[j].l, sum, 0, 0, 0);
+                sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(r.h, COARSE ? col[j].h : col[j].l, sum, 0, 0, 0);          // (coarse: the earlier of the two steps first, as in product_tile)
             }
             if constexpr (!COARSE) {
 #pragma unroll
                 for (int j = 0; j < TN; ++j) small[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(r.l, col[j].h, small[i][j], 0, 0, 0);
             }
 #pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(r.h, col[j].h, acc[i][j], 0, 0, 0);
+            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(COARSE ? r.l : r.h, COARSE ? col[j].l : col[j].h, acc[i][j], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
         const int was = now;

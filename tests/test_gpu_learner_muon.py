@@ -363,3 +363,14 @@ def test_a_recurrent_policy_learns_through_both():
         scale = 0.02 * np.sqrt(max(1, w.shape[0] / w.shape[1]))
         check_orthogonal((w - p.detach().cpu()) / scale, torch.from_numpy(1.95 * g), half_step=2.0 ** -23 * np.linalg.norm(np64(w)) / scale + 4.0 ** 5 * 2.0 ** -23)
         assert np.linalg.norm(np64(p) - want) < 1e-4 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize('batch,rows,cols', [(4, 1024, 2048), (2, 1031, 4099), (7, 900, 1100), (20, 512, 512), (3, 2000, 130), (9, 100, 8000), (16, 833, 833)])
+def test_a_matrix_has_the_same_result_in_any_stack(batch, rows, cols, dtype):
+    """The tiles' sizes change with the number of matrices (4 x 1024 x 2048 fills the chip with the largest, one does not), the order of an element's sums does not."""
+    from drloco_amd.muon import orthogonalise
+    g = gradient(batch, rows, cols, seed=8, dtype=dtype).cuda()
+    o = orthogonalise(g)
+    for k in range(batch):
+        assert torch.equal(o[k], orthogonalise(g[k]))
