@@ -374,3 +374,18 @@ def test_a_matrix_has_the_same_result_in_any_stack(batch, rows, cols, dtype):
     o = orthogonalise(g)
     for k in range(batch):
         assert torch.equal(o[k], orthogonalise(g[k]))
+
+
+def test_the_training_example_runs_with_muon():
+    """Two updates of examples/train_ppo.py: it runs, every weight is finite, the trunk's matrices have moved (nothing is said of the loss)."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'examples', 'train_ppo.py')
+    spec = importlib.util.spec_from_file_location('train_ppo', path)
+    mod = importlib.util.module_from_spec(spec); spec.loader.exec_module(mod)
+    args = dict(n_envs=64, batch=512, minibatch=256, epochs=1, seed=1, log_every=1, quiet=True, return_objects=True, optimizer='muon')
+    one, two = (mod.train(mio=mio, **args)[1] for mio in (600e-6, 1100e-6))
+    for name in ('w1', 'b1', 'w2', 'b2', 'wa', 'ba', 'wv', 'bv', 'log_std'):
+        assert torch.isfinite(getattr(two, name)).all(), name
+    for name in ('w1', 'w2', 'wa', 'wv'):
+        assert not torch.equal(getattr(one, name), getattr(two, name)), name
