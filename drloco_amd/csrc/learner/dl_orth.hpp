@@ -112,7 +112,7 @@ struct place {
 };
 
 // rows x cols as they are read: one long row where the rows of all arrays follow each other
-// (and counters for later kernels to zero)
+// (and counters for later kernels to zero).  4096 x 8192 bf16: 67 MB in 32 us, 2.1 TB/s, half of what memory gives; 0.6 % of the update.
 __global__ __launch_bounds__(256) void k_orth_norm(source s, int64_t rows, int64_t cols, double* __restrict__ partials, uint32_t* __restrict__ counters, int n_counters) {
     if (blockIdx.x == 0 && blockIdx.y == 0) for (int k = threadIdx.x; k < n_counters; k += 256) counters[k] = 0;
     constexpr int AT_ONCE = 4;
@@ -141,6 +141,7 @@ __global__ __launch_bounds__(256) void k_orth_norm(source s, int64_t rows, int64
 }
 
 // ---- X = G / |G| into both orientations: one workgroup per 64 x 64 ---------------------------------------------------------------
+// 4096 x 8192 bf16: 335 MB in 80 us, 4.2 TB/s; bound by memory.
 __global__ __launch_bounds__(256) void k_orth_load(source s, plan p, int turned, const double* __restrict__ partials, _Float16* __restrict__ xr, _Float16* __restrict__ xc) {
     const int b = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     __shared__ float tile[64][65];          // [short side][long side]
@@ -496,7 +497,8 @@ __device__ __forceinline__ void wide_tile(const product& p, int i0, int j0, char
 
 // Tiles of 128 x 128, two workgroups per CU; those that would be left for a last round that fills less than two thirds of the chip are
 // cut into four.  Workgroups go round the eight dies by their index: each die gets a run of neighbouring tiles, so that its L2 cache
-// serves their common operands.
+// serves their common operands.  2 x 1031 x 4099: A 55, Q 19, Q X 65 us, the latter 815 TFLOP/s of 16-bit products (1031 is padded to 1152,
+// and its last round is short).
 template <int MODE, bool COARSE>
 __global__ __launch_bounds__(256, 2) void k_orth_product(product p) {
     typedef staged<128, 128, 64, 64, 2> big;
@@ -525,7 +527,8 @@ __global__ __launch_bounds__(256, 2) void k_orth_product(product p) {
 
 // Tiles of 256 x 128, one workgroup per CU, for results that fill the chip with them.  A wave's 128 x 64 need 24 reads of LDS for 96
 // products; with 64 x 64 it is 16 for 48, and LDS is what they wait for.  `whole` tiles, the rest of them in 64 x 64, and 64 x 64 for
-// the last 128 rows where the padded short side is an odd multiple of 128.
+// the last 128 rows where the padded short side is an odd multiple of 128.  4096 x 8192: A 363, Q 193, Q X 630 us, the latter 1310 TFLOP/s of
+// 16-bit products, the rate of the library's large product of 16-bit matrices: bound by the matrix cores (and by what power they may draw).
 template <int MODE, bool COARSE>
 __global__ __launch_bounds__(256, 1) void k_orth_wide(product p) {
     typedef staged<256, 128, 128, 64, 3> big;
@@ -568,6 +571,7 @@ __global__ __launch_bounds__(256, 1) void k_orth_wide(product p) {
 // (m n k / 4 bytes in all), which is what bounds it from some 800^3 on.
 // A = X X' of a short and long X has few tiles and many steps: they are split over workgroups, and the last of a tile's to finish sums
 // what all have left, in their order, not in that of their coming (100 x 8000, all five steps: 208 -> 126 us).
+// 512 x 512: 5 to 7 us a product, of which the launch and the sum over the waves are the most.
 template <int MODE>
 __global__ __launch_bounds__(512) void k_orth_direct(product p) {
     constexpr int WAVES = 8;
@@ -679,7 +683,7 @@ __global__ __launch_bounds__(512) void k_orth_direct(product p) {
 // stand: X goes from step to step in registers, and Q, being symmetric, is one as it comes out (with RB = 1 the products over rows
 // are those of 16 k's, whose operand is a result as it stands, A too).  Only A = X X', which sums over columns, reads X in its other
 // orientation, from the wave's own part of LDS.  X itself stays in 32 bits: here Q is without its a I, and X = a X + Q X.  Two barriers per step, one with RB = 1, where A's parts are summed.
-// Bound by the instructions of one CU, some 450 per wave and step with RB = 2, JB = 4, and by the way in and out.
+// Bound by the instructions of one CU, some 450 per wave and step with RB = 2, JB = 4, and by the way in and out.  8 x 512: 13.4 us, 512 x 29 with momentum and weight: 28.5.
 struct small {
     source s;
     int32_t m, n, steps, turned, flat;          // flat: the rows of every array follow each other, they are read as one
@@ -969,7 +973,7 @@ __global__ __launch_bounds__(512) void k_orth_small(small p) {
 // ---- short sides of up to 64 with a long one: a workgroup per 128 JB columns ("slab"), a launch per step ---------------------------------------
 // Slab s leaves its part of A behind each launch; the next one sums all slabs' parts for itself, makes Q, moves its part of X on.
 // X waits in memory between the launches, in 32 bits and in the order of the lanes.  Seven launches instead of seventeen, each bound by
-// its way to the caches and back.
+// its way to the caches and back.  All five steps of 8 x 8000: 34 us (157 with a launch per product), 30 x 8000: 52, 8 x 100000: 72.
 struct slabs {
     const double* partials; int32_t n_partials;
     float* x;                     // [batch][slab][JB * RB][512 lanes][4]
