@@ -101,7 +101,8 @@ def muon_update(weight, grad, momentum, lr, beta=0.95, nesterov=True, weight_dec
 class HipMuon(torch.optim.Optimizer):
     """Muon for the weight matrices of a policy, each step one muon_update in place per matrix.  Parameters need at least two axes, contiguous,
     on a HIP device; everything else (biases, log_std, usually the first and the last layer) belongs to another optimiser.
-    With walkers sharded over GPUs the gradients are summed over the ranks first (collectives.FlatGradAllReducer); every rank then takes the same step."""
+    With walkers sharded over GPUs the gradients are summed over the ranks first (collectives.FlatGradAllReducer); every rank then takes the same step.
+    step() can be captured into a graph after a first eager one; a replay takes the learning rate that was set at the capture."""
 
     def __init__(self, params, lr=0.02, beta=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=COEFFICIENTS):
         if not lr >= 0.0 or not weight_decay >= 0.0 or not 0.0 <= beta < 1.0:
@@ -130,6 +131,8 @@ class HipMuon(torch.optim.Optimizer):
                     raise RuntimeError('HipMuon: sparse gradients are not supported')
                 state = self.state[p]
                 if not state:
+                    if torch.cuda.is_current_stream_capturing():          # (every replay would begin with no momentum)
+                        raise RuntimeError('HipMuon: the first step makes the momenta: take it before it is captured into a graph')
                     state['momentum'] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 muon_update(p, p.grad, state['momentum'], lr=float(group['lr']), beta=group['beta'], nesterov=group['nesterov'], weight_decay=group['weight_decay'],
                             steps=group['steps'], coefficients=group['coefficients'], out=p, momentum_out=state['momentum'])

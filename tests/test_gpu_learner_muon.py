@@ -389,3 +389,42 @@ def test_the_training_example_runs_with_muon():
         assert torch.isfinite(getattr(two, name)).all(), name
     for name in ('w1', 'w2', 'wa', 'wv'):
         assert not torch.equal(getattr(one, name), getattr(two, name)), name
+
+
+@pytest.mark.parametrize('shape', [(8, 512), (3, 20, 1500), (1500, 50), (100, 6000), (600, 130)], ids=str)
+def test_everything_in_place(shape):
+    from drloco_amd.muon import muon_update, orthogonalise
+    w, g, m = (gradient(*shape, seed=s).cuda() for s in (1, 2, 3))
+    want, factor = muon_update(w, g, m, lr=0.1, weight_decay=0.1), orthogonalise(g)
+    muon_update(w, g, m, lr=0.1, weight_decay=0.1, out=w, momentum_out=m)
+    assert torch.equal(w, want[0]) and torch.equal(m, want[1])
+    orthogonalise(g, out=g)
+    assert torch.equal(g, factor)
+
+
+def test_a_captured_optimiser_carries_its_momentum():
+    from drloco_amd.muon import HipMuon
+    shapes = ((64, 29), (20, 1500), (130, 200))
+    params, other = ([torch.nn.Parameter(gradient(*s, seed=i, scale=0.1).cuda()) for i, s in enumerate(shapes)] for _ in range(2))
+    grads = [gradient(*s, seed=10 + i).cuda() for i, s in enumerate(shapes)]
+    opt, eager = HipMuon(params, lr=0.05), HipMuon(other, lr=0.05)
+    for p, q, g in zip(params, other, grads):
+        p.grad, q.grad = g, g.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opt.step()          # makes the momenta
+    torch.cuda.current_stream().wait_stream(side)
+    eager.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for k in range(4):
+        for q, g, i in zip(other, grads, range(3)):
+            g.copy_(gradient(*g.shape, seed=20 * k + i))
+            q.grad.copy_(g)
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        for p, q in zip(params, other):
+            assert torch.equal(p, q) and torch.equal(opt.state[p]['momentum'], eager.state[q]['momentum'])

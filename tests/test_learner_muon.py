@@ -119,3 +119,13 @@ def test_the_optimiser_state_round_trips_in_32_bits():
     m = b.state[q]['momentum']
     assert m.dtype == torch.float32 and torch.equal(m, a.state[q]['momentum']) and m.data_ptr() != a.state[q]['momentum'].data_ptr()
     assert b.param_groups[0]['lr'] == 0.02
+
+
+def test_a_first_step_is_not_captured(monkeypatch):
+    p = torch.nn.Parameter(torch.ones(4, 5))
+    p.grad = torch.ones(4, 5)
+    opt = muon.HipMuon([p])
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
+    with pytest.raises(RuntimeError, match='before it is captured'):
+        opt.step()
+    assert not opt.state[p]
