@@ -23,7 +23,6 @@
 namespace dlo {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float float4_ __attribute__((ext_vector_type(4)));
 
 constexpr float SCALE = 1024.0f;
@@ -681,9 +680,11 @@ __global__ __launch_bounds__(512) void k_orth_direct(product p) {
 // with rows 16 I + 4 q + r of column c; as an operand over k = 32 s .. a lane needs eight k's, the same ones in both operands, in
 // any order.  With the order {32 s + 4 q + r, 32 s + 16 + 4 q + r} the results of the blocks I = 2 s and 2 s + 1 are an operand as they
 // stand: X goes from step to step in registers, and Q, being symmetric, is one as it comes out (with RB = 1 the products over rows
-// are those of 16 k's, whose operand is a result as it stands, A too).  Only A = X X', which sums over columns, reads X in its other
+// are those of the matrix cores' 32-bit instruction, whose operands are the results as they stand: with so few terms to average over, 22 bits
+// in them left 3 x 700 off by up to 3.7 times what 32-bit products are).  Only A = X X', which sums over columns, reads X in its other
 // orientation, from the wave's own part of LDS.  X itself stays in 32 bits: here Q is without its a I, and X = a X + Q X.  Two barriers per step, one with RB = 1, where A's parts are summed.
-// Bound by the instructions of one CU, some 450 per wave and step with RB = 2, JB = 4, and by the way in and out.  8 x 512: 13.4 us, 512 x 29 with momentum and weight: 28.5.
+// Bound by the instructions of one CU, some 450 per wave and step with RB = 2, JB = 4, and by the way in and out.  8 x 512: 14.6 us (13.4 with 16-bit products throughout, which lost
+// the precision said above), 512 x 29 with momentum and weight: 28.5.
 struct small {
     source s;
     int32_t m, n, steps, turned, flat;          // flat: the rows of every array follow each other, they are read as one
@@ -835,29 +836,20 @@ template <int RB, int JB> struct rowwise {
         for (int t = 0; t < TILES; ++t) *(float4_*)&red[wave][t][lane * 4] = acc[t];
         __syncthreads();
         if constexpr (RB == 1) {
-            const float4_ a = total(red, 0, lane);
-            half4 ah, al, qh, ql;
+            // A and Q are symmetric: what a lane holds of rows 4 q + r is an operand over those four k's as it stands, and so is x
+            const float4_ a = total(red, 0, lane) * (1.0f / (SCALE * SCALE));
+            float4_ t = {}, m;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) { _Float16 h, l; split(a[r] * (1.0f / SCALE), h, l); ah[r] = h; al[r] = l; }
-            float4_ t = {};
-            t = __builtin_amdgcn_mfma_f32_16x16x16f16(ah, al, t, 0, 0, 0);
-            t = __builtin_amdgcn_mfma_f32_16x16x16f16(al, ah, t, 0, 0, 0);
-            t = __builtin_amdgcn_mfma_f32_16x16x16f16(ah, ah, t, 0, 0, 0);
+            for (int r = 0; r < 4; ++r) t = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], a[r], t, 0, 0, 0);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                _Float16 h, l;
-                split(fmaf(p.c, t[r] * (1.0f / SCALE), p.b * (a[r] * (1.0f / SCALE))), h, l);
-                qh[r] = h; ql[r] = l;
-            }
+            for (int r = 0; r < 4; ++r) m[r] = fmaf(p.c, t[r], p.b * a[r]);
 #pragma unroll
             for (int jb = 0; jb < JB; ++jb) {
-                const half4 h = __builtin_shufflevector(o.h[jb][0], o.h[jb][0], 0, 1, 2, 3), l = __builtin_shufflevector(o.l[jb][0], o.l[jb][0], 0, 1, 2, 3);
                 float4_ y = {};
-                y = __builtin_amdgcn_mfma_f32_16x16x16f16(qh, l, y, 0, 0, 0);
-                y = __builtin_amdgcn_mfma_f32_16x16x16f16(ql, h, y, 0, 0, 0);
-                y = __builtin_amdgcn_mfma_f32_16x16x16f16(qh, h, y, 0, 0, 0);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[jb][0][r] = fmaf(p.a, x[jb][0][r], y[r] * (1.0f / SCALE));
+                for (int r = 0; r < 4; ++r) y = __builtin_amdgcn_mfma_f32_16x16x4f32(m[r], x[jb][0][r], y, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[jb][0][r] = fmaf(p.a, x[jb][0][r], y[r]);
             }
         } else {
             for (int t = wave; t < TILES; t += NWAVES) {          // a wave sums a tile and writes it, and its mirror image, as operands
@@ -973,7 +965,7 @@ __global__ __launch_bounds__(512) void k_orth_small(small p) {
 // ---- short sides of up to 64 with a long one: a workgroup per 128 JB columns ("slab"), a launch per step ---------------------------------------
 // Slab s leaves its part of A behind each launch; the next one sums all slabs' parts for itself, makes Q, moves its part of X on.
 // X waits in memory between the launches, in 32 bits and in the order of the lanes.  Seven launches instead of seventeen, each bound by
-// its way to the caches and back.  All five steps of 8 x 8000: 34 us (157 with a launch per product), 30 x 8000: 52, 8 x 100000: 72.
+// its way to the caches and back.  All five steps of 8 x 8000: 35 us (157 with a launch per product), 30 x 8000: 51, 8 x 100000: 73.
 struct slabs {
     const double* partials; int32_t n_partials;
     float* x;                     // [batch][slab][JB * RB][512 lanes][4]

@@ -428,3 +428,23 @@ def test_a_captured_optimiser_carries_its_momentum():
         torch.cuda.synchronize()
         for p, q in zip(params, other):
             assert torch.equal(p, q) and torch.equal(opt.state[p]['momentum'], eager.state[q]['momentum'])
+
+
+@pytest.mark.parametrize('rows,cols', [(8, 512), (3, 700), (2, 40), (16, 1000), (5, 3100), (9, 9000)])
+def test_few_rows_are_as_exact_as_32_bits(rows, cols):
+    """Over sixteen matrices, so that one lucky rounding says nothing: the mean error is at most that of float32 products.  Of the kernel's roundings
+    those of A (22 bits held, some 2^-23 relative) are the larger ones, those of its other products are float32's own; the definition's
+    float32 form rounds A's sum too.  A factor of 1.5 for the sampling: errors of single matrices spread by a factor of two, the mean of sixteen by a quarter of it."""
+    from drloco_amd.muon import COEFFICIENTS, orthogonalise
+    a, b, c = COEFFICIENTS
+    g = torch.stack([gradient(rows, cols, seed=100 + k) for k in range(16)])
+    got, plain, exact = orthogonalise(g.cuda()).cpu().double(), g.clone(), g.double()
+    def steps(x):
+        x = x / (x * x).sum(dim=(-2, -1), keepdim=True).sqrt()
+        for _ in range(5):
+            p = x @ x.transpose(-2, -1).contiguous()
+            x = a * x + (b * p + c * (p @ p)) @ x
+        return x
+    plain, exact = steps(plain).double(), steps(exact)
+    off = lambda o: ((o - exact).flatten(1).norm(dim=1) / exact.flatten(1).norm(dim=1)).mean()
+    assert off(got) <= 1.5 * off(plain) + 2.0 ** -24
