@@ -625,9 +625,10 @@ __global__ __launch_bounds__(512) void k_orth_direct(product p) {
         if (wave < 4) {
             __hip_atomic_store(mine, (uint64_t)__float_as_uint(v[1]) << 32 | __float_as_uint(v[0]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __hip_atomic_store(mine + 1, (uint64_t)__float_as_uint(v[3]) << 32 | __float_as_uint(v[2]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // every wave's own have arrived before the count says so: the barrier waits for none, the count for its wave's only
         }
         __shared__ uint32_t before;
-        __syncthreads();          // (waits for the stores too)
+        __syncthreads();
         if (threadIdx.x == 0) before = __hip_atomic_fetch_add(p.arrived + at, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
         if ((int)before + 1 < p.splits) return;
