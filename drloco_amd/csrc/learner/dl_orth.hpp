@@ -217,7 +217,8 @@ __device__ __forceinline__ void below(int t, int& ti, int& tj) {          // the
 template <int I, int J, int THREADS>
 __device__ __forceinline__ void emit(const product& p, int64_t b, const float* tile, int pitch, int i0, int j0) {
     const float gain = p.gain / (SCALE * SCALE);
-    const bool down = p.out_at.si == 1 && p.out_at.sj != 1;          // the caller's rows run along the short side
+    // the caller's rows run along the short side; along the long one if they have one element each, which follow each other in every array
+    const bool down = p.out_at.si == 1 && (p.out_at.sj != 1 || (p.w && p.w_at.sj != 1));
 #pragma unroll 4
     for (int e = threadIdx.x; e < I * J / 4; e += THREADS) {
         const int i = down ? e % (I / 4) * 4 : e / (J / 4), j = down ? e / (I / 4) : e % (J / 4) * 4;

@@ -448,3 +448,28 @@ def test_few_rows_are_as_exact_as_32_bits(rows, cols):
     plain, exact = steps(plain).double(), steps(exact)
     off = lambda o: ((o - exact).flatten(1).norm(dim=1) / exact.flatten(1).norm(dim=1)).mean()
     assert off(got) <= 1.5 * off(plain) + 2.0 ** -24
+
+
+WEIGHTS = {'part of wider rows': lambda w: torch.cat((w, w + 1), -1)[..., :w.shape[-1]], 'transposed': lambda w: w.transpose(-2, -1).contiguous().transpose(-2, -1),
+           'every other row': lambda w: torch.stack((w, w + 1), -2).flatten(-3, -2)[..., ::2, :], 'one row for all': lambda w: w[..., :1, :].expand(w.shape)}
+
+
+@pytest.mark.parametrize('layout', WEIGHTS)
+@pytest.mark.parametrize('shape', [(140000, 1), (1, 140000), (131000, 16), (64, 70000), (5000, 1), (900, 1), (2, 140000, 1), (45, 77), (200, 130), (600, 1)], ids=str)
+def test_weights_and_momenta_lie_anywhere(shape, layout):
+    """Strides of weight, gradient and momentum other than the result's, one column among them on every kernel: the same bits as from contiguous copies."""
+    from drloco_amd.muon import muon_update
+    w, g, m = (gradient(*shape, seed=s).cuda() for s in (1, 2, 3))
+    w, m = WEIGHTS[layout](w), WEIGHTS[layout](m)
+    want = muon_update(w.contiguous(), g, m.contiguous(), lr=0.1, weight_decay=0.1)
+    got = muon_update(w, WEIGHTS[layout](g) if layout != 'one row for all' else g, m, lr=0.1, weight_decay=0.1)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize('rows,cols', [(1, 140000), (140000, 1), (16, 131073), (64, 65537), (70000, 33)])
+def test_long_sides_beyond_the_slabs(rows, cols, dtype):
+    """Short sides of up to 64 whose long side is cut into 256 slabs and more: the kernels of the larger matrices take them."""
+    from drloco_amd.muon import orthogonalise
+    g = gradient(rows, cols, seed=11, dtype=dtype)
+    check_orthogonal(orthogonalise(g.cuda()), g)
