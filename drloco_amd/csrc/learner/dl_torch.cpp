@@ -38,6 +38,9 @@ bool memory_takes(const Tensor& x, const Tensor& gate, const Maybe& starts, cons
     return !state || (state->scalar_type() == at::kFloat && state->sizes() == x.sizes().slice(axes - 2) && state->device() == x.device());
 }
 
+// A forward-mode derivative would be lost without a word: there is no rule for it.
+bool has_tangent(const Tensor& t) { return c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined(); }
+
 // The last axis contiguous, walkers near enough for the kernels' 32-bit row offsets.
 Tensor rows(const Tensor& t) {
     const int64_t D = t.size(-1), N = t.size(-2);
@@ -104,7 +107,7 @@ struct GatedMemory : torch::autograd::Function<GatedMemory> {
 };
 
 py::object gated_memory(const Tensor& x_, const Tensor& gate_, Maybe starts, Maybe state) {
-    if (!memory_takes(x_, gate_, starts, state, 3)) return py::none();
+    if (!memory_takes(x_, gate_, starts, state, 3) || has_tangent(x_) || has_tangent(gate_) || (state && has_tangent(*state))) return py::none();
     if (x_.numel() == 0) return py::cast(std::make_tuple(x_.clone(), state ? state->clone() : at::zeros({x_.size(1), x_.size(2)}, x_.options().dtype(at::kFloat))));
     const Tensor x = rows(x_), gate = rows(gate_);
     if (starts && starts->scalar_type() == at::kBool) starts = starts->view(at::kByte);

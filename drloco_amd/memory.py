@@ -9,12 +9,13 @@ buffers carry them (an episode that begins at t sees nothing of the one before).
 CustomActorCriticPolicy, drloco/custom/policies.py:13-51, is a plain trunk); the operator stands where that trunk's hidden
 layer stands, over the rollouts of drloco/train.py:110-118."""
 import torch
+from torch.autograd import forward_ad
 
 from . import learner_lib as ll
 from . import lib
 
 
-def _check(name, x, gate, starts, state, axes):
+def _check(name, x, gate, starts, state, axes, differentiable=False):
     for i, t in enumerate((x, gate, starts, state)):
         if not torch.is_tensor(t) and (i < 2 or t is not None):
             raise TypeError(f'{name}: expected tensors, got {type(t).__name__}')
@@ -36,6 +37,8 @@ def _check(name, x, gate, starts, state, axes):
             raise TypeError(f'{name}: state must be float32, got {state.dtype}')
         if state.shape != x.shape[-2:]:
             raise ValueError(f'{name}: state {tuple(state.shape)} is not {tuple(x.shape[-2:])}')
+    if differentiable and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (x, gate, state)):
+        raise NotImplementedError(f'{name}: forward-mode derivatives are not supported')
     ll.require_device(name, x, gate, starts, state)
 
 
@@ -43,13 +46,13 @@ def gated_memory(x, gate, starts=None, state=None):
     """The memory over a rollout.  x, gate: [T, N, D] of one type (float32, bfloat16, float16) with any strides (a last axis that is
     not contiguous is copied); starts: uint8 or bool [T, N], nonzero = an episode begins at that step, or None; state: float32
     [N, D], the memory before the first step, or None for zeros.  Returns (h [T, N, D] of x's type, the state after the last step,
-    float32 [N, D], unrounded).  Differentiable once with respect to x, gate and state.
+    float32 [N, D], unrounded).  Differentiable once with respect to x, gate and state, in reverse mode (forward-mode derivatives are refused).
 
     The memory is held and summed in float32 whatever the type of x; nothing before an episode's start is read, not even a NaN.
     An infinity within an episode makes that channel NaN until the next start.  T = 0 gives an empty h and the state as it came."""
     out = ll.ops().gated_memory(x, gate, starts, state) if torch.is_tensor(x) and torch.is_tensor(gate) else None
     if out is None:
-        _check('gated_memory', x, gate, starts, state, 3)
+        _check('gated_memory', x, gate, starts, state, 3, differentiable=True)
         raise lib.DrlocoError('gated_memory: the arguments were refused')
     return out
 

@@ -376,3 +376,29 @@ def test_repeats_are_bit_identical():
     first = check_all(x, gate, b, st, gh, gl)
     second = check_all(x, gate, b, st, gh, gl)
     assert torch.equal(first[0], second[0]) and all(torch.equal(p, q) for p, q in zip(first[2], second[2]))
+
+
+@pytest.mark.parametrize('which', [0, 1, 3])
+def test_forward_mode_derivatives_are_refused(which):
+    from torch.autograd import forward_ad
+    from drloco_amd.memory import gated_memory
+    x, gate, b, st, _, _ = (dev(t) for t in make(9, 3, 8, torch.float32))
+    args = [x, gate, b, st]
+    with forward_ad.dual_level():
+        args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        for grad in (False, True):
+            x.requires_grad_(grad)
+            with pytest.raises(RuntimeError):
+                gated_memory(*args)
+        args[which] = forward_ad.unpack_dual(args[which]).primal.detach()
+        gated_memory(*args)
+
+
+def test_transforms_are_refused_or_right():
+    """torch.func's wrapped tensors have no memory for a kernel to read: an error, not a wrong result"""
+    from drloco_amd.memory import gated_memory
+    x, gate, b, st, _, _ = (dev(t) for t in make(9, 3, 8, torch.float32))
+    f = lambda v: gated_memory(v, gate, b, st)[0].sum()
+    for call in (lambda: torch.func.grad(f)(x), lambda: torch.vmap(f)(torch.stack((x, x))), lambda: torch.func.jvp(f, (x,), (x,))):
+        with pytest.raises(RuntimeError):
+            call()

@@ -184,3 +184,14 @@ def test_the_gradient_formula_against_differences():
             args[which][at] -= 2 * e
             # central differences: e^2 of truncation, 2^-53 * |f| / e of rounding
             assert abs((up - f(*args)) / (2 * e) - grad[at]) < 1e-7
+
+
+@pytest.mark.parametrize('which', [0, 1, 3])
+def test_forward_mode_derivatives_are_refused(which):
+    """(not dropped: the result would have no tangent, which reads as a zero one)"""
+    from torch.autograd import forward_ad
+    args = [t3(4, 3, 8), t3(4, 3, 8), None, t3(3, 8)]
+    with forward_ad.dual_level():
+        args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(NotImplementedError):
+            memory.gated_memory(*args)
