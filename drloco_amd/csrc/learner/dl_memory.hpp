@@ -440,7 +440,7 @@ __global__ __launch_bounds__(64 * W) void k_memory_short(shape s, chain ch, cons
             ph += plane;
         }
     }
-    if (state_out && wave == 0 && c.valid && (!CHAIN || (int)k + 1 == s.chunks)) store_floats<V>(state_out + corner, floats, next);
+    if (state_out && c.valid && len > 0 && t0 + len == s.T) store_floats<V>(state_out + corner, floats, in);          // (what h[T-1] was rounded from, not a join of maps)
 }
 
 // ---- gradients of a run.  hs: the states before each step, recomputed from the saved one --------------------------------------------------
@@ -567,7 +567,7 @@ __global__ __launch_bounds__(64 * W) void k_memory_short_back(shape s, chain ch,
     join<V, true>(la, lb, lane, W, W - 1 - wave, carry, in, next);
     if constexpr (CHAIN) leave<V, true>(ch, k, s.chunks, plane, corner + floats / 4, c.valid, wave, next);
     if (len > 0) b.finish(c, t0, len, begin, m, hs, in, dx, dgate, plane, corner, elems);
-    if (dstate && wave == 0 && c.valid && k == 0) store_floats<V>(dstate + corner, floats, next);
+    if (dstate && wave == 0 && c.valid && k == 0) store_floats<V>(dstate + corner, floats, in);
 }
 
 // One control step.  state_out may be state: a thread reads its own columns, which are no other's, before it writes them.

@@ -49,7 +49,7 @@ def gated_memory(x, gate, starts=None, state=None):
     float32 [N, D], unrounded).  Differentiable once with respect to x, gate and state, in reverse mode (forward-mode derivatives are refused).
 
     The memory is held and summed in float32 whatever the type of x; nothing before an episode's start is read, not even a NaN.
-    An infinity within an episode makes that channel NaN until the next start.  T = 0 gives an empty h and the state as it came."""
+    An infinity within an episode leaves that channel infinite or NaN until the next start.  T = 0 gives an empty h and the state as it came."""
     out = ll.ops().gated_memory(x, gate, starts, state) if torch.is_tensor(x) and torch.is_tensor(gate) else None
     if out is None:
         _check('gated_memory', x, gate, starts, state, 3, differentiable=True)

@@ -44,7 +44,7 @@ int dl_learner_abi_version(void);
  *     h[t] = a[t] * (starts[t] ? 0 : h[t-1]) + (1 - a[t]) * x[t],        h[-1] = state (NULL: zeros)
  *
  * starts: uint8 [T, N], nonzero = an episode begins at t and nothing of the memory before it is read (a NaN or an
- * infinity there does not leak); NULL: none.  Elements of x, gate, h and of the gradients have `dtype`; states, sums and
+ * infinity there does not leak; within an episode an infinity leaves its channel infinite or NaN until the next one begins); NULL: none.  Elements of x, gate, h and of the gradients have `dtype`; states, sums and
  * gradients of states are float.  Strides are in elements, for the first two axes; the last axis is contiguous; a stride
  * of 0 (a broadcast input) is allowed for inputs.  h, dx and dgate are contiguous [T, N, D], states [N, D]. */
 typedef struct dl_memory_shape {

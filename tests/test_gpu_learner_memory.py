@@ -402,3 +402,20 @@ def test_transforms_are_refused_or_right():
     for call in (lambda: torch.func.grad(f)(x), lambda: torch.vmap(f)(torch.stack((x, x))), lambda: torch.func.jvp(f, (x,), (x,))):
         with pytest.raises(RuntimeError):
             call()
+
+
+@pytest.mark.parametrize('T', [1, 7, 16, 17, 100, 128, 129, 300, 2050, 9000])
+@pytest.mark.parametrize('N,D', [(1, 5), (3, 64), (600, 130)])
+def test_the_state_is_the_last_step(T, N, D):
+    """state = h[T-1] before it is rounded: the same bits in float32, also where the last step takes in an infinity, whatever the form"""
+    from drloco_amd.memory import gated_memory
+    if T * N * D > 3e7:
+        T = 300
+    x, gate, b, st, _, _ = (dev(t) for t in make(T, N, D, torch.float32, seed=T))
+    h, last = gated_memory(x, gate, b, st)
+    assert torch.equal(h[-1], last)
+    bad = x.clone()
+    bad[-1, :, 0], bad[-1, :, 1], bad[-1, :, 2] = float('inf'), -float('inf'), float('nan')
+    h2, last2 = gated_memory(bad, gate, b, st)
+    assert torch.equal(h2[-1].nan_to_num(1.5, 2.5, 3.5), last2.nan_to_num(1.5, 2.5, 3.5)) and not torch.isfinite(last2[:, :3]).any()
+    assert torch.equal(last2[:, 3:], last[:, 3:]) and torch.equal(h2[:-1], h[:-1])
