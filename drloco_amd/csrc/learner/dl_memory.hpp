@@ -14,7 +14,8 @@
 //
 // Rounding.  The smaller of a and s is computed as e / (1 + e), e = exp(-|g|), and both products go through it:
 //     g >= 0:  h = h' + s (x - h'),  c = l - s l        g < 0:  h = x + a (h' - x),  c = a l
-// so that a long memory (s small) loses nothing to the rounding of a = 1 - s, and a closed gate gives x exactly.
+// so that a long memory (s small) loses nothing to the rounding of a = 1 - s, and a closed gate gives x exactly.  The differences
+// are taken of halves: x and h of up to the largest number are well.
 //
 // Columns.  A lane takes V neighbouring channels with one load (4 or 8 bytes, any alignment); where V does not divide D the last
 // lane of a row moves back, and two lanes compute, and write, the same values.
@@ -53,9 +54,15 @@ __device__ __forceinline__ float gate_of(float g) {
     return copysignf(e * __builtin_amdgcn_rcpf(1.0f + e), g);
 }
 __device__ __forceinline__ bool keeps(float m) { return !(__float_as_uint(m) >> 31); }          // s is the smaller one
+// f (x - h) + rest.  The difference may be beyond the largest number where the product is not, so it is taken of halves (2 f is a number: f is a gate
+// or a quarter of a gradient at most); not with x in float16, from which no float32 is further away than that (100003 x 333: 105 us, of halves 113).
+template <typename E> constexpr bool wide = !std::is_same<E, _Float16>::value;
+template <typename E> __device__ __forceinline__ float times_apart(float f, float x, float h, float rest) {
+    return wide<E> ? fmaf(f + f, fmaf(-0.5f, h, 0.5f * x), rest) : fmaf(f, x - h, rest);
+}
 // one step of the state
-__device__ __forceinline__ float step_of(float m, float x, float h) {
-    return fmaf(m, x - h, keeps(m) ? h : x);           // (m < 0: x + |m| (h - x) = x + m (x - h))
+template <typename E> __device__ __forceinline__ float step_of(float m, float x, float h) {
+    return times_apart<E>(m, x, h, keeps(m) ? h : x);           // (m < 0: x + |m| (h - x) = x + m (x - h))
 }
 // one step of a product of a: l -> a l
 __device__ __forceinline__ float decay_of(float m, float l) {
@@ -77,6 +84,12 @@ struct factor {
     __device__ __forceinline__ float held(bool begun) const { return begun ? BEGUN : p <= 0.5f ? p : -a; }          // (a NaN stays one)
 };
 __device__ __forceinline__ float apply(float m, float b, float h) { return m > 1.0f ? b : decay_of(m, h) + b; }
+// Of states: the sum of two shares of finite values lies between them, but may be rounded past the largest number (not with x in float16, whose
+// share is lost next to such a state's).
+__device__ __forceinline__ float apply_state(float m, float b, float h) {
+    const float r = apply(m, b, h);
+    return __builtin_isinf(r) && __builtin_isfinite(b) && __builtin_isfinite(h) ? copysignf(__FLT_MAX__, r) : r;
+}
 __device__ __forceinline__ float after(float m, float n) {          // m, then n
     if (m > 1.0f || n > 1.0f) return BEGUN;
     factor f;
@@ -119,8 +132,8 @@ template <typename T> __device__ __forceinline__ void store_at(void* base, uint3
 }
 
 // The value that enters the run of each wave from the maps of the waves before it (`before` of them, in the order of the
-// recurrence), and the one behind the last.
-template <int V, bool BACK>
+// recurrence), and the one behind the last.  STATE: of states that may reach the largest number.
+template <int V, bool BACK, bool STATE>
 __device__ __forceinline__ void join(const float (*la)[64 * V], const float (*lb)[64 * V], int lane, int waves, int before, const float (&carry)[V], float (&mine)[V], float (&next)[V]) {
 #pragma unroll
     for (int v = 0; v < V; ++v) next[v] = mine[v] = carry[v];
@@ -128,7 +141,7 @@ __device__ __forceinline__ void join(const float (*la)[64 * V], const float (*lb
         const int w = BACK ? waves - 1 - i : i;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            next[v] = apply(la[w][v * 64 + lane], lb[w][v * 64 + lane], next[v]);
+            next[v] = STATE ? apply_state(la[w][v * 64 + lane], lb[w][v * 64 + lane], next[v]) : apply(la[w][v * 64 + lane], lb[w][v * 64 + lane], next[v]);
             if (i + 1 == before) mine[v] = next[v];
         }
     }
@@ -249,7 +262,7 @@ __global__ __launch_bounds__(64) void k_memory_run(shape s, const E* __restrict_
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     if (!decltype(all)::value) now[v] = (begin >> t) & 1 ? 0.0f : now[v];
-                    now[v] = step_of(gate_of(get<E, V>(r.g[t], v)), get<E, V>(r.x[t], v), now[v]);
+                    now[v] = step_of<E>(gate_of(get<E, V>(r.g[t], v)), get<E, V>(r.x[t], v), now[v]);
                     put<E, V>(o, v, now[v]);
                 }
                 if (c.valid) store_at<vec>(ph, elems, o);
@@ -297,7 +310,7 @@ template <int V> __device__ __forceinline__ void link(uint64_t* at, const float 
     }
 }
 // m, b: joined with the links of the chunks first, first + way, .. (`count` of them)
-template <int V> __device__ __forceinline__ void follow(const uint64_t* links, int64_t plane, int first, int way, int count, float (&m)[V], float (&b)[V]) {
+template <int V, bool STATE> __device__ __forceinline__ void follow(const uint64_t* links, int64_t plane, int first, int way, int count, float (&m)[V], float (&b)[V]) {
     constexpr int AT_ONCE = 4;
     for (int i = 0; i < count; i += AT_ONCE) {
         uint64_t l[AT_ONCE][V];
@@ -315,7 +328,7 @@ template <int V> __device__ __forceinline__ void follow(const uint64_t* links, i
                     l[k][v] = __hip_atomic_load(links + (int64_t)(first + way * (i + k)) * plane + v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
                 const float n = __uint_as_float((uint32_t)l[k][v]), c = __uint_as_float((uint32_t)(l[k][v] >> 32));
-                b[v] = apply(n, c, b[v]);
+                b[v] = STATE ? apply_state(n, c, b[v]) : apply(n, c, b[v]);
                 m[v] = after(m[v], n);
             }
         }
@@ -328,7 +341,7 @@ __device__ __forceinline__ uint32_t take_ticket(const chain& ch) {
     return __builtin_amdgcn_readfirstlane((int)mine);
 }
 // Leaves the workgroup's link (from its waves' maps la, lb) and finds the value that enters it; carry: the one that enters the chain.
-template <int V, bool BACK>
+template <int V, bool BACK, bool STATE>
 __device__ __forceinline__ void pass_on(const chain& ch, int k, int chunks, int64_t plane, int64_t col, bool valid, int wave, int lane, const float (*la)[64 * V], const float (*lb)[64 * V],
                                         float (*lc)[64 * V], float (*ld)[64 * V], float (&carry)[V]) {
     const int order = BACK ? chunks - 1 - k : k, before = order % GROUP;
@@ -336,7 +349,7 @@ __device__ __forceinline__ void pass_on(const chain& ch, int k, int chunks, int6
 #pragma unroll
     for (int v = 0; v < V; ++v) m[v] = b[v] = zero[v] = 0.0f;
     if (wave == 0 && before + 1 < GROUP && order + 1 < chunks) {          // (of the last one of a group nobody takes the link)
-        join<V, BACK>(la, lb, lane, WAVES, 0, zero, mine, next);
+        join<V, BACK, STATE>(la, lb, lane, WAVES, 0, zero, mine, next);
         for (int w = 0; w < WAVES; ++w) {
 #pragma unroll
             for (int v = 0; v < V; ++v) m[v] = after(m[v], la[w][v * 64 + lane]);
@@ -347,7 +360,7 @@ __device__ __forceinline__ void pass_on(const chain& ch, int k, int chunks, int6
 #pragma unroll
         for (int v = 0; v < V; ++v) m[v] = b[v] = 0.0f;
         const int lo = before * wave / WAVES, hi = before * (wave + 1) / WAVES, way = BACK ? -1 : 1;
-        follow<V>(ch.links + col, plane, k - way * (before - lo), way, hi - lo, m, b);
+        follow<V, STATE>(ch.links + col, plane, k - way * (before - lo), way, hi - lo, m, b);
 #pragma unroll
         for (int v = 0; v < V; ++v) { lc[wave][v * 64 + lane] = m[v]; ld[wave][v * 64 + lane] = b[v]; }
     }
@@ -365,7 +378,7 @@ __device__ __forceinline__ void pass_on(const chain& ch, int k, int chunks, int6
     }
     if (before > 0) {
         __syncthreads();
-        join<V, false>(lc, ld, lane, WAVES, 0, carry, mine, next);
+        join<V, false, STATE>(lc, ld, lane, WAVES, 0, carry, mine, next);
 #pragma unroll
         for (int v = 0; v < V; ++v) carry[v] = next[v];
     }
@@ -409,7 +422,7 @@ __global__ __launch_bounds__(64 * W) void k_memory_short(shape s, chain ch, cons
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             m[t][v] = t < len ? gate_of(get<E, V>(r.g[t], v)) : 0.0f;          // (behind the end: an open gate, h stays as it is)
-            B[v] = step_of(m[t][v], get<E, V>(r.x[t], v), (begin >> t) & 1 ? 0.0f : B[v]);
+            B[v] = step_of<E>(m[t][v], get<E, V>(r.x[t], v), (begin >> t) & 1 ? 0.0f : B[v]);
             A[v].step(m[t][v]);
         }
         pause<V>(t);
@@ -420,10 +433,10 @@ __global__ __launch_bounds__(64 * W) void k_memory_short(shape s, chain ch, cons
     __syncthreads();
     if constexpr (CHAIN) {
         __shared__ float lc[W][64 * V], ld[W][64 * V];
-        pass_on<V, false>(ch, (int)k, s.chunks, plane, corner + floats / 4, c.valid, wave, lane, la, lb, lc, ld, carry);
+        pass_on<V, false, wide<E>>(ch, (int)k, s.chunks, plane, corner + floats / 4, c.valid, wave, lane, la, lb, lc, ld, carry);
     }
     float in[V], next[V];
-    join<V, false>(la, lb, lane, W, wave, carry, in, next);
+    join<V, false, wide<E>>(la, lb, lane, W, wave, carry, in, next);
     if constexpr (CHAIN) leave<V, false>(ch, (int)k, s.chunks, plane, corner + floats / 4, c.valid, wave, next);
     if (marks && c.valid && len > 0) store_floats<V>(marks + (int64_t)(t0 / MARK) * plane + corner, floats, in);
     E* ph = h + (int64_t)t0 * plane + corner;
@@ -433,7 +446,7 @@ __global__ __launch_bounds__(64 * W) void k_memory_short(shape s, chain ch, cons
             vec o;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                in[v] = step_of(m[t][v], get<E, V>(r.x[t], v), (begin >> t) & 1 ? 0.0f : in[v]);
+                in[v] = step_of<E>(m[t][v], get<E, V>(r.x[t], v), (begin >> t) & 1 ? 0.0f : in[v]);
                 put<E, V>(o, v, in[v]);
             }
             if (c.valid) store_at<vec>(ph, elems, o);
@@ -460,7 +473,7 @@ template <typename E, int V> struct run_back {
             for (int v = 0; v < V; ++v) {
                 m[t][v] = t < len ? gate_of(get<E, V>(r.g[t], v)) : 0.0f;
                 hs[t][v] = (begin >> t) & 1 ? 0.0f : h0[v];
-                h0[v] = step_of(m[t][v], get<E, V>(r.x[t], v), hs[t][v]);
+                h0[v] = step_of<E>(m[t][v], get<E, V>(r.x[t], v), hs[t][v]);
             }
             pause<V>(t);
         }
@@ -480,7 +493,7 @@ template <typename E, int V> struct run_back {
                     const float l = get<E, V>(r.d[t], v) + in[v];
                     const float q = fabsf(m[t][v]), w = q * l, o = l - w;          // the smaller and the larger share
                     put<E, V>(ox, v, keeps(m[t][v]) ? w : o);
-                    put<E, V>(og, v, (hs[t][v] - get<E, V>(r.x[t], v)) * fmaf(-q, w, w));
+                    put<E, V>(og, v, times_apart<E>(fmaf(q, w, -w), get<E, V>(r.x[t], v), hs[t][v], 0.0f));
                     in[v] = (begin >> t) & 1 ? 0.0f : keeps(m[t][v]) ? o : w;
                 }
                 if (c.valid) { store_at<vec>(dx, elems, ox); store_at<vec>(dgate, elems, og); }
@@ -561,10 +574,10 @@ __global__ __launch_bounds__(64 * W) void k_memory_short_back(shape s, chain ch,
     __syncthreads();
     if constexpr (CHAIN) {
         __shared__ float lc[W][64 * V], ld[W][64 * V];
-        pass_on<V, true>(ch, k, s.chunks, plane, corner + floats / 4, c.valid, wave, lane, la, lb, lc, ld, carry);
+        pass_on<V, true, false>(ch, k, s.chunks, plane, corner + floats / 4, c.valid, wave, lane, la, lb, lc, ld, carry);
     }
     float in[V], next[V];
-    join<V, true>(la, lb, lane, W, W - 1 - wave, carry, in, next);
+    join<V, true, false>(la, lb, lane, W, W - 1 - wave, carry, in, next);
     if constexpr (CHAIN) leave<V, true>(ch, k, s.chunks, plane, corner + floats / 4, c.valid, wave, next);
     if (len > 0) b.finish(c, t0, len, begin, m, hs, in, dx, dgate, plane, corner, elems);
     if (dstate && wave == 0 && c.valid && k == 0) store_floats<V>(dstate + corner, floats, in);
@@ -593,7 +606,7 @@ __global__ __launch_bounds__(256) void k_memory_step(int64_t N, int64_t D, int64
     }
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        r[v] = step_of(gate_of(get<E, V>(gs, v)), get<E, V>(xs, v), begin ? 0.0f : r[v]);
+        r[v] = step_of<E>(gate_of(get<E, V>(gs, v)), get<E, V>(xs, v), begin ? 0.0f : r[v]);
         put<E, V>(o, v, r[v]);
         put<float, V>(last, v, r[v]);
     }

@@ -419,3 +419,35 @@ def test_the_state_is_the_last_step(T, N, D):
     h2, last2 = gated_memory(bad, gate, b, st)
     assert torch.equal(h2[-1].nan_to_num(1.5, 2.5, 3.5), last2.nan_to_num(1.5, 2.5, 3.5)) and not torch.isfinite(last2[:, :3]).any()
     assert torch.equal(last2[:, 3:], last[:, 3:]) and torch.equal(h2[:-1], h[:-1])
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize('T,N,D', [(1, 3, 5), (12, 5, 8), (128, 2, 7), (300, 3, 20), (2000, 2, 6), (9000, 1, 5), (40, 2100, 66)])
+def test_the_largest_numbers(T, N, D, dtype):
+    """x and state of up to the type's largest number, of either sign and next to small ones: every h lies between them, so nothing may
+    be infinite, though x - h is beyond float32 and joined states are rounded against its end"""
+    x, gate, b, st, gh, gl = make(T, N, D, dtype, seed=T)
+    g = torch.Generator().manual_seed(T)
+    most = torch.finfo(dtype).max
+    big = lambda *s: (torch.randint(0, 2, s, generator=g) * 2 - 1).float() * most
+    x = torch.where(torch.rand(T, N, D, generator=g) < 0.7, big(T, N, D), x.float()).to(dtype)
+    st = torch.where(torch.rand(N, D, generator=g) < 0.7, big(N, D), st)
+    x[:, :, 1], st[:, 1] = most, most          # a channel that stays there
+    h, last, got = check_all(x, gate, b, st, gh * 2.0 ** -10, gl * 2.0 ** -10)
+    assert torch.isfinite(h).all() and torch.isfinite(last).all() and all(torch.isfinite(t).all() for t in got)
+    if T == 1:
+        from drloco_amd.memory import gated_memory_step
+        o, s = gated_memory_step(x[0].cuda(), gate[0].cuda(), st.cuda(), b[0].cuda())
+        assert torch.equal(o, h[0]) and torch.equal(s, last)
+
+
+@pytest.mark.parametrize('T,N,D', [(1, 3, 5), (128, 2, 7), (2000, 2, 6), (40, 2100, 66)])
+def test_the_largest_state_of_a_float16_memory(T, N, D):
+    from drloco_amd.memory import gated_memory
+    x, gate, _, st, _, _ = make(T, N, D, torch.float16, seed=T, shift=6.0)
+    most = torch.finfo(torch.float32).max
+    x, st = torch.sign(x) * torch.finfo(torch.float16).max, torch.sign(st) * most
+    gate[:, :, 1] = float('inf')          # a channel that stays there
+    _, last = gated_memory(x.cuda(), gate.cuda(), None, st.cuda())
+    _, last_ = R.memory(np64(x), np64(gate), None, np64(st))
+    assert torch.isfinite(last).all() and np.all(np.abs(np64(last.cpu()) - last_) <= 12 * U * most * (T + 1)) and torch.equal(last[:, 1].cpu(), st[:, 1])
