@@ -190,23 +190,22 @@ int32_t whole_tiles(int64_t tiles, int64_t batch, int64_t slots) {
 // Tiles of 256 x 128 (a CU each) where they come to at least nine tenths of a round of whole ones and what is left in 64 x 64 to one
 // round at most, else of 128 x 128 (two to a CU).  4096 x 8192 x 4096: 610 instead of 652 us; 2 x 1031 x 4099 x 1031, where 328 of
 // 64 x 64 would be left: 71 and 68 us.
-template <int TILE, int MODE, bool COARSE> void launch_product(dlo::product p, int64_t tiles, int64_t batch, const orth_form& f, hipStream_t st) {
+template <int TILE, int MODE> void launch_product(dlo::product p, int64_t tiles, int64_t batch, const orth_form& f, hipStream_t st) {
     const dlo::plan& q = f.p;
     if (TILE == 32 || (MODE == dlo::GRAM && f.gram_direct) || (MODE == dlo::POLY && f.poly_direct)) {
         if (TILE != 32) tiles = (int64_t)(q.mp / 32) * (q.mp / 32 + 1) / 2;
         dlo::k_orth_direct<MODE><<<dim3((unsigned)(MODE == dlo::GRAM ? tiles * p.splits : tiles), 1, (unsigned)batch), 512, 0, st>>>(p);
     } else if constexpr (TILE != 32) {
-        if (COARSE) p.kb /= 2;          // two at once
         constexpr bool half = MODE == dlo::GRAM || MODE == dlo::POLY;
         const int64_t wi = q.mp / 256, wj = q.np / 128, wide = half ? wi * (wi + 1) : wi * wj, whole = whole_tiles(wide, batch, 256);
         const int64_t left = (wide - whole) * 8 + (q.mp % 256 ? 2 * (half ? q.mp / 64 : q.np / 64) : 0);
         if (whole * batch >= 230 && left * batch <= 256) {
             p.tiles = (int32_t)wide; p.whole = (int32_t)whole;
             p.tiles_i = (int32_t)wi; p.tiles_j = (int32_t)wj;
-            return dlo::k_orth_wide<MODE, COARSE><<<dim3((unsigned)(whole + left), 1, (unsigned)batch), 256, 0, st>>>(p);
+            return dlo::k_orth_wide<MODE><<<dim3((unsigned)(whole + left), 1, (unsigned)batch), 256, 0, st>>>(p);
         }
         p.tiles = (int32_t)tiles; p.whole = whole_tiles(tiles, batch, 512);
-        dlo::k_orth_product<MODE, COARSE><<<dim3((unsigned)(p.whole + (tiles - p.whole) * 4), 1, (unsigned)batch), 256, 0, st>>>(p);
+        dlo::k_orth_product<MODE><<<dim3((unsigned)(p.whole + (tiles - p.whole) * 4), 1, (unsigned)batch), 256, 0, st>>>(p);
     }
 }
 
@@ -218,21 +217,19 @@ template <int TILE> void launch_steps(const dl_orth_shape* s, const orth_form& f
     const int64_t ti = f.p.mp / TILE, tj = f.p.np / TILE, tri = ti * (ti + 1) / 2;
     const int32_t km = f.p.mp / 32, kn = f.p.np / 32;
     for (int k = 0; k < s->steps; ++k) {
-        const bool end = k + 1 == s->steps, coarse = TILE != 32 && end && s->out_type == DL_BF16;
+        const bool end = k + 1 == s->steps;
         dlo::product p = last;
         p.P = p.Q = xr; p.P_b = p.Q_b = f.p.x_size; p.kb = kn;
         p.out0 = A; p.out0_b = f.p.a_size; p.out0_kb = km;
-        if (coarse) launch_product<TILE, dlo::GRAM, TILE != 32>(p, tri, s->batch, f, st); else launch_product<TILE, dlo::GRAM, false>(p, tri, s->batch, f, st);
+        launch_product<TILE, dlo::GRAM>(p, tri, s->batch, f, st);
         p.P = p.Q = A; p.P_b = p.Q_b = f.p.a_size; p.kb = km;
         p.A = A; p.out0 = Q;
-        if (coarse) launch_product<TILE, dlo::POLY, TILE != 32>(p, tri, s->batch, f, st); else launch_product<TILE, dlo::POLY, false>(p, tri, s->batch, f, st);
+        launch_product<TILE, dlo::POLY>(p, tri, s->batch, f, st);
         p.P = Q; p.Q = xc[k & 1]; p.Q_b = f.p.x_size;
         p.tiles_i = (int32_t)ti; p.tiles_j = (int32_t)tj;
         p.out0 = xr; p.out0_b = f.p.x_size; p.out0_kb = kn;
         p.out1 = xc[(k + 1) & 1]; p.out1_b = f.p.x_size; p.out1_kb = km;
-        if (!end) launch_product<TILE, dlo::STEP, false>(p, ti * tj, s->batch, f, st);
-        else if (coarse) launch_product<TILE, dlo::LAST, TILE != 32>(p, ti * tj, s->batch, f, st);
-        else launch_product<TILE, dlo::LAST, false>(p, ti * tj, s->batch, f, st);
+        if (end) launch_product<TILE, dlo::LAST>(p, ti * tj, s->batch, f, st); else launch_product<TILE, dlo::STEP>(p, ti * tj, s->batch, f, st);
     }
 }
 

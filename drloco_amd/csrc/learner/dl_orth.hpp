@@ -7,9 +7,7 @@
 // held as the sum of two float16 planes, hi + lo = 22 bits, and a product is three 16-bit ones accumulated in 32 bits,
 // hi hi + hi lo + lo hi (what is left out is below 2^-22): the splitting of Ootomo and Yokota (2022).  All entries are at most
 // about one, so they are held times 2^10, which keeps lo clear of float16's smallest numbers.
-// A bfloat16 result holds 8 bits: its last step, whose errors no other step amplifies, is one product of the hi planes (11 bits) where
-// the products are staged (below): 4096 x 8192, 0.7 of 5.9 ms; the result is off by 1.72e-3 of its norm instead of the 1.66e-3 that
-// its own rounding makes.  One step earlier it would be 1.9e-3 to 2.9e-3, so that step is whole.
+// That goes for every step and every type of result: a result of 16 bits is the 32-bit one, rounded once.
 // A and Q are symmetric: only their tiles on and below the diagonal are computed, and written to both places.
 //
 // Layout.  A matrix that is an operand lies in memory as the matrix cores read it: for 16 rows and 32 columns k a "fragment" of
@@ -303,27 +301,26 @@ __device__ __forceinline__ void finish(const product& p, float* tile, int i0, in
     }
 }
 
-// i0, j0: the tile's first row and column.  COARSE: the hi planes only, and those of two steps along k in the place of both planes of one.
-template <int BM, int BN, int WM, int WN, int NS, int MODE, bool COARSE>
+// i0, j0: the tile's first row and column
+template <int BM, int BN, int WM, int WN, int NS, int MODE>
 __device__ __forceinline__ void product_tile(const product& p, int i0, int j0, char* lds) {
     typedef staged<BM, BN, WM, WN, NS> L;
     constexpr int WAVES = L::WAVES, TM = WM / 16, TN = WN / 16, ROWS = L::ROWS, PITCH = L::PITCH, STAGE = L::STAGE;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int64_t b = blockIdx.z;
-    constexpr int STEP_SIZE = COARSE ? 2 * FRAG : FRAG;
-    const int64_t along = (int64_t)p.kb * STEP_SIZE;          // of a row of fragments
+    const int64_t along = (int64_t)p.kb * FRAG;          // of a row of fragments
     const _Float16* P = p.P + b * p.P_b + i0 / 16 * along;
     const _Float16* Q = p.Q + b * p.Q_b + j0 / 16 * along;
 
     // a step's copies into a stage: one instruction of a wave moves 1 KB, a plane of a fragment
     auto copy = [&](int f, int k, int stage) {
         const int piece = f * WAVES + wave, r = piece >> 1, plane = piece & 1;
-        const _Float16* from = (r < BM / 16 ? P + r * along : Q + (r - BM / 16) * along) + ((int64_t)k * STEP_SIZE + plane * (STEP_SIZE / 2));
+        const _Float16* from = (r < BM / 16 ? P + r * along : Q + (r - BM / 16) * along) + ((int64_t)k * FRAG + plane * (FRAG / 2));
         auto at = (const __attribute__((address_space(1))) char*)from;
         asm("" : "+s"(at));          // the same for the wave: stays in scalar registers
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(at + (uint32_t)(lane * 16)), (__attribute__((address_space(3))) void*)(lds + stage * STAGE + piece * 1024), 16, 0, 0);
     };
-    constexpr int READS = 2 * (TM + TN), PRODUCTS = (COARSE ? 2 : 3) * TM * TN;
+    constexpr int READS = 2 * (TM + TN), PRODUCTS = 3 * TM * TN;
     // The small products hi lo and lo hi have sums of their own: every addition to a long sum rounds it, and these are two of three.
     float4_ acc[TM][TN] = {}, small[TM][TN] = {};
     const int wi = wave / (BN / WN), wj = wave % (BN / WN);
@@ -335,7 +332,7 @@ __device__ __forceinline__ void product_tile(const product& p, int i0, int j0, c
     };
     auto multiply = [&](const fragments& f, int n) {          // hi lo for all, lo hi for all, hi hi for all: no sum twice in a row
         const int kind = n / (TM * TN), i = n / TN % TM, j = n % TN;
-        const bool p_lo = kind == 1, q_lo = COARSE ? kind == 1 : kind == 0;
+        const bool p_lo = kind == 1, q_lo = kind == 0;
         float4_& sum = p_lo != q_lo ? small[i][j] : acc[i][j];
         sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(p_lo ? f.l[i] : f.h[i], q_lo ? f.l[TM + j] : f.h[TM + j], sum, 0, 0, 0);
     };
@@ -389,7 +386,7 @@ __device__ __forceinline__ void product_tile(const product& p, int i0, int j0, c
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) tile[(wi * WM + i * 16 + (lane >> 4) * 4 + r) * PITCH + wj * WN + j * 16 + (lane & 15)] = COARSE ? acc[i][j][r] : acc[i][j][r] + small[i][j][r];
+            for (int r = 0; r < 4; ++r) tile[(wi * WM + i * 16 + (lane >> 4) * 4 + r) * PITCH + wj * WN + j * 16 + (lane & 15)] = acc[i][j][r] + small[i][j][r];
     __syncthreads();
     finish<BM, BN, WAVES, MODE>(p, tile, i0, j0);
 }
@@ -397,19 +394,18 @@ __device__ __forceinline__ void product_tile(const product& p, int i0, int j0, c
 // 256 x 128 in four waves of 128 x 64: a wave keeps the four column fragments of a step and lets the eight row fragments pass by, two
 // ahead of their products; the next step's column fragments come in during the second half of a step, behind the one barrier.
 // (With all fragments of two steps at hand the sums no longer fit the vector registers, and are carried to and fro.)
-template <int MODE, bool COARSE>
+template <int MODE>
 __device__ __forceinline__ void wide_tile(const product& p, int i0, int j0, char* lds) {
     typedef staged<256, 128, 128, 64, 3> L;
     constexpr int TM = 8, TN = 4, PITCH = L::PITCH, STAGE = L::STAGE;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), wi = wave >> 1, wj = wave & 1;
     const int64_t b = blockIdx.z;
-    constexpr int STEP_SIZE = COARSE ? 2 * FRAG : FRAG;
-    const int64_t along = (int64_t)p.kb * STEP_SIZE;          // of a row of fragments
+    const int64_t along = (int64_t)p.kb * FRAG;          // of a row of fragments
     const _Float16* P = p.P + b * p.P_b + i0 / 16 * along;
     const _Float16* Q = p.Q + b * p.Q_b + j0 / 16 * along;
     auto copy = [&](int f, int k, int stage) {
         const int piece = f * 4 + wave, r = piece >> 1, plane = piece & 1;
-        const _Float16* from = (r < 16 ? P + r * along : Q + (r - 16) * along) + ((int64_t)k * STEP_SIZE + plane * (STEP_SIZE / 2));
+        const _Float16* from = (r < 16 ? P + r * along : Q + (r - 16) * along) + ((int64_t)k * FRAG + plane * (FRAG / 2));
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from + lane * 8), (__attribute__((address_space(3))) void*)(lds + stage * STAGE + piece * 1024), 16, 0, 0);
     };
     struct fragment { half8 h, l; };
@@ -439,16 +435,11 @@ __device__ __forceinline__ void wide_tile(const product& p, int i0, int j0, char
             }
             const fragment& r = row[i & 3];
 #pragma unroll
-            for (int j = 0; j < TN; ++j) {
-                float4_& sum = COARSE ? acc[i][j] : small[i][j];
-                sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(r.h, COARSE ? col[j].h : col[j].l, sum, 0, 0, 0);          // (coarse: the earlier of the two steps first, as in product_tile)
-            }
-            if constexpr (!COARSE) {
+            for (int j = 0; j < TN; ++j) small[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(r.h, col[j].l, small[i][j], 0, 0, 0);
 #pragma unroll
-                for (int j = 0; j < TN; ++j) small[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(r.l, col[j].h, small[i][j], 0, 0, 0);
-            }
+            for (int j = 0; j < TN; ++j) small[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(r.l, col[j].h, small[i][j], 0, 0, 0);
 #pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(COARSE ? r.l : r.h, COARSE ? col[j].l : col[j].h, acc[i][j], 0, 0, 0);
+            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(r.h, col[j].h, acc[i][j], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
         const int was = now;
@@ -471,7 +462,7 @@ __device__ __forceinline__ void wide_tile(const product& p, int i0, int j0, char
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
                 asm volatile("" : "+a"(acc[i][j]));
-                if constexpr (!COARSE) asm volatile("" : "+a"(small[i][j]));
+                asm volatile("" : "+a"(small[i][j]));
             }
     };
     pin();
@@ -490,7 +481,7 @@ __device__ __forceinline__ void wide_tile(const product& p, int i0, int j0, char
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) tile[(wi * 128 + i * 16 + (lane >> 4) * 4 + r) * PITCH + wj * 64 + j * 16 + (lane & 15)] = COARSE ? acc[i][j][r] : acc[i][j][r] + small[i][j][r];
+            for (int r = 0; r < 4; ++r) tile[(wi * 128 + i * 16 + (lane >> 4) * 4 + r) * PITCH + wj * 64 + j * 16 + (lane & 15)] = acc[i][j][r] + small[i][j][r];
     __syncthreads();
     finish<256, 128, 4, MODE>(p, tile, i0, j0);
 }
@@ -499,7 +490,7 @@ __device__ __forceinline__ void wide_tile(const product& p, int i0, int j0, char
 // cut into four.  Workgroups go round the eight dies by their index: each die gets a run of neighbouring tiles, so that its L2 cache
 // serves their common operands.  2 x 1031 x 4099: A 55, Q 19, Q X 65 us, the latter 815 TFLOP/s of 16-bit products (1031 is padded to 1152,
 // and its last round is short).
-template <int MODE, bool COARSE>
+template <int MODE>
 __global__ __launch_bounds__(256, 2) void k_orth_product(product p) {
     typedef staged<128, 128, 64, 64, 2> big;
     __shared__ __attribute__((aligned(16))) char lds[big::BYTES];
@@ -517,11 +508,11 @@ __global__ __launch_bounds__(256, 2) void k_orth_product(product p) {
         const int band = t / (8 * p.tiles_j), r = t - band * 8 * p.tiles_j, rows = min(8, p.tiles_i - band * 8);
         ti = band * 8 + r % rows; tj = r / rows;
     }
-    if (quarter < 0) product_tile<128, 128, 64, 64, 2, MODE, COARSE>(p, ti * 128, tj * 128, lds);
+    if (quarter < 0) product_tile<128, 128, 64, 64, 2, MODE>(p, ti * 128, tj * 128, lds);
     else {
         ti = ti * 2 + (quarter >> 1); tj = tj * 2 + (quarter & 1);
         if (HALF && tj > ti) return;
-        product_tile<64, 64, 32, 32, 4, MODE, COARSE>(p, ti * 64, tj * 64, lds);
+        product_tile<64, 64, 32, 32, 4, MODE>(p, ti * 64, tj * 64, lds);
     }
 }
 
@@ -529,7 +520,7 @@ __global__ __launch_bounds__(256, 2) void k_orth_product(product p) {
 // products; with 64 x 64 it is 16 for 48, and LDS is what they wait for.  `whole` tiles, the rest of them in 64 x 64, and 64 x 64 for
 // the last 128 rows where the padded short side is an odd multiple of 128.  4096 x 8192: A 363, Q 193, Q X 630 us, the latter 1310 TFLOP/s of
 // 16-bit products, the rate of the library's large product of 16-bit matrices: bound by the matrix cores (and by what power they may draw).
-template <int MODE, bool COARSE>
+template <int MODE>
 __global__ __launch_bounds__(256, 1) void k_orth_wide(product p) {
     typedef staged<256, 128, 128, 64, 3> big;
     __shared__ __attribute__((aligned(16))) char lds[big::BYTES];
@@ -540,7 +531,7 @@ __global__ __launch_bounds__(256, 1) void k_orth_wide(product p) {
         t -= p.whole + cut;
         ti = p.tiles_i * 4 + (t & 1); tj = t >> 1;
         if (HALF && tj > ti) return;
-        return product_tile<64, 64, 32, 32, 8, MODE, COARSE>(p, ti * 64, tj * 64, lds);
+        return product_tile<64, 64, 32, 32, 8, MODE>(p, ti * 64, tj * 64, lds);
     }
     int part = -1;
     if (t < p.whole) {
@@ -559,10 +550,10 @@ __global__ __launch_bounds__(256, 1) void k_orth_wide(product p) {
         const int band = t / (4 * p.tiles_j), r = t - band * 4 * p.tiles_j, rows = min(4, p.tiles_i - band * 4);
         ti = band * 4 + r % rows; tj = r / rows;
     }
-    if (part < 0) return wide_tile<MODE, COARSE>(p, ti * 256, tj * 128, lds);
+    if (part < 0) return wide_tile<MODE>(p, ti * 256, tj * 128, lds);
     ti = ti * 4 + (part >> 1); tj = tj * 2 + (part & 1);
     if (HALF && tj > ti) return;
-    product_tile<64, 64, 32, 32, 8, MODE, COARSE>(p, ti * 64, tj * 64, lds);
+    product_tile<64, 64, 32, 32, 8, MODE>(p, ti * 64, tj * 64, lds);
 }
 
 // ---- the same products where there are too few tiles, or too few steps along k, to fill the chip with staged ones ----------------------

@@ -52,7 +52,7 @@ def orthogonalise(g, steps=5, coefficients=COEFFICIENTS, out=None):
     may be g).  Not differentiable: it makes an update, not an activation.
 
     Operands are held to 22 bits (short sides of up to 16: to 32 in all products but X X') and summed in 32, for every type of g: a step multiplies what is lost in the directions of small
-    singular values by a, five steps by 485.  (The last step of a large bfloat16 result, which holds 8 bits, takes operands of 11.)  The coefficients have to keep X's entries below 60 (the default ones: 1.3)."""
+    singular values by a, five steps by 485.  The coefficients have to keep X's entries below 60 (the default ones: 1.3)."""
     _matrix('orthogonalise', 'g', g, tuple(ll.DTYPES))
     _coefficients('orthogonalise', steps, coefficients)
     ll.require_device('orthogonalise', g, out)

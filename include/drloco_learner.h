@@ -89,8 +89,7 @@ int dl_memory_step(const dl_memory_shape* shape, const void* x, const void* gate
  *     X = U / |U|_F   (zeros stay zeros);   steps times:  A = X X',  X = (a I + b A + c A A) X      from the short side
  *     out = weight_keep * weight + gain * X               weight == NULL: out = gain * X
  *
- * Products are exact to about 2^-22 of their operands (the last step's of a bfloat16 out that is larger than a few hundred a side: 2^-11) and
- * summed in 32 bits, norms in 64; out is rounded once.  A NaN or an
+ * Products are exact to about 2^-22 of their operands and summed in 32 bits, norms in 64; out is rounded once.  A NaN or an
  * infinity anywhere in U makes the whole of its matrix NaN.  The coefficients have to keep every iterate's entries below
  * 60 in size (those of the Muon optimiser, 3.4445 -4.7750 2.0315, and of the classic cubic, 1.5 -0.5 0, keep them
  * below 1.3).  Strides are in elements: of a matrix in its batch and of a row; rows are contiguous. */

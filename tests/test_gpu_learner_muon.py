@@ -473,3 +473,22 @@ def test_long_sides_beyond_the_slabs(rows, cols, dtype):
     from drloco_amd.muon import orthogonalise
     g = gradient(rows, cols, seed=11, dtype=dtype)
     check_orthogonal(orthogonalise(g.cuda()), g)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize('shape', [(8, 512), (512, 29), (20, 1500), (64, 9000), (300, 300), (100, 6000), (700, 900), (1500, 1700), (2050, 1300), (2, 1031, 4099), (4, 1024, 2048), (2170, 4090)], ids=str)
+def test_16_bit_results_are_the_32_bit_ones_rounded_once(shape, dtype):
+    """The type of a result says how it leaves, not how it is computed: on every kernel it is the float32 result of the same input, rounded to nearest
+    (half a step of the type; of float16 half its smallest number too).  A float32 sum that is rounded to float16 at once may differ from
+    one that was a float32 number in between by the half step of that, 2^-24."""
+    from drloco_amd.muon import muon_update, orthogonalise
+    w, g, m = (gradient(*shape, seed=s, dtype=t).cuda() for s, t in ((1, dtype), (2, dtype), (3, torch.float32)))
+    w = w / 64          # (small against lr times the factor's entries)
+    pairs = [(orthogonalise(g), orthogonalise(g.float())), (orthogonalise(g, 1), orthogonalise(g.float(), 1)),
+             (muon_update(w, g, m, lr=0.1, weight_decay=0.1)[0], muon_update(w.float(), g, m, lr=0.1, weight_decay=0.1)[0])]
+    for got, full in pairs:
+        assert got.dtype == dtype and full.dtype == torch.float32
+        if dtype == torch.bfloat16:
+            assert torch.equal(got, full.to(dtype))
+        else:
+            assert bool(((got.double() - full.double()).abs() <= torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -12) * full.double().abs() + 2.0 ** -25).all())
