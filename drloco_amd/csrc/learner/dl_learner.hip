@@ -2,6 +2,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <algorithm>
+#include <cmath>
 #include <string>
 
 #include "drloco_learner.h"
@@ -120,6 +121,32 @@ const char* orth_shape_error(const dl_orth_shape* s) {
     for (int64_t st : {s->grad_b, s->grad_r, s->momentum_b, s->momentum_r, s->momentum_out_b, s->momentum_out_r, s->weight_b, s->weight_r, s->out_b, s->out_r})
         if (st < 0) return "negative strides";
     return nullptr;
+}
+
+// What the planes hold (dl_orth.hpp) times 2^10, and float16 only up to 65504: X, A = X X' and Q = a I + b A + c A A of every step.  An entry is at most
+// the largest singular value.  X's lie in [0, 1] at first, and a step takes s to s q(s^2), q(u) = a + b u + c u^2; the largest of either is at an end of
+// the interval or where a derivative is zero.
+constexpr double MOST = 60.0;
+bool coefficients_hold(int steps, double a, double b, double c) {
+    auto q = [&](double u) { return a + u * (b + u * c); };
+    double s = 1.0;          // the largest singular value there may be
+    for (int k = 0; k < steps; ++k) {
+        const double u1 = s * s;
+        auto inside = [&](double u) { return u > 0.0 && u < u1; };
+        double most_q = std::max(std::fabs(q(0.0)), std::fabs(q(u1)));
+        const double top = -b / (2.0 * c);
+        if (inside(top)) most_q = std::max(most_q, std::fabs(q(top)));
+        if (!(s < MOST && u1 < MOST && most_q < MOST)) return false;
+        double next = s * std::fabs(q(u1));
+        const double root = 9.0 * b * b - 20.0 * a * c;          // a + 3 b u + 5 c u^2 = 0
+        if (root >= 0.0) {
+            const double t = -0.5 * (3.0 * b + std::copysign(std::sqrt(root), b));
+            for (double u : {t / (5.0 * c), a / t})
+                if (inside(u)) next = std::max(next, std::sqrt(u) * std::fabs(q(u)));
+        }
+        s = next;
+    }
+    return true;
 }
 
 struct orth_form {
@@ -326,6 +353,12 @@ int dl_memory_step(const dl_memory_shape* s, const void* x, const void* gate, co
     return launched("dl_memory_step");
 }
 
+int dl_orth_check_coefficients(int32_t steps, double a, double b, double c) {
+    if (steps < 1 || steps > 100) return fail(DL_E_INVAL, "steps must be 1 .. 100");
+    if (!coefficients_hold(steps, a, b, c)) return fail(DL_E_INVAL, "the coefficients let X, X X' or a I + b X X' + c (X X')^2 grow to 60 or more within these steps");
+    return DL_OK;
+}
+
 int64_t dl_orth_workspace_bytes(const dl_orth_shape* s) {
     if (const char* e = orth_shape_error(s)) return fail(DL_E_INVAL, e);
     if (s->batch == 0 || s->rows == 0 || s->cols == 0) return 0;
@@ -336,6 +369,7 @@ int64_t dl_orth_workspace_bytes(const dl_orth_shape* s) {
 int dl_orth_update(const dl_orth_shape* s, const void* grad, const float* momentum, float* momentum_out, const void* weight, void* out, void* workspace, void* stream) {
     if (const char* e = orth_shape_error(s)) return fail(DL_E_INVAL, e);
     if (s->batch == 0 || s->rows == 0 || s->cols == 0) return DL_OK;
+    if (const int e = dl_orth_check_coefficients(s->steps, s->a, s->b, s->c)) return e;
     if (!grad || !out) return fail(DL_E_INVAL, "dl_orth_update: grad and out must not be NULL");
     if (!momentum != !momentum_out) return fail(DL_E_INVAL, "dl_orth_update: momentum and momentum_out must be given together");
     if (dl_orth_workspace_bytes(s) > 0 && !workspace) return fail(DL_E_INVAL, "dl_orth_update: workspace must not be NULL (dl_orth_workspace_bytes)");

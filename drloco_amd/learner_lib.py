@@ -43,6 +43,7 @@ _SIGNATURES = {
     'dl_memory_forward': (C.c_int, [C.POINTER(MemoryShape), _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     'dl_memory_backward': (C.c_int, [C.POINTER(MemoryShape), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P]),
     'dl_memory_step': (C.c_int, [C.POINTER(MemoryShape), _P, _P, _P, _P, _P, _P, _P]),
+    'dl_orth_check_coefficients': (C.c_int, [_I32, C.c_double, C.c_double, C.c_double]),
     'dl_orth_workspace_bytes': (_I64, [C.POINTER(OrthShape)]),
     'dl_orth_update': (C.c_int, [C.POINTER(OrthShape), _P, _P, _P, _P, _P, _P, _P]),
 }

@@ -4,6 +4,7 @@ the matrix cores, next to the Adam steps the reference takes (drloco/train.py:11
     orthogonalise(g)       the orthogonal factor of a gradient, by Newton-Schulz products
     muon_update(w, g, m)   momentum, orthogonalisation and the new weight in one call
     HipMuon                a torch optimiser of matrices built on it; vectors (biases, log_std) stay with Adam"""
+import functools
 import math
 
 import torch
@@ -28,6 +29,15 @@ def _coefficients(name, steps, coefficients):
         raise ValueError(f'{name}: steps must be 1 .. 100, got {steps}')
     if len(coefficients) != 3 or not all(math.isfinite(c) for c in coefficients):
         raise ValueError(f'{name}: coefficients must be three finite numbers, got {coefficients}')
+    refused = _refused(int(steps), *(float(c) for c in coefficients))
+    if refused:
+        raise ValueError(f'{name}: {refused}, got {coefficients}')
+
+
+@functools.lru_cache(maxsize=None)
+def _refused(steps, a, b, c):
+    L = ll.load()
+    return L.dl_learner_last_error().decode() if L.dl_orth_check_coefficients(steps, a, b, c) < 0 else None
 
 
 def _result(name, what, t, like, dtype, aliases):
@@ -52,7 +62,8 @@ def orthogonalise(g, steps=5, coefficients=COEFFICIENTS, out=None):
     may be g).  Not differentiable: it makes an update, not an activation.
 
     Operands are held to 22 bits (short sides of up to 16: to 32 in all products but X X') and summed in 32, for every type of g: a step multiplies what is lost in the directions of small
-    singular values by a, five steps by 485.  The coefficients have to keep X's entries below 60 (the default ones: 1.3)."""
+    singular values by a, five steps by 485.  Coefficients that let X, X X' or a + b X X' + c (X X')^2
+    grow to 60 or more (default ones: 3.5) are refused."""
     _matrix('orthogonalise', 'g', g, tuple(ll.DTYPES))
     _coefficients('orthogonalise', steps, coefficients)
     ll.require_device('orthogonalise', g, out)

@@ -90,9 +90,9 @@ int dl_memory_step(const dl_memory_shape* shape, const void* x, const void* gate
  *     out = weight_keep * weight + gain * X               weight == NULL: out = gain * X
  *
  * Products are exact to about 2^-22 of their operands and summed in 32 bits, norms in 64; out is rounded once.  A NaN or an
- * infinity anywhere in U makes the whole of its matrix NaN.  The coefficients have to keep every iterate's entries below
- * 60 in size (those of the Muon optimiser, 3.4445 -4.7750 2.0315, and of the classic cubic, 1.5 -0.5 0, keep them
- * below 1.3).  Strides are in elements: of a matrix in its batch and of a row; rows are contiguous. */
+ * infinity anywhere in U makes the whole of its matrix NaN.  The coefficients have to keep X, A and a I + b A + c A A
+ * of every step below 60 in size, whatever singular values in [0, 1] a matrix has (those of the Muon optimiser, 3.4445 -4.7750 2.0315, and of
+ * the classic cubic, 1.5 -0.5 0, keep them below 3.5); dl_orth_update refuses others.  Strides are in elements: of a matrix in its batch and of a row; rows are contiguous. */
 typedef struct dl_orth_shape {
     int64_t batch, rows, cols;
     int64_t grad_b, grad_r;
@@ -105,6 +105,9 @@ typedef struct dl_orth_shape {
     int32_t steps, nesterov;
     int32_t grad_type, weight_type, out_type, reserved;
 } dl_orth_shape;
+
+/* DL_OK if `steps` steps with these coefficients stay in that range, or DL_E_INVAL. */
+int dl_orth_check_coefficients(int32_t steps, double a, double b, double c);
 
 /* Bytes of device workspace dl_orth_update needs for this shape, or a DL_E_ code. */
 int64_t dl_orth_workspace_bytes(const dl_orth_shape* shape);

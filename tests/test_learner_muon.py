@@ -129,3 +129,52 @@ def test_a_first_step_is_not_captured(monkeypatch):
     with pytest.raises(RuntimeError, match='before it is captured'):
         opt.step()
     assert not opt.state[p]
+
+
+def grows(steps, a, b, c):
+    """The largest |s|, s^2 and |q(s^2)| over singular values 0 .. 1 on a fine grid, before each of the steps."""
+    import numpy as np
+    s, most = np.linspace(0.0, 1.0, 200001), 0.0
+    for _ in range(steps):
+        q = a + b * s ** 2 + c * s ** 4
+        with np.errstate(over='ignore', invalid='ignore'):
+            most = max(most, np.abs(s).max(), (s ** 2).max(), np.abs(q).max())
+        # (every value up to the largest may be a singular value)
+        s = np.linspace(0.0, np.abs(s * q).max(), 200001)
+        if not most < 1e6:
+            return 1e6
+    return most
+
+
+COEFS = [(5, muon.COEFFICIENTS), (100, muon.COEFFICIENTS), (5, muon.CUBIC), (100, muon.CUBIC), (1, (59.9, 0.0, 0.0)), (1, (60.1, 0.0, 0.0)), (1, (64.0, -64.0, 0.0)), (1, (1.0, -61.5, 0.0)), (1, (0.0, 100.0, -100.0)),
+         (1, (0.0, 300.0, -300.0)), (2, (7.7, 0.0, 0.0)), (2, (7.8, 0.0, 0.0)), (5, (3.0, -4.0, 2.0)), (4, (3.0, -4.0, 2.0)), (3, (8.287, -23.596, 17.3)), (5, (2.0, -1.5, 0.5)), (1, (0.0, 0.0, 0.0)),
+         (1, (1e300, 1.0, 1.0)), (2, (1.0, 1e200, -1e200)), (5, (1.875, -1.25, 0.375)), (7, (0.0, 0.0, 1.0)), (3, (-3.4445, 4.775, -2.0315))]
+
+
+@pytest.mark.parametrize('steps,coefficients', COEFS, ids=str)
+def test_coefficients_that_leave_the_range_are_refused(L, steps, coefficients):
+    """float16 planes times 2^10 end at 63.97: what grows to 60 is refused, by the C entry points and the Python ones alike"""
+    fits = grows(steps, *coefficients) < 60
+    a, b, c = coefficients
+    assert L.dl_orth_check_coefficients(steps, a, b, c) == (0 if fits else -1)
+    s = shape(steps=steps, a=a, b=b, c=c)
+    assert L.dl_orth_update(C.byref(s), None, None, None, None, None, None, None) == -1
+    assert (b'coefficients' in L.dl_learner_last_error()) == (not fits)
+    make = lambda: muon.HipMuon([torch.nn.Parameter(z(4, 4))], steps=steps, coefficients=coefficients)
+    if fits:
+        make()
+        with pytest.raises(lib.DrlocoError):          # (nothing wrong but the device)
+            muon.orthogonalise(z(2, 2), steps, coefficients)
+    else:
+        for call in (make, lambda: muon.orthogonalise(z(2, 2), steps, coefficients), lambda: muon.muon_update(z(2, 2), z(2, 2), z(2, 2), lr=0.1, steps=steps, coefficients=coefficients)):
+            with pytest.raises(ValueError):
+                call()
+
+
+def test_coefficients_that_are_no_numbers_are_refused(L):
+    for bad in (math.nan, math.inf, -math.inf):
+        for k in range(3):
+            cs = [1.5, -0.5, 0.1]
+            cs[k] = bad
+            assert L.dl_orth_check_coefficients(1, *cs) == -1
+    assert L.dl_orth_check_coefficients(0, 1.5, -0.5, 0.0) == -1 and L.dl_orth_check_coefficients(101, 1.5, -0.5, 0.0) == -1
