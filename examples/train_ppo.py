@@ -152,8 +152,10 @@ def train(mio=2.0, n_envs=128, batch=16384, minibatch=2048, epochs=4, seed=0, lo
         os.makedirs(os.path.join(save_path, 'models'), exist_ok=True); os.makedirs(os.path.join(save_path, 'envs'), exist_ok=True)
         ckpt = f'{int(total / 1e5)}'
         # SB3 1.0's save_to_zip_file layout: data (spaces, policy class, hyperparameters), policy.pth, policy.optimizer.pth (Adam's moments)
-        checkpoint.write_model_zip(pol, os.path.join(save_path, 'models', f'model_{ckpt}.zip'), observation_space=venv.observation_space, action_space=venv.action_space, optimizer=opt if muon is None else None,
+        checkpoint.write_model_zip(pol, os.path.join(save_path, 'models', f'model_{ckpt}.zip'), observation_space=venv.observation_space, action_space=venv.action_space, optimizer=opt,
                                    hyper=dict(n_envs=n_envs, num_timesteps=int(total), n_steps=batch // n_envs, batch_size=minibatch, n_epochs=epochs, learning_rate=float(lr)))
+        if muon is not None:          # (the zip holds what SB3 knows: Adam's moments, of the parameters that are Adam's)
+            torch.save(muon.state_dict(), os.path.join(save_path, 'models', f'muon_{ckpt}.pth'))
         vn.save(os.path.join(save_path, 'envs', f'env_{ckpt}'), sb3_format=True)
         if not quiet:
             print('saved', os.path.join(save_path, 'models', f'model_{ckpt}.zip'), 'and', os.path.join(save_path, 'envs', f'env_{ckpt}'))
@@ -172,7 +174,7 @@ if __name__ == '__main__':
     ap.add_argument('--save', default=None, help='directory for models/model_<ckpt>.zip (policy.pth with SB3 1.0 key names) and envs/env_<ckpt> (VecNormalize statistics), drloco_amd/checkpoint.py')
     ap.add_argument('--no-norm-reward', action='store_true', help='VecNormalize(norm_reward=False)')
     ap.add_argument('--moments', choices=['per_step', 'per_rollout'], default='per_step', help="VecNormalize moments inside a rollout: SB3's per-step update (default) or the opt-in per-rollout relaxation of the persistent rollout kernel")
-    ap.add_argument('--optimizer', choices=['adam', 'muon'], default='adam', help="the reference's Adam (default), or Muon (drloco_amd.muon.HipMuon) for the trunk's two matrices and Adam for the rest; a saved model then has no optimiser state")
+    ap.add_argument('--optimizer', choices=['adam', 'muon'], default='adam', help="the reference's Adam (default), or Muon (drloco_amd.muon.HipMuon) for the trunk's two matrices and Adam for the rest; a saved model then holds Adam's moments of the rest, and models/muon_<ckpt>.pth beside it Muon's momenta")
     ap.add_argument('--muon-lr', type=float, default=0.01, help='Muon: learning rate of the matrices at the start, decays as the other')
     args = ap.parse_args()
     train(args.mio, args.envs, batch=args.batch, minibatch=args.minibatch, seed=args.seed, norm_reward=not args.no_norm_reward, evaluate=True, save_path=args.save, moments=args.moments, optimizer=args.optimizer, muon_lr=args.muon_lr)

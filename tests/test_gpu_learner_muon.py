@@ -492,3 +492,30 @@ def test_16_bit_results_are_the_32_bit_ones_rounded_once(shape, dtype):
             assert torch.equal(got, full.to(dtype))
         else:
             assert bool(((got.double() - full.double()).abs() <= torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -12) * full.double().abs() + 2.0 ** -25).all())
+
+
+def test_the_training_example_saves_both_optimisers(tmp_path):
+    """--optimizer muon --save: Adam's moments of its seven parameters in the zip, the momenta of the trunk's two matrices beside it, both ready to be loaded"""
+    import importlib.util
+    import io
+    import os
+    import zipfile
+    from drloco_amd import checkpoint
+    from drloco_amd.muon import HipMuon
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'examples', 'train_ppo.py')
+    spec = importlib.util.spec_from_file_location('train_ppo', path)
+    mod = importlib.util.module_from_spec(spec); spec.loader.exec_module(mod)
+    pol = mod.train(mio=1100e-6, n_envs=64, batch=512, minibatch=256, epochs=1, seed=1, log_every=1, quiet=True, return_objects=True, optimizer='muon', save_path=str(tmp_path))[1]
+    names = sorted(os.listdir(tmp_path / 'models'))
+    assert [n.split('_')[0] for n in names] == ['model', 'muon']
+    with zipfile.ZipFile(tmp_path / 'models' / names[0]) as z:
+        adam = torch.load(io.BytesIO(z.read('policy.optimizer.pth')), weights_only=True)
+    order = list(checkpoint._PARAM_ORDER)
+    assert sorted(order[i] for i in adam['state']) == sorted(set(order) - {'w1', 'w2'})
+    assert all(bool(torch.isfinite(s['exp_avg']).all()) and float(s['step']) > 0 for s in adam['state'].values())
+    params = [torch.nn.Parameter(getattr(pol, n).detach().clone()) for n in ('w1', 'w2')]
+    opt = HipMuon(params)
+    opt.load_state_dict(torch.load(tmp_path / 'models' / names[1], weights_only=True))
+    for p in params:
+        m = opt.state[p]['momentum']
+        assert m.shape == p.shape and m.dtype == torch.float32 and float(m.abs().sum()) > 0
