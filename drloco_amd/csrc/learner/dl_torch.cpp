@@ -9,6 +9,8 @@
 
 #include <cmath>
 #include <optional>
+#include <stdexcept>
+#include <string>
 #include <tuple>
 #include <vector>
 
@@ -22,8 +24,9 @@ typedef std::optional<Tensor> Maybe;
 int type_of(at::ScalarType t) { return t == at::kFloat ? DL_F32 : t == at::kBFloat16 ? DL_BF16 : t == at::kHalf ? DL_F16 : -1; }
 const void* ptr(const Maybe& t) { return t ? t->data_ptr() : nullptr; }
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+struct Failed : std::runtime_error { using std::runtime_error::runtime_error; };          // DrlocoError in Python
 int64_t check(int64_t rc) {
-    TORCH_CHECK(rc >= 0, "drloco_learner error ", rc, ": ", dl_learner_last_error());
+    if (rc < 0) throw Failed("drloco_learner error " + std::to_string(rc) + ": " + dl_learner_last_error());
     return rc;
 }
 Tensor floats(const Tensor& like, at::IntArrayRef shape) { return at::empty(shape, like.options().dtype(at::kFloat)); }
@@ -199,6 +202,13 @@ void orth_update(const Tensor& grad, const Maybe& momentum, const Maybe& momentu
 }  // namespace
 
 PYBIND11_MODULE(dl_learner_torch, m) {
+    py::register_local_exception_translator([](std::exception_ptr p) {
+        try {
+            if (p) std::rethrow_exception(p);
+        } catch (const Failed& e) {
+            PyErr_SetString(py::module_::import("drloco_amd.lib").attr("DrlocoError").ptr(), e.what());
+        }
+    });
     m.def("gated_memory", &gated_memory);
     m.def("gated_memory_step", &gated_memory_step);
     m.def("orth_update", &orth_update);

@@ -519,3 +519,14 @@ def test_the_training_example_saves_both_optimisers(tmp_path):
     for p in params:
         m = opt.state[p]['momentum']
         assert m.shape == p.shape and m.dtype == torch.float32 and float(m.abs().sum()) > 0
+
+
+def test_what_the_library_refuses_is_a_drloco_error():
+    """as everywhere in the package: here more matrices than a launch takes"""
+    from drloco_amd import lib
+    from drloco_amd.muon import muon_update, orthogonalise
+    many = torch.zeros(1, 2, 2, device='cuda').expand(65536, 2, 2)
+    with pytest.raises(lib.DrlocoError, match='65535'):
+        orthogonalise(many)
+    with pytest.raises(lib.DrlocoError, match='65535'):
+        muon_update(many, many, many, lr=0.1)
