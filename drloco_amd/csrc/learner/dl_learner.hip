@@ -167,7 +167,7 @@ orth_form orth_plan(const dl_orth_shape* s) {
     f.p.n = (int32_t)std::max(s->rows, s->cols);
     f.small = f.p.n <= (f.p.m <= 16 ? 1024 : f.p.m <= 32 ? 512 : f.p.m <= 64 ? 256 : 0);          // what a workgroup's LDS and registers hold
     // Short sides of up to 64: a slab of 512 columns (up to 32 rows) or 256 per workgroup; from 256 slabs on the sums over them weigh more
-    // than the launches they save.
+    // than the launches they save (and the products of up to 16 rows are those of 22-bit operands, as for larger matrices).
     f.slab_rows = f.p.m <= 16 ? 1 : f.p.m <= 32 ? 2 : 4;
     f.slab_cols = f.slab_rows == 4 ? 256 : 512;
     f.n_slabs = ceil_div(f.p.n, f.slab_cols);

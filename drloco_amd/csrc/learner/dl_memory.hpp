@@ -239,7 +239,7 @@ struct yes { static constexpr bool value = true; };
 struct no { static constexpr bool value = false; };
 
 // ---- whole: a wave runs through all steps, half a run ahead with its loads --------------------------------------------------------------
-// 512 x 4096 x 128 bf16 with marks: 1.68 GB in 350 us, 4.8 TB/s, what a large copy reaches; bound by memory.
+// 512 x 4096 x 128 bf16 with marks: 1.68 GB in 355 us, 4.7 TB/s, what a large copy reaches; bound by memory.
 template <typename E, int V>
 __global__ __launch_bounds__(64) void k_memory_run(shape s, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ state,
                                                    E* __restrict__ h, float* __restrict__ state_out, float* __restrict__ marks) {
@@ -392,9 +392,9 @@ template <int V, bool BACK> __device__ __forceinline__ void leave(const chain& c
 }
 
 // ---- short: W waves of a workgroup take one run each ----------------------------------------------------------------------------------
-// 128 x 128 x 512 bf16: 52 MB in 16.6 us, 3.1 TB/s: a wave has one run, nothing is loaded meanwhile.  Chains: 2048 x 8 x 512
-// float32, 103 MB in 31.7 us, 3.2 TB/s; 3000 x 20 x 256 float32, 184 MB in 43 us, 4.2 TB/s; 100003 x 333 float16, 200 MB in 106 us, 1.9 TB/s:
-// there 782 workgroups wait along one chain, in 13 groups, and the vector units are the busiest part.
+// 128 x 128 x 512 bf16: 52 MB in 17.6 us, 3.0 TB/s: a wave has one run, nothing is loaded meanwhile (vector units 0.69 busy).  Chains: 2048 x 8 x 512
+// float32, 103 MB in 33 us, 3.1 TB/s; 3000 x 20 x 256 float32, 184 MB in 45 us, 4.1 TB/s; 100003 x 333 float16, 200 MB in 106 us, 1.9 TB/s:
+// there 782 workgroups wait along one chain, in 13 groups that follow each other; waves wait 0.56 of their time, the vector units are 0.56 busy.
 template <typename E, int V, int W, bool CHAIN>
 __global__ __launch_bounds__(64 * W) void k_memory_short(shape s, chain ch, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ state,
                                                          E* __restrict__ h, float* __restrict__ state_out, float* __restrict__ marks) {
@@ -504,7 +504,7 @@ template <typename E, int V> struct run_back {
     }
 };
 
-// whole: a wave runs back through all steps, a run ahead with its loads.  512 x 4096 x 128 bf16: 2.75 GB in 605 us, 4.6 TB/s; bound by memory.
+// whole: a wave runs back through all steps, a run ahead with its loads.  512 x 4096 x 128 bf16: 2.75 GB in 600 us, 4.6 TB/s; bound by memory.
 template <typename E, int V>
 __global__ __launch_bounds__(64) void k_memory_run_back(shape s, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ marks,
                                                             const E* __restrict__ grad_h, const float* __restrict__ grad_state, E* __restrict__ dx, E* __restrict__ dgate, float* __restrict__ dstate) {
@@ -536,7 +536,7 @@ __global__ __launch_bounds__(64) void k_memory_run_back(shape s, const E* __rest
     if (dstate && c.valid) store_floats<V>(dstate + corner, floats, in);
 }
 
-// short and chain, back: 128 x 128 x 512 bf16: 86 MB in 28.8 us, 3.0 TB/s, bound by its arithmetic; 2048 x 8 x 512 float32: 170 MB in 38.8 us, 4.4 TB/s.
+// short and chain, back: 128 x 128 x 512 bf16: 86 MB in 28.8 us, 3.0 TB/s, two waves per SIMD unit with a run each, vector units 0.50 busy; 2048 x 8 x 512 float32: 170 MB in 40 us, 4.2 TB/s.
 template <typename E, int V, int W, bool CHAIN>
 __global__ __launch_bounds__(64 * W) void k_memory_short_back(shape s, chain ch, const E* __restrict__ x, const E* __restrict__ gate, const uint8_t* __restrict__ starts, const float* __restrict__ marks,
                                                               const E* __restrict__ grad_h, const float* __restrict__ grad_state, E* __restrict__ dx, E* __restrict__ dgate, float* __restrict__ dstate) {
@@ -584,7 +584,7 @@ __global__ __launch_bounds__(64 * W) void k_memory_short_back(shape s, chain ch,
 }
 
 // One control step.  state_out may be state: a thread reads its own columns, which are no other's, before it writes them.
-// 8 x 512 float32: 3.0 us, a launch; 4096 x 512 bf16: 29 MB in 5.2 us, 5.7 TB/s from the last-level cache.
+// 8 x 512 float32: 2.6 to 2.8 us, a launch; 4096 x 512 bf16: 29 MB in 5.0 to 5.3 us, 5.5 TB/s and more from the last-level cache.
 template <typename E, int V>
 __global__ __launch_bounds__(256) void k_memory_step(int64_t N, int64_t D, int64_t x_n, int64_t gate_n, int64_t starts_n, const E* __restrict__ x, const E* __restrict__ gate,
                                                      const uint8_t* __restrict__ starts, const float* state, E* __restrict__ h, float* state_out) {

@@ -109,7 +109,7 @@ struct place {
 };
 
 // rows x cols as they are read: one long row where the rows of all arrays follow each other
-// (and counters for later kernels to zero).  4096 x 8192 bf16: 67 MB in 32 us, 2.1 TB/s, half of what memory gives; 0.6 % of the update.
+// (and counters for later kernels to zero).  4096 x 8192 bf16: 67 MB in 32 us, 2.1 TB/s, half of what memory gives; 0.5 % of the update.
 __global__ __launch_bounds__(256) void k_orth_norm(source s, int64_t rows, int64_t cols, double* __restrict__ partials, uint32_t* __restrict__ counters, int n_counters) {
     if (blockIdx.x == 0 && blockIdx.y == 0) for (int k = threadIdx.x; k < n_counters; k += 256) counters[k] = 0;
     constexpr int AT_ONCE = 4;
@@ -138,7 +138,7 @@ __global__ __launch_bounds__(256) void k_orth_norm(source s, int64_t rows, int64
 }
 
 // ---- X = G / |G| into both orientations: one workgroup per 64 x 64 ---------------------------------------------------------------
-// 4096 x 8192 bf16: 335 MB in 80 us, 4.2 TB/s; bound by memory.
+// 4096 x 8192 bf16: 335 MB in 76 to 81 us, 4.1 to 4.4 TB/s; bound by memory.
 __global__ __launch_bounds__(256) void k_orth_load(source s, plan p, int turned, const double* __restrict__ partials, _Float16* __restrict__ xr, _Float16* __restrict__ xc) {
     const int b = blockIdx.z, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     __shared__ float tile[64][65];          // [short side][long side]
@@ -488,7 +488,7 @@ __device__ __forceinline__ void wide_tile(const product& p, int i0, int j0, char
 
 // Tiles of 128 x 128, two workgroups per CU; those that would be left for a last round that fills less than two thirds of the chip are
 // cut into four.  Workgroups go round the eight dies by their index: each die gets a run of neighbouring tiles, so that its L2 cache
-// serves their common operands.  2 x 1031 x 4099: A 55, Q 19, Q X 65 us, the latter 815 TFLOP/s of 16-bit products (1031 is padded to 1152,
+// serves their common operands.  2 x 1031 x 4099: A 55, Q 19, Q X 64 to 70 us, the latter 750 to 810 TFLOP/s of 16-bit products (1031 is padded to 1152,
 // and its last round is short).
 template <int MODE>
 __global__ __launch_bounds__(256, 2) void k_orth_product(product p) {
@@ -518,8 +518,8 @@ __global__ __launch_bounds__(256, 2) void k_orth_product(product p) {
 
 // Tiles of 256 x 128, one workgroup per CU, for results that fill the chip with them.  A wave's 128 x 64 need 24 reads of LDS for 96
 // products; with 64 x 64 it is 16 for 48, and LDS is what they wait for.  `whole` tiles, the rest of them in 64 x 64, and 64 x 64 for
-// the last 128 rows where the padded short side is an odd multiple of 128.  4096 x 8192: A 363, Q 193, Q X 630 us, the latter 1310 TFLOP/s of
-// 16-bit products, the rate of the library's large product of 16-bit matrices: bound by the matrix cores (and by what power they may draw).
+// the last 128 rows where the padded short side is an odd multiple of 128.  4096 x 8192: A 366, Q 192, Q X 626 us, 1130, 1070 and 1320 TFLOP/s of
+// 16-bit products; the library's large product of 16-bit matrices reaches 1330 to 1420: bound by the matrix cores, 0.63 to 0.68 busy (and by what power they may draw).
 template <int MODE>
 __global__ __launch_bounds__(256, 1) void k_orth_wide(product p) {
     typedef staged<256, 128, 128, 64, 3> big;
@@ -676,8 +676,9 @@ __global__ __launch_bounds__(512) void k_orth_direct(product p) {
 // are those of the matrix cores' 32-bit instruction, whose operands are the results as they stand: with so few terms to average over, 22 bits
 // in them left 3 x 700 off by up to 3.7 times what 32-bit products are).  Only A = X X', which sums over columns, reads X in its other
 // orientation, from the wave's own part of LDS.  X itself stays in 32 bits: here Q is without its a I, and X = a X + Q X.  Two barriers per step, one with RB = 1, where A's parts are summed.
-// Bound by the instructions of one CU, some 450 per wave and step with RB = 2, JB = 4, and by the way in and out.  8 x 512: 14.6 us (13.4 with 16-bit products throughout, which lost
-// the precision said above), 512 x 29 with momentum and weight: 28.5.
+// Bound by what one CU does in sequence, some 450 instructions per wave and step with RB = 2, JB = 4, and the way in and out (vector units 0.29 and 0.43
+// busy below, waves wait half of their time).  8 x 512: 14.7 us (13.4 with 16-bit products throughout, which lost
+// the precision said above), 512 x 29 with momentum and weight: 29.
 struct small {
     source s;
     int32_t m, n, steps, turned, flat;          // flat: the rows of every array follow each other, they are read as one

@@ -61,8 +61,8 @@ def orthogonalise(g, steps=5, coefficients=COEFFICIENTS, out=None):
     stay zero.  A matrix that holds a NaN or an infinity becomes NaN, the others of the batch do not.  Returns a tensor like g, or writes `out` (which
     may be g).  Not differentiable: it makes an update, not an activation.
 
-    Operands are held to 22 bits (short sides of up to 16: to 32 in all products but X X') and summed in 32, for every type of g: a step multiplies what is lost in the directions of small
-    singular values by a, five steps by 485.  Coefficients that let X, X X' or a + b X X' + c (X X')^2
+    Operands are held to 22 bits (short sides of up to 16 next to long ones of up to 130560: to 32 in all products but X X') and summed in 32, for every type
+    of g; a 16-bit result is the float32 one rounded.  A step multiplies what is lost in the directions of small singular values by a, five steps by 485.  Coefficients that let X, X X' or a + b X X' + c (X X')^2
     grow to 60 or more (default ones: 3.5) are refused."""
     _matrix('orthogonalise', 'g', g, tuple(ll.DTYPES))
     _coefficients('orthogonalise', steps, coefficients)
@@ -111,7 +111,7 @@ def muon_update(weight, grad, momentum, lr, beta=0.95, nesterov=True, weight_dec
 
 class HipMuon(torch.optim.Optimizer):
     """Muon for the weight matrices of a policy, each step one muon_update in place per matrix.  Parameters need at least two axes, contiguous,
-    on a HIP device; everything else (biases, log_std, usually the first and the last layer) belongs to another optimiser.
+    on a HIP device; of more than two axes the last two are the matrices, the others a stack of them (for a convolution's weight, give a [out, rest] parameter); everything else (biases, log_std, usually the first and the last layer) belongs to another optimiser.
     With walkers sharded over GPUs the gradients are summed over the ranks first (collectives.FlatGradAllReducer); every rank then takes the same step.
     step() can be captured into a graph after a first eager one; a replay takes the learning rate that was set at the capture."""
 
