@@ -34,7 +34,7 @@ def _coefficients(name, steps, coefficients):
         raise ValueError(f'{name}: {refused}, got {coefficients}')
 
 
-@functools.lru_cache(maxsize=None)
+@functools.lru_cache
 def _refused(steps, a, b, c):
     L = ll.load()
     return L.dl_learner_last_error().decode() if L.dl_orth_check_coefficients(steps, a, b, c) < 0 else None

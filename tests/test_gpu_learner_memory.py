@@ -451,3 +451,25 @@ def test_the_largest_state_of_a_float16_memory(T, N, D):
     _, last = gated_memory(x.cuda(), gate.cuda(), None, st.cuda())
     _, last_ = R.memory(np64(x), np64(gate), None, np64(st))
     assert torch.isfinite(last).all() and np.all(np.abs(np64(last.cpu()) - last_) <= 12 * U * most * (T + 1)) and torch.equal(last[:, 1].cpu(), st[:, 1])
+
+
+@pytest.mark.parametrize('dtype', TYPES, ids=str)
+def test_a_captured_step_replays(dtype):
+    """a control step in a graph, the state kept in place, replayed over new inputs with eager steps between"""
+    from drloco_amd.memory import gated_memory_step
+    x, gate, b, st, _, _ = (dev(t) for t in make(6, 7, 20, dtype, seed=2))
+    xs, gs, bs, state, eager, out = x[0].clone(), gate[0].clone(), b[0].clone(), st.clone(), st.clone(), torch.empty_like(x[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        gated_memory_step(xs, gs, st, bs)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gated_memory_step(xs, gs, state, bs, out=out, state_out=state)
+    for t in range(6):
+        xs.copy_(x[t]), gs.copy_(gate[t]), bs.copy_(b[t])
+        graph.replay()
+        h, _ = gated_memory_step(x[t], gate[t], eager, b[t], state_out=eager)
+        torch.cuda.synchronize()
+        assert torch.equal(out, h) and torch.equal(state, eager)
