@@ -959,7 +959,7 @@ __global__ __launch_bounds__(512) void k_orth_small(small p) {
 // ---- short sides of up to 64 with a long one: a workgroup per 128 JB columns ("slab"), a launch per step ---------------------------------------
 // Slab s leaves its part of A behind each launch; the next one sums all slabs' parts for itself, makes Q, moves its part of X on.
 // X waits in memory between the launches, in 32 bits and in the order of the lanes.  Seven launches instead of seventeen, each bound by
-// its way to the caches and back.  All five steps of 8 x 8000: 35 us (157 with a launch per product), 30 x 8000: 51, 8 x 100000: 73.
+// its way to the caches and back.  All five steps of 8 x 8000: 35 to 38 us (157 with a launch per product), 30 x 8000: 51, 8 x 100000: 73.
 struct slabs {
     const double* partials; int32_t n_partials;
     float* x;                     // [batch][slab][JB * RB][512 lanes][4]
